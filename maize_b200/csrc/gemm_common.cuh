@@ -266,7 +266,7 @@ struct RepackSegment {
     uint32_t rows;
 };
 
-__global__ void __launch_bounds__(256) repack_rows_kernel(RepackSegment s0, RepackSegment s1, uint32_t cols16)
+static __global__ void __launch_bounds__(256) repack_rows_kernel(RepackSegment s0, RepackSegment s1, uint32_t cols16)
 {
     // a GEMM launched behind this copy with programmatic stream serialization may do its set-up meanwhile (it
     // waits for this grid to complete before it loads anything)
@@ -369,7 +369,7 @@ __device__ __forceinline__ void tma_store_drain(uint32_t lane)
 }
 
 // One CTA waits on a barrier that nothing completes; exercises the bounded wait.
-__global__ void wait_expires_kernel(DeviceStatus *status, uint64_t budget_ns)
+static __global__ void wait_expires_kernel(DeviceStatus *status, uint64_t budget_ns)
 {
     __shared__ __align__(8) uint64_t bar;
     __shared__ int abort_flag;

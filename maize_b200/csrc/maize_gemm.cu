@@ -7,14 +7,12 @@
 // device every compute entry point returns an error.
 #include "../../include/maize_gemm.h"
 
-#include <cuda_runtime.h>
-
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
-#include <string>
 
+#include "maize_ctx.cuh"
 #include "gemm_sm100.cuh"
 #include "gemm_sm100_2cta.cuh"
 #include "gemm_sm100_2cta_tail.cuh"
@@ -26,12 +24,14 @@
 
 namespace {
 
+using maize::DeviceGuard;
 using maize::DeviceStatus;
+using maize::EncodeTiledFn;
+using maize::fail;
+using maize::fail_cuda;
 using maize::GemmParams;
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+using maize::kMaxChainLanes;
+using maize::kMaxHostSlabs;
 
 struct KernelVariant {
     const char *name;
@@ -69,101 +69,11 @@ constexpr int kPairTail = 9;
 constexpr int kSkinnyPairTall = 10;
 constexpr int kPairWideTile = 11;
 constexpr int kNumVariants = static_cast<int>(sizeof(kVariants) / sizeof(kVariants[0]));
+static_assert(kNumVariants <= maize::kMaxVariants, "the context keeps a flag per variant");
 constexpr int kMaxProfileCtas = 1024;
-constexpr uint32_t kMaxChainLanes = 4;  // streams maize_chain_forward may spread its chunks over
-constexpr int kMaxHostSlabs = 16;  // row slabs of A / C that the host entry point pipelines over PCIe
 constexpr size_t kPartialsBytes = size_t(32) << 20;  // stream-K scratch per context
 constexpr size_t kDefaultRepackBytes = size_t(128) << 20;  // scratch of the pitch-aligning pre-pass per context
 constexpr uint32_t kMaxSkinnyTiles = 65536;          // 4 counters each; N up to 8M rows
-
-class DeviceGuard {
-public:
-    explicit DeviceGuard(int device) : prev_(-1), changed_(false)
-    {
-        if (cudaGetDevice(&prev_) == cudaSuccess && prev_ != device) {
-            changed_ = cudaSetDevice(device) == cudaSuccess;
-        }
-    }
-    ~DeviceGuard()
-    {
-        if (changed_)
-            cudaSetDevice(prev_);
-    }
-
-private:
-    int prev_;
-    bool changed_;
-};
-
-}  // namespace
-
-struct maize_ctx {
-    int device = 0;
-    int sm_count = 0;
-    DeviceStatus *d_status = nullptr;
-    DeviceStatus *h_status = nullptr;  // pinned
-    uint64_t timeout_ns = 2000000000ull;
-    int force_kernel = 0;
-    int last_kernel = 0;             // public id of the GEMM kernel the last call launched
-    int max_ctas = 0;
-    uint32_t debug_flags = 0;
-    uint32_t group_rows = 0;         // rows of A scheduled together; 0 = by kernel (see tile_group_rows)
-    uint32_t pdl = 1;       // launch the GEMM kernels with programmatic stream serialization
-    uint32_t b_static = 0;  // the caller guarantees that nothing earlier in the stream writes B (weights)
-    uint32_t push_threads = 512;  // threads per CTA of the copy kernels of the multi-GPU path
-    uint32_t c_evict_first = 1;   // TMA stores of C carry an evict-first L2 hint
-    uint64_t wide_max_gflop = 1000000;  // largest GEMM (2MNK / 1e9) that takes the wide tile
-    uint32_t wide_tile = 1;       // use the 256 x 512 pair tile where it suits (long K, full rounds, about a millisecond of work)
-    uint32_t tma_store = 1;       // tiled kernels: C through shared memory and TMA stores when its rows are 16-byte aligned
-    uint32_t serpentine = 1;      // odd groups of row-blocks sweep the column-blocks backwards
-    uint32_t tma_promotion = 3;   // CUtensorMapL2promotion of the operand maps: 0 none, 1 64 B, 2 128 B, 3 256 B
-    uint32_t tail_split = 1;      // split the last partial round of pair tiles along K when pairs would idle
-    uint32_t chain_stagger = 1;   // two lanes on a source that is all there: offset them by half a chunk
-    uint32_t chain_streams = 2;   // 2: maize_chain_forward alternates chunks between the caller's stream and a helper
-    cudaStream_t chain_helper[kMaxChainLanes] = {};  // lanes 1 .. L-1 of maize_chain_forward (lane 0 is the caller's stream)
-    cudaEvent_t chain_ev_fork = nullptr;             // the caller's stream as of the call
-    cudaEvent_t chain_ev_pub[kMaxChainLanes] = {};   // "chunk published" per lane
-    cudaEvent_t chain_ev_part[kMaxChainLanes] = {};  // pieces of the first chunk sent (offsets the lanes)
-    uint64_t launches = 0;
-    EncodeTiledFn encode = nullptr;
-    void *staging = nullptr;  // device staging for the *_host entry point
-    size_t staging_bytes = 0;
-    // B of the last *_host call, still in the staging area: re-used instead of re-uploaded under "b_static"
-    const void *host_b_ptr = nullptr;
-    uint32_t host_b_rows = 0, host_b_cols = 0;
-    char *host_b_dev = nullptr;
-    void *repack = nullptr;  // scratch for operands copied to a 128-byte-aligned pitch ("repack_bytes")
-    size_t repack_bytes = 0;
-    const void *repack_b_ptr = nullptr;  // B whose aligned-pitch copy sits at the front of `repack` ("b_static" only)
-    uint32_t repack_b_rows = 0, repack_b_cols = 0;
-    uint64_t repack_b_ld = 0;
-    // helper streams and events of the *_host entry point (created on first use)
-    cudaStream_t copy_in = nullptr, copy_out = nullptr;
-    cudaEvent_t ev_start = nullptr, ev_done = nullptr;
-    cudaEvent_t ev_in[kMaxHostSlabs] = {}, ev_gemm[kMaxHostSlabs] = {};
-    bool attr_set[kNumVariants] = {};
-    bool attr_set_kn[kNumVariants] = {};  // the same for the K x N (MN-major B) instantiations
-    float *d_partials = nullptr;        // stream-K scratch of the skinny kernels
-    unsigned int *d_counters = nullptr;  // arrival counters, zero between launches
-    unsigned int *d_push_counter = nullptr;  // [0]: CTA arrivals of the multicast push; [16 + p]: of the scatter per rank
-    unsigned long long *d_profile = nullptr;  // kProfileSlots counters per CTA, allocated when "profile" is set
-    int profile_ctas = 0;                      // CTAs of the last profiled launch
-    std::string err;
-};
-
-namespace {
-
-maize_status_t fail(maize_ctx_t *ctx, maize_status_t st, const std::string &msg)
-{
-    if (ctx)
-        ctx->err = msg;
-    return st;
-}
-
-maize_status_t fail_cuda(maize_ctx_t *ctx, const char *what, cudaError_t e)
-{
-    return fail(ctx, MAIZE_ERR_CUDA, std::string(what) + ": " + cudaGetErrorName(e) + " (" + cudaGetErrorString(e) + ")");
-}
 
 // 2-D bf16 tensor map over a row-major [rows x cols] matrix with row pitch `ld`
 // elements; box = [box_rows x 64 elements], 128-byte swizzle, zero fill outside.
