@@ -321,6 +321,41 @@ MAIZE_API maize_status_t maize_gemm_bf16_nsharded_host(maize_mgpu_t *mg, int roo
 MAIZE_API maize_status_t maize_mgpu_sync(maize_mgpu_t *mg);
 
 /*
+ * Products of rows that belong to different weight matrices ("experts" of a mixture), forward and backward.  They have
+ * no counterpart in the reference.
+ *
+ * The rows of A (`rows` x K) are sorted by group: group g owns rows offsets[g] .. offsets[g+1]-1.  `offsets` is a DEVICE
+ * array of groups + 1 int32 values, ascending, within [0, rows]; nothing about the groups' sizes is needed on the host,
+ * and no call synchronises.  A group may be empty.  Rows before offsets[0] and from offsets[groups] on belong to no
+ * group: they are not read into any result and their rows of C are left as they were.  Offsets that do not ascend or
+ * leave [0, rows] are reported by maize_ctx_poll as MAIZE_ERR_DEVICE_ABORT; nothing is written then.
+ *
+ *   maize_grouped_gemm_bf16        C[r, :] = A[r, :] * B[g]^T   B[g] stored N x K
+ *   maize_grouped_gemm_bf16_kn     C[r, :] = A[r, :] * B[g]     B[g] stored K x N (also the gradient with respect to A
+ *                                  of the N x K form: pass DC as A, the same B, and swap N and K)
+ *   maize_grouped_gemm_bf16_wgrad  DB[g] = sum over the group's rows of DC[r, :]^T * A[r, :]   N x K each, the gradient
+ *                                  with respect to B; a group without rows gets zeros
+ *
+ * Matrix g of a stack starts `b_stride` (`db_stride`) elements after matrix g-1.  bf16 operands, fp32 accumulation, one
+ * rounding to bf16.  Limits: groups <= 1024; lda, ldb, lddc and b_stride multiples of 8, A, B and DC 16-byte aligned,
+ * and K % 8 == 0 where B is N x K; C and DB need only 2-byte alignment (16-byte aligned rows of DB, 4-byte aligned rows
+ * of C are stored faster).  K == 0 sets the groups' rows of C to zero.  The calls use no scratch memory: calls on
+ * different streams, or captured into different graphs, do not disturb each other.
+ */
+MAIZE_API maize_status_t maize_grouped_gemm_bf16(maize_ctx_t *ctx, const void *a, uint64_t lda, const void *b,
+                                                 uint64_t ldb, uint64_t b_stride, void *c, uint64_t ldc,
+                                                 const void *offsets, uint32_t groups, uint32_t rows, uint32_t n,
+                                                 uint32_t k, void *cuda_stream);
+MAIZE_API maize_status_t maize_grouped_gemm_bf16_kn(maize_ctx_t *ctx, const void *a, uint64_t lda, const void *b,
+                                                    uint64_t ldb, uint64_t b_stride, void *c, uint64_t ldc,
+                                                    const void *offsets, uint32_t groups, uint32_t rows, uint32_t n,
+                                                    uint32_t k, void *cuda_stream);
+MAIZE_API maize_status_t maize_grouped_gemm_bf16_wgrad(maize_ctx_t *ctx, const void *a, uint64_t lda, const void *dc,
+                                                       uint64_t lddc, void *db, uint64_t lddb, uint64_t db_stride,
+                                                       const void *offsets, uint32_t groups, uint32_t rows, uint32_t n,
+                                                       uint32_t k, void *cuda_stream);
+
+/*
  * Self-test of the bounded-wait machinery: launches one CTA that waits on a
  * barrier nothing will ever complete, with a budget of `budget_ns`.  The kernel
  * returns by itself; the following maize_ctx_poll reports MAIZE_ERR_TIMEOUT.

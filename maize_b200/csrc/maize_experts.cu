@@ -1,0 +1,301 @@
+// C ABI of the grouped ("expert") products (declared in include/maize_gemm.h): argument validation, tensor maps over
+// stacks of matrices, launches.  The sizes of the groups are known on the device only; what the host checks is
+// everything else.
+#include "../../include/maize_gemm.h"
+
+#include <cstdio>
+#include <cstring>
+
+#include "maize_ctx.cuh"
+#include "gemm_sm100_grouped.cuh"
+#include "gemm_sm100_grouped_wgrad.cuh"
+
+namespace {
+
+using maize::DeviceGuard;
+using maize::fail;
+using maize::fail_cuda;
+using maize::GroupedParams;
+
+constexpr uint32_t kMaxRows = 0x7fffff00u;  // row numbers are 32-bit offsets and TMA coordinates; room for a tile past the end
+constexpr uint32_t kMaxDim = 0x7fffff00u;
+
+// ctx->attr_experts slots
+enum { kAttrGrouped = 0, kAttrGroupedKn = 1, kAttrWgrad = 2 };
+
+bool aligned(const void *p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+maize_status_t encode_map(maize_ctx_t *ctx, CUtensorMap *map, CUtensorMapDataType type, uint32_t element_bytes,
+                          const void *base, uint32_t rank, const uint64_t *dims, const uint64_t *strides,
+                          const uint32_t *box_dims, CUtensorMapL2promotion promotion)
+{
+    cuuint64_t gdim[3], gstride[2];
+    cuuint32_t box[3], estride[3] = {1, 1, 1};
+    for (uint32_t i = 0; i < rank; ++i) {
+        gdim[i] = dims[i];
+        box[i] = box_dims[i];
+        if (i + 1 < rank)
+            gstride[i] = strides[i] * element_bytes;
+    }
+    const CUresult r = ctx->encode(map, type, rank, const_cast<void *>(base), gdim, gstride, box, estride,
+                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, promotion,
+                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS)
+        return MAIZE_OK;
+    char buf[160];
+    snprintf(buf, sizeof buf, "cuTensorMapEncodeTiled failed (CUresult %d) for %llu x %llu, ld %llu", (int)r,
+             (unsigned long long)dims[1], (unsigned long long)dims[0], (unsigned long long)strides[0]);
+    return fail(ctx, MAIZE_ERR_CUDA, buf);
+}
+
+// [rows x cols] bf16, boxes of box_rows x 64.
+maize_status_t matrix_map(maize_ctx_t *ctx, CUtensorMap *map, const void *base, uint64_t rows, uint64_t cols, uint64_t ld,
+                          uint32_t box_rows)
+{
+    const uint64_t dims[2] = {cols, rows}, strides[1] = {ld};
+    const uint32_t box[2] = {maize::kBlockK, box_rows};
+    return encode_map(ctx, map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, 2, dims, strides, box,
+                      static_cast<CUtensorMapL2promotion>(ctx->tma_promotion));
+}
+
+// A stack of `count` bf16 matrices [rows x cols], `stride` elements apart, boxes of 1 x box_rows x 64.
+maize_status_t stack_map(maize_ctx_t *ctx, CUtensorMap *map, const void *base, uint64_t count, uint64_t rows, uint64_t cols,
+                         uint64_t ld, uint64_t stride, uint32_t box_rows, CUtensorMapL2promotion promotion)
+{
+    const uint64_t dims[3] = {cols, rows, count}, strides[2] = {ld, stride};
+    const uint32_t box[3] = {maize::kBlockK, box_rows, 1};
+    return encode_map(ctx, map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, 3, dims, strides, box, promotion);
+}
+
+template <typename Kernel, typename... Args>
+maize_status_t launch(maize_ctx_t *ctx, int attr_slot, Kernel kernel, uint32_t grid, uint32_t threads, uint32_t smem,
+                      cudaStream_t stream, const Args &...args)
+{
+    if (!ctx->attr_experts[attr_slot]) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess)
+            return fail_cuda(ctx, "cudaFuncSetAttribute(max dynamic smem)", e);
+        ctx->attr_experts[attr_slot] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ctx->pdl ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (e != cudaSuccess)
+        return fail_cuda(ctx, "kernel launch", e);
+    ctx->launches += 1;
+    return MAIZE_OK;
+}
+
+// CTAs that may run at a time, a multiple of `unit` (the cluster size), at most what `tiles` clusters need.
+uint32_t persistent_grid(const maize_ctx_t *ctx, uint64_t tiles, uint32_t unit)
+{
+    uint32_t cap = static_cast<uint32_t>(ctx->sm_count);
+    if (ctx->max_ctas > 0 && static_cast<uint32_t>(ctx->max_ctas) < cap)
+        cap = static_cast<uint32_t>(ctx->max_ctas);
+    cap /= unit;
+    if (cap == 0)
+        cap = 1;
+    return (tiles < cap ? static_cast<uint32_t>(tiles) : cap) * unit;
+}
+
+// What the three grouped entry points check alike.
+maize_status_t check_groups(maize_ctx_t *ctx, const void *offsets, uint32_t groups, uint32_t rows)
+{
+    if (!offsets || !aligned(offsets, 4))
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "offsets must be a 4-byte aligned device array of groups + 1 integers");
+    if (groups > maize::kGroupedMaxGroups)
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "more than 1024 groups");
+    if (rows > kMaxRows)
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "too many rows for 32-bit offsets");
+    return MAIZE_OK;
+}
+
+// A stack of row-major matrices [rows x cols]: the matrices may not overlap.
+bool stack_ok(uint32_t count, uint64_t stride, uint64_t rows, uint64_t cols, uint64_t ld)
+{
+    return count <= 1 || rows == 0 || stride >= (rows - 1) * ld + cols;
+}
+
+maize_status_t grouped_impl(maize_ctx_t *ctx, const void *a, uint64_t lda, const void *b, uint64_t ldb, uint64_t b_stride,
+                            void *c, uint64_t ldc, const void *offsets, uint32_t groups, uint32_t rows, uint32_t n,
+                            uint32_t k, cudaStream_t stream, bool b_kn)
+{
+    if (!ctx)
+        return MAIZE_ERR_INVALID_ARG;
+    ctx->err.clear();
+    if (rows == 0 || n == 0 || groups == 0)
+        return MAIZE_OK;
+    maize_status_t st = check_groups(ctx, offsets, groups, rows);
+    if (st != MAIZE_OK)
+        return st;
+    if (!c)
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "C pointer is null");
+    if (ldc < n)
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "ldc is smaller than N");
+    if (!aligned(c, 2))
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "C must be 2-byte aligned");
+    if (n > kMaxDim || k > kMaxDim)
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "N or K beyond the kernel's range");
+    GroupedParams p = {};
+    p.c = static_cast<__nv_bfloat16 *>(c);
+    p.ldc = ldc;
+    p.offsets = static_cast<const int32_t *>(offsets);
+    p.groups = groups;
+    p.rows = rows;
+    p.n = n;
+    p.k = k;
+    p.c_pair_ok = (ldc % 2 == 0 && aligned(c, 4)) ? 1u : 0u;
+    p.pdl = ctx->pdl;
+    p.status = ctx->d_status;
+    p.timeout_ns = ctx->timeout_ns;
+    DeviceGuard guard(ctx->device);
+    if (k == 0) {
+        maize::grouped_zero_rows_kernel<<<static_cast<uint32_t>(ctx->sm_count), 256, 0, stream>>>(p);
+        ctx->launches += 1;
+        const cudaError_t e = cudaGetLastError();
+        return e == cudaSuccess ? MAIZE_OK : fail_cuda(ctx, "kernel launch", e);
+    }
+    if (!a || !b)
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "A or B pointer is null");
+    if (lda < k || ldb < (b_kn ? n : k))
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "lda/ldb is smaller than the row length");
+    if (!stack_ok(groups, b_stride, b_kn ? k : n, b_kn ? n : k, ldb))
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "the matrices of B overlap: b_stride is smaller than a matrix");
+    if (groups == 1)
+        b_stride = uint64_t(b_kn ? k : n) * ldb;  // not used for addressing; the map wants a valid pitch
+    if (lda % 8 != 0 || ldb % 8 != 0 || b_stride % 8 != 0 || (!b_kn && k % 8 != 0))
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "K, lda, ldb and b_stride must be multiples of 8 (16-byte TMA pitch)");
+    if (!aligned(a, 16) || !aligned(b, 16))
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "A and B must be 16-byte aligned");
+    if (lda * 2 >= (1ull << 40) || ldb * 2 >= (1ull << 40) || b_stride * 2 >= (1ull << 40))
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "pitch beyond the TMA limit of 2^40 bytes");
+
+    maize::RowMaps ta;
+    for (uint32_t i = 0; i < 4; ++i)
+        if ((st = matrix_map(ctx, &ta.box[i], a, rows, k, lda, 16u << i)) != MAIZE_OK)
+            return st;
+    CUtensorMap tw;
+    const CUtensorMapL2promotion promotion = static_cast<CUtensorMapL2promotion>(ctx->tma_promotion);
+    st = b_kn ? stack_map(ctx, &tw, b, groups, k, n, ldb, b_stride, maize::kBlockK, promotion)
+              : stack_map(ctx, &tw, b, groups, n, k, ldb, b_stride, maize::kBlockM, promotion);
+    if (st != MAIZE_OK)
+        return st;
+
+    const uint64_t n_blocks = (uint64_t(n) + maize::kGroupedTileCols - 1) / maize::kGroupedTileCols;
+    // at most: whole row tiles plus one more in every group that has rows
+    const uint64_t row_tiles = rows / maize::kGroupedTileRows + (rows < groups ? rows : groups);
+    const uint32_t grid = persistent_grid(ctx, row_tiles * n_blocks, 2);
+    using L = maize::GroupedSmemLayout<6>;
+    return b_kn ? launch(ctx, kAttrGroupedKn, maize::gemm_bf16_sm100_grouped<true, 6>, grid, maize::kNumThreads,
+                         L::kDynamicBytes, stream, ta, tw, p)
+                : launch(ctx, kAttrGrouped, maize::gemm_bf16_sm100_grouped<false, 6>, grid, maize::kNumThreads,
+                         L::kDynamicBytes, stream, ta, tw, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+maize_status_t maize_grouped_gemm_bf16(maize_ctx_t *ctx, const void *a, uint64_t lda, const void *b, uint64_t ldb,
+                                       uint64_t b_stride, void *c, uint64_t ldc, const void *offsets, uint32_t groups,
+                                       uint32_t rows, uint32_t n, uint32_t k, void *cuda_stream)
+{
+    return grouped_impl(ctx, a, lda, b, ldb, b_stride, c, ldc, offsets, groups, rows, n, k,
+                        static_cast<cudaStream_t>(cuda_stream), false);
+}
+
+maize_status_t maize_grouped_gemm_bf16_kn(maize_ctx_t *ctx, const void *a, uint64_t lda, const void *b, uint64_t ldb,
+                                          uint64_t b_stride, void *c, uint64_t ldc, const void *offsets, uint32_t groups,
+                                          uint32_t rows, uint32_t n, uint32_t k, void *cuda_stream)
+{
+    return grouped_impl(ctx, a, lda, b, ldb, b_stride, c, ldc, offsets, groups, rows, n, k,
+                        static_cast<cudaStream_t>(cuda_stream), true);
+}
+
+maize_status_t maize_grouped_gemm_bf16_wgrad(maize_ctx_t *ctx, const void *a, uint64_t lda, const void *dc, uint64_t lddc,
+                                             void *db, uint64_t lddb, uint64_t db_stride, const void *offsets,
+                                             uint32_t groups, uint32_t rows, uint32_t n, uint32_t k, void *cuda_stream)
+{
+    if (!ctx)
+        return MAIZE_ERR_INVALID_ARG;
+    ctx->err.clear();
+    if (n == 0 || k == 0 || groups == 0)
+        return MAIZE_OK;
+    maize_status_t st = check_groups(ctx, offsets, groups, rows);
+    if (st != MAIZE_OK)
+        return st;
+    if (!db)
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "DB pointer is null");
+    if (lddb < k)
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "lddb is smaller than K");
+    if (!aligned(db, 2))
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "DB must be 2-byte aligned");
+    if (!stack_ok(groups, db_stride, n, k, lddb))
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "the matrices of DB overlap: db_stride is smaller than a matrix");
+    if (n > kMaxDim || k > kMaxDim)
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "N or K beyond the kernel's range");
+    const uint64_t tiles = uint64_t(groups) * ((uint64_t(n) + 255) / 256) * ((uint64_t(k) + 255) / 256);
+    if (tiles > 0x7fffffffull)
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "too many output tiles");
+    DeviceGuard guard(ctx->device);
+    cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    if (rows == 0) {
+        // no rows at all: every gradient is zero
+        for (uint32_t g = 0; g < groups; ++g) {
+            const cudaError_t e = cudaMemset2DAsync(static_cast<char *>(db) + uint64_t(g) * db_stride * 2, lddb * 2, 0,
+                                                    size_t(k) * 2, n, stream);
+            if (e != cudaSuccess)
+                return fail_cuda(ctx, "cudaMemset2DAsync", e);
+        }
+        return MAIZE_OK;
+    }
+    if (!a || !dc)
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "A or DC pointer is null");
+    if (lda < k || lddc < n)
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "lda/lddc is smaller than the row length");
+    if (lda % 8 != 0 || lddc % 8 != 0)
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "lda and lddc must be multiples of 8 (16-byte TMA pitch)");
+    if (!aligned(a, 16) || !aligned(dc, 16))
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "A and DC must be 16-byte aligned");
+    if (lda * 2 >= (1ull << 40) || lddc * 2 >= (1ull << 40))
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "pitch beyond the TMA limit of 2^40 bytes");
+    CUtensorMap tdc, ta, tdw;
+    if ((st = matrix_map(ctx, &tdc, dc, rows, n, lddc, maize::kBlockK)) != MAIZE_OK ||
+        (st = matrix_map(ctx, &ta, a, rows, k, lda, maize::kBlockK)) != MAIZE_OK)
+        return st;
+    memset(&tdw, 0, sizeof tdw);
+    if (groups == 1)
+        db_stride = uint64_t(n) * lddb;
+    GroupedParams p = {};
+    p.c = static_cast<__nv_bfloat16 *>(db);
+    p.ldc = lddb;
+    p.c_stride = db_stride;
+    p.offsets = static_cast<const int32_t *>(offsets);
+    p.groups = groups;
+    p.rows = rows;
+    p.n = n;
+    p.k = k;
+    p.pdl = ctx->pdl;
+    p.status = ctx->d_status;
+    p.timeout_ns = ctx->timeout_ns;
+    // Rows of DB that TMA can store: a store writes whole 16-byte pieces, so K has to end on one (a K of 57 had zeros
+    // written into the seven columns behind it).  A stack the driver refuses goes by plain stores too.
+    if (ctx->tma_store && k % 8 == 0 && lddb % 8 == 0 && db_stride % 8 == 0 && aligned(db, 16) && lddb * 2 < (1ull << 40) &&
+        db_stride * 2 < (1ull << 40)) {
+        p.c_tma_ok = stack_map(ctx, &tdw, db, groups, n, k, lddb, db_stride, 32, CU_TENSOR_MAP_L2_PROMOTION_NONE) == MAIZE_OK;
+        ctx->err.clear();
+    }
+    const uint32_t grid = persistent_grid(ctx, tiles, 2);
+    return launch(ctx, kAttrWgrad, maize::gemm_bf16_sm100_grouped_wgrad<5>, grid, maize::kWgradThreads,
+                  maize::WgradSmemLayout<5>::kDynamicBytes, stream, tdc, ta, tdw, p);
+}
+
+}  // extern "C"

@@ -143,6 +143,27 @@ __device__ __forceinline__ void tma_load_2d_pair_hint(uint32_t smem_dst, const C
         : "memory");
 }
 
+// 3-D forms (x innermost, z = matrix of a stack): the same rules.
+__device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap *map, uint32_t bar, int32_t x,
+                                            int32_t y, int32_t z)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t smem_dst, const CUtensorMap *map, uint32_t bar_cluster_addr,
+                                                 int32_t x, int32_t y, int32_t z)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
 // 2-D tiled store shared memory -> global (the box of the tensor map, swizzled as the map says); elements outside
 // the tensor are not written.  x * 2 bytes must be a multiple of 16 and no coordinate negative.  Completion is
 // tracked by bulk groups of the issuing thread.
@@ -161,6 +182,14 @@ __device__ __forceinline__ void tma_store_2d_hint(const CUtensorMap *map, uint32
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group.L2::cache_hint [%0, {%2, %3}], [%1], %4;" ::"l"(
                      reinterpret_cast<uint64_t>(map)),
                  "r"(smem_src), "r"(x), "r"(y), "l"(policy)
+                 : "memory");
+}
+
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, uint32_t smem_src, int32_t x, int32_t y, int32_t z)
+{
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(smem_src), "r"(x), "r"(y), "r"(z)
                  : "memory");
 }
 
@@ -310,10 +339,11 @@ __device__ __forceinline__ uint64_t make_smem_desc_sw128_mn(uint32_t smem_addr, 
 // Instruction descriptor for kind::f16 with bf16 A/B (both K-major), fp32 D:
 //   bits 4-5 D format (1 = f32), 7-9 A format (1 = bf16), 10-12 B format (1 = bf16),
 //   bit 15/16 A/B major (0 = K), bits 17-22 N >> 3, bits 24-28 M >> 4.
-__host__ __device__ constexpr uint32_t make_instr_desc_bf16(uint32_t mma_m, uint32_t mma_n, bool b_mn_major = false)
+__host__ __device__ constexpr uint32_t make_instr_desc_bf16(uint32_t mma_m, uint32_t mma_n, bool b_mn_major = false,
+                                                            bool a_mn_major = false)
 {
-    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn_major ? (1u << 16) : 0u) | ((mma_n >> 3) << 17) |
-           ((mma_m >> 4) << 24);
+    return (1u << 4) | (1u << 7) | (1u << 10) | (a_mn_major ? (1u << 15) : 0u) | (b_mn_major ? (1u << 16) : 0u) |
+           ((mma_n >> 3) << 17) | ((mma_m >> 4) << 24);
 }
 
 // D[tmem] (+)= A[smem] * B[smem]^T, one CTA.  Issued by ONE thread.

@@ -239,6 +239,97 @@ class Context:
                                                     m, n, k, _stream_handle(stream)))
         return out
 
+    # ------------------------------------------- products grouped by expert --
+    def _own(self, name: str, t, dims: int, dtype) -> None:
+        """The checks every operand of the calls below shares: kind, device, unit stride along the rows."""
+        if (t.dim() != dims or t.dtype != dtype or not t.is_cuda or t.device.index != self.device
+                or (t.shape[-1] > 1 and t.stride(-1) != 1)):
+            raise MaizeError(_ffi.INVALID_ARG, f"{name}: expected a {dims}-D {dtype} tensor with unit column stride on "
+                                               f"cuda:{self.device}")
+
+    def _stream(self, stream) -> int:
+        """Handle of the stream a call runs on: the given one, or the current stream of the context's device."""
+        if stream is None:
+            import torch
+            return torch.cuda.current_stream(self.device).cuda_stream
+        return stream if isinstance(stream, int) else stream.cuda_stream
+
+    def _new(self, shape, dtype, stream):
+        """An output tensor, allocated for the stream the call runs on."""
+        import torch
+        if stream is None:
+            return torch.empty(shape, dtype=dtype, device=torch.device("cuda", self.device))
+        if isinstance(stream, int):
+            stream = torch.cuda.ExternalStream(stream, device=self.device)
+        with torch.cuda.stream(stream):
+            return torch.empty(shape, dtype=dtype, device=torch.device("cuda", self.device))
+
+    def _offsets(self, offsets, groups: int) -> None:
+        import torch
+        if (offsets.dim() != 1 or offsets.dtype != torch.int32 or not offsets.is_cuda
+                or offsets.device.index != self.device or offsets.shape[0] != groups + 1 or not offsets.is_contiguous()):
+            raise MaizeError(_ffi.INVALID_ARG, f"offsets: expected {groups + 1} contiguous int32 values on cuda:{self.device}")
+
+    def _grouped(self, entry, a, b, offsets, out, stream, n: int, kb: int):
+        import torch
+        bf16 = torch.bfloat16
+        self._own("a", a, 2, bf16)
+        self._own("b", b, 3, bf16)
+        rows, k = a.shape
+        groups = b.shape[0]
+        if k != kb:
+            raise MaizeError(_ffi.INVALID_ARG, f"a has {k} columns, the matrices of b a K of {kb}")
+        self._offsets(offsets, groups)
+        if out is None:
+            out = self._new((rows, n), bf16, stream)
+        else:
+            self._own("out", out, 2, bf16)
+            if out.shape != (rows, n):
+                raise MaizeError(_ffi.INVALID_ARG, f"out: expected {rows} x {n}")
+        self._check(entry(self._h, a.data_ptr(), a.stride(0) if rows > 1 else max(k, -(-k // 8) * 8), b.data_ptr(),
+                          b.stride(1) if b.shape[1] > 1 else -(-b.shape[2] // 8) * 8, b.stride(0), out.data_ptr(),
+                          out.stride(0) if rows > 1 else max(n, 1), offsets.data_ptr(), groups, rows, n, k,
+                          self._stream(stream)))
+        return out
+
+    def grouped_gemm(self, a, b, offsets, out=None, stream=None):
+        """``out[r] = a[r] @ b[g].T`` for the rows ``offsets[g] <= r < offsets[g + 1]`` of every group g: a is rows x K,
+        b is groups x N x K (one weight matrix per expert), offsets int32 on the device, ascending, groups + 1 of them.
+        Rows outside all groups are left as they were.  Groups may be empty; their sizes are never read on the host."""
+        return self._grouped(self._lib.maize_grouped_gemm_bf16, a, b, offsets, out, stream, b.shape[-2], b.shape[-1])
+
+    def grouped_gemm_kn(self, a, b, offsets, out=None, stream=None):
+        """``out[r] = a[r] @ b[g]`` with b given groups x K x N.  With ``a`` the gradient of ``grouped_gemm``'s result and
+        the same b this is the gradient of its input."""
+        return self._grouped(self._lib.maize_grouped_gemm_bf16_kn, a, b, offsets, out, stream, b.shape[-1], b.shape[-2])
+
+    def grouped_gemm_wgrad(self, a, dc, offsets, out=None, stream=None):
+        """``out[g] = dc[rows of g].T @ a[rows of g]``: the gradient of ``grouped_gemm``'s b (groups x N x K) from its
+        input ``a`` (rows x K) and the gradient ``dc`` (rows x N) of its result.  A group without rows gets zeros."""
+        import torch
+        bf16 = torch.bfloat16
+        self._own("a", a, 2, bf16)
+        self._own("dc", dc, 2, bf16)
+        rows, k = a.shape
+        n = dc.shape[1]
+        if dc.shape[0] != rows:
+            raise MaizeError(_ffi.INVALID_ARG, f"a has {rows} rows, dc {dc.shape[0]}")
+        if offsets.dim() != 1 or offsets.shape[0] < 1:
+            raise MaizeError(_ffi.INVALID_ARG, "offsets: expected groups + 1 int32 values")
+        groups = offsets.shape[0] - 1
+        self._offsets(offsets, groups)
+        if out is None:
+            out = self._new((groups, n, k), bf16, stream)
+        else:
+            self._own("out", out, 3, bf16)
+            if out.shape != (groups, n, k):
+                raise MaizeError(_ffi.INVALID_ARG, f"out: expected {groups} x {n} x {k}")
+        self._check(self._lib.maize_grouped_gemm_bf16_wgrad(
+            self._h, a.data_ptr(), a.stride(0) if rows > 1 else -(-k // 8) * 8, dc.data_ptr(),
+            dc.stride(0) if rows > 1 else -(-n // 8) * 8, out.data_ptr(), out.stride(1) if n > 1 else max(k, 1),
+            out.stride(0), offsets.data_ptr(), groups, rows, n, k, self._stream(stream)))
+        return out
+
     def debug_wait_expires(self, budget_ns: int, stream=None) -> None:
         self._check(self._lib.maize_debug_wait_expires(self._h, int(budget_ns), _stream_handle(stream)))
 
@@ -259,6 +350,27 @@ def default_context(device: Optional[int] = None) -> Context:
 def gemm(a, b, out=None, stream=None):
     """``a @ b.T`` on the B200 kernels (module-level convenience over a cached Context)."""
     return default_context(a.device.index).gemm(a, b, out=out, stream=stream)
+
+
+def _context_of(t) -> Context:
+    if not t.is_cuda:
+        raise MaizeError(_ffi.INVALID_ARG, "expected CUDA tensors")
+    return default_context(t.device.index)
+
+
+def grouped_gemm(a, b, offsets, out=None, stream=None):
+    """``Context.grouped_gemm`` over a cached Context of a's device."""
+    return _context_of(a).grouped_gemm(a, b, offsets, out, stream)
+
+
+def grouped_gemm_kn(a, b, offsets, out=None, stream=None):
+    """``Context.grouped_gemm_kn`` over a cached Context of a's device."""
+    return _context_of(a).grouped_gemm_kn(a, b, offsets, out, stream)
+
+
+def grouped_gemm_wgrad(a, dc, offsets, out=None, stream=None):
+    """``Context.grouped_gemm_wgrad`` over a cached Context of a's device."""
+    return _context_of(a).grouped_gemm_wgrad(a, dc, offsets, out, stream)
 
 
 def gemm_skinny_static(a, b, out, stream=None, device_status=None):
