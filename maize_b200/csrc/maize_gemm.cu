@@ -364,7 +364,7 @@ maize_status_t gemm_impl(maize_ctx_t *ctx, const void *a, uint64_t lda, const vo
     // The wide tile's epilogue is not hidden behind the next tile's main loop, so it has to be the fast one: rows
     // of C that TMA can store.  (4111 x 3967 x 4104, odd row pitch of C: 0.164 ms against 0.137 ms.)
     if (vi == kPairWideTile && ctx->force_kernel == 0 &&
-        !(ctx->tma_store && ldc % 8 == 0 && reinterpret_cast<uintptr_t>(c) % 16 == 0))
+        !(ctx->tma_store && n % 8 == 0 && ldc % 8 == 0 && reinterpret_cast<uintptr_t>(c) % 16 == 0))
         vi = kPairWide;
     const KernelVariant &kv = kVariants[vi];
     ctx->last_kernel = vi + 1;
@@ -534,11 +534,12 @@ maize_status_t gemm_impl(maize_ctx_t *ctx, const void *a, uint64_t lda, const vo
         return st;
 
     // C leaves the tiled kernels (tiles of 64 columns and more) through shared memory and TMA stores when its
-    // rows are 16-byte aligned
+    // rows are 16-byte aligned.  A TMA store writes whole 16-byte pieces, also at the edge of the tensor: N has to end on
+    // one, or up to seven columns behind C's would be set to zero.
     CUtensorMap tc;
     memset(&tc, 0, sizeof tc);
     const bool c_rows_aligned = ldc % 8 == 0 && reinterpret_cast<uintptr_t>(c) % 16 == 0;
-    const bool c_tma = ctx->tma_store && c_rows_aligned && kv.block_n >= 64 && ldc * 2 < (1ull << 40) &&
+    const bool c_tma = ctx->tma_store && c_rows_aligned && n % 8 == 0 && kv.block_n >= 64 && ldc * 2 < (1ull << 40) &&
                        make_store_map(ctx, &tc, c, m, n, ldc);
 
     GemmParams p;
