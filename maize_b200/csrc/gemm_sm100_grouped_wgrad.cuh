@@ -28,7 +28,7 @@ struct WgradSmemLayout {
     static constexpr uint32_t kStageBytes = 2 * kOperandBytes;        // [DC0, DC1, A0, A1]
     static constexpr uint32_t kStagingOffset = STAGES * kStageBytes;
     static constexpr uint32_t kBarOffset = kStagingOffset + kTmaStageBytesTotal;
-    static constexpr uint32_t kNumBars = 3 * STAGES + 4;
+    static constexpr uint32_t kNumBars = 4 * STAGES + 4;
     static constexpr uint32_t kTmemSlotOffset = kBarOffset + kNumBars * 8;
     static constexpr uint32_t kAbortOffset = kTmemSlotOffset + 4;
     static constexpr uint32_t kTableOffset = (kAbortOffset + 4 + 15) / 16 * 16;
@@ -152,6 +152,7 @@ gemm_bf16_sm100_grouped_wgrad(const __grid_constant__ CUtensorMap tma_dc, const 
     auto acc_full_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + b); };
     auto acc_empty_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + 2 + b); };
     auto tail_bar = [&](uint32_t s) { return bar_base + 8u * (2 * STAGES + 4 + s); };  // this CTA's bytes of a cut block
+    auto peer_bar = [&](uint32_t s) { return bar_base + 8u * (3 * STAGES + 4 + s); };  // leader: the peer's cut block is clear
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + L::kTmemSlotOffset);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem_gen + L::kAbortOffset);
     GroupTable tab;
@@ -173,9 +174,10 @@ gemm_bf16_sm100_grouped_wgrad(const __grid_constant__ CUtensorMap tma_dc, const 
         if (p.c_tma_ok)
             ptx::prefetch_tensormap(&tma_dw);
         for (uint32_t s = 0; s < STAGES; ++s) {
-            ptx::mbar_init(full_bar(s), 2);   // one arrival per CTA (producer, or fix warp for a cut block) and the bytes
+            ptx::mbar_init(full_bar(s), 1);   // the leader's producer and the bytes of both CTAs, or the leader's fix warp
             ptx::mbar_init(empty_bar(s), 1);  // one tcgen05.commit of the leader
             ptx::mbar_init(tail_bar(s), 1);   // this CTA's producer and its bytes
+            ptx::mbar_init(peer_bar(s), 1);   // the peer's fix warp
         }
         for (uint32_t b = 0; b < 2; ++b) {
             ptx::mbar_init(acc_full_bar(b), 1);
@@ -231,8 +233,6 @@ gemm_bf16_sm100_grouped_wgrad(const __grid_constant__ CUtensorMap tma_dc, const 
                         const uint32_t leader_full = ptx::mapa_shared(full_bar(stage), 0);
                         if (cta_rank == 0)
                             ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * L::kStageBytes);
-                        else
-                            ptx::mbar_arrive_cluster_addr(leader_full);
 #pragma unroll
                         for (uint32_t j = 0; j < 2; ++j) {
                             ptx::tma_load_2d_pair(sd + j * kChunkBytes, &tma_dc, leader_full, n0 + static_cast<int32_t>(64u * j), r);
@@ -296,7 +296,7 @@ gemm_bf16_sm100_grouped_wgrad(const __grid_constant__ CUtensorMap tma_dc, const 
     } else if (warp == 6) {
         // ----------------------------------------------------------- fix warp --
         uint32_t stage = 0;
-        uint32_t tail_phase = 0;  // bit s: parity of the next use of tail_bar(s)
+        uint32_t tail_phase = 0;  // bit s: parity of the next use of tail_bar(s) and peer_bar(s)
         bool ok = true;
         for (uint32_t t = pair; ok && t < num_tiles; t += num_pairs) {
             const WgradTile tile = wgrad_tile(t, m_blocks, n_blocks, tab);
@@ -311,7 +311,6 @@ gemm_bf16_sm100_grouped_wgrad(const __grid_constant__ CUtensorMap tma_dc, const 
             ok = __all_sync(0xffffffffu, ok);
             if (!ok)
                 break;
-            tail_phase ^= 1u << last;
             const uint32_t sd = smem_base + last * L::kStageBytes;
             const uint32_t end = (left + 15u) & ~15u;
             // 8 lanes clear a 128-byte row, 4 rows at a time, in the four boxes of the stage
@@ -322,8 +321,21 @@ gemm_bf16_sm100_grouped_wgrad(const __grid_constant__ CUtensorMap tma_dc, const 
             }
             ptx::fence_proxy_async_shared();
             __syncwarp();
-            if (lane == 0)
-                ptx::mbar_arrive_cluster_addr(ptx::mapa_shared(full_bar(last), 0));
+            // The peer tells the leader's fix warp and that one the MMA thread.  (An arrival of the peer's producer on
+            // every stage instead, so that the stage's barrier itself counts both CTAs, cost two thirds of the rate: a
+            // remote arrival releases at cluster scope, and the loads behind it wait for that.)
+            if (cta_rank != 0) {
+                if (lane == 0)
+                    ptx::mbar_arrive_cluster_addr(ptx::mapa_shared(peer_bar(last), 0));
+            } else {
+                ok = wait_bounded<true>(peer_bar(last), (tail_phase >> last) & 1u, ctl, 4);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok)
+                    break;
+                if (lane == 0)
+                    ptx::mbar_arrive(full_bar(last));
+            }
+            tail_phase ^= 1u << last;
             __syncwarp();
         }
         role_ok = ok;
