@@ -356,6 +356,33 @@ MAIZE_API maize_status_t maize_grouped_gemm_bf16_wgrad(maize_ctx_t *ctx, const v
                                                        uint32_t k, void *cuda_stream);
 
 /*
+ * 8-bit products: e4m3 operands (1 sign, 4 exponent, 3 mantissa bits; no infinities, largest 448) with one fp32 scale for
+ * each block of 128 along K.  They have no counterpart in the reference.
+ *
+ * maize_quantize_e4m3: bf16 X (`rows` x `cols`, row pitch ldx) -> e4m3 Q and scales.  `block_rows` = 1 gives a scale for
+ * each 1 x 128 block (activations; scales rows x ceil(cols/128)), 128 one for each 128 x 128 block (weights; scales
+ * ceil(rows/128) x ceil(cols/128)); the last block of a row or column may be cut short.  The scale is the smallest power
+ * of two s >= 2^-126 with max|x| <= 448 s (1 for a block of zeros), so x / s is exact and the one rounding is to e4m3,
+ * nearest even.  An element that is not finite becomes NaN and has no part in the maximum.  Any alignment that the element
+ * types allow; rows of X that start 16-byte and rows of Q that start 8-byte aligned go faster.
+ *
+ * maize_gemm_e4m3: C (M x N bf16) = sum over k-blocks j of a_scales[m][j] * b_scales[n / 128][j] * (the product of the
+ * block's elements of A (M x K, e4m3) and B (N x K, e4m3)).  a_scales is M x ceil(K/128), b_scales ceil(N/128) x
+ * ceil(K/128), row pitches ld_a_scales and ld_b_scales; any fp32 scales (the product of two should be a normal fp32
+ * number).  Sums are fp32, C is rounded once.  K, lda and ldb multiples of 16, A and B 16-byte aligned; C needs 2-byte
+ * alignment.
+ *
+ * Neither call uses scratch memory.
+ */
+MAIZE_API maize_status_t maize_quantize_e4m3(maize_ctx_t *ctx, const void *x, uint64_t ldx, uint32_t rows, uint32_t cols,
+                                             uint32_t block_rows, void *q, uint64_t ldq, void *scales,
+                                             uint64_t ld_scales, void *cuda_stream);
+MAIZE_API maize_status_t maize_gemm_e4m3(maize_ctx_t *ctx, const void *a, uint64_t lda, const void *a_scales,
+                                         uint64_t ld_a_scales, const void *b, uint64_t ldb, const void *b_scales,
+                                         uint64_t ld_b_scales, void *c, uint64_t ldc, uint32_t m, uint32_t n, uint32_t k,
+                                         void *cuda_stream);
+
+/*
  * Self-test of the bounded-wait machinery: launches one CTA that waits on a
  * barrier nothing will ever complete, with a budget of `budget_ns`.  The kernel
  * returns by itself; the following maize_ctx_poll reports MAIZE_ERR_TIMEOUT.

@@ -7,8 +7,8 @@ computing needs the built library and a B200.
 """
 from . import tile  # noqa: F401
 from ._ffi import LIB_PATH, STATUS_NAMES  # noqa: F401
-from .gemm import (Context, MaizeError, Matrix, default_context, gemm, gemm_skinny_static, grouped_gemm,  # noqa: F401
-                   grouped_gemm_kn, grouped_gemm_wgrad)
+from .gemm import (Context, MaizeError, Matrix, default_context, gemm, gemm_e4m3, gemm_skinny_static,  # noqa: F401
+                   grouped_gemm, grouped_gemm_kn, grouped_gemm_wgrad, quantize_e4m3)
 
-__all__ = ["Context", "MaizeError", "Matrix", "default_context", "gemm", "gemm_skinny_static", "grouped_gemm",
-           "grouped_gemm_kn", "grouped_gemm_wgrad", "tile", "LIB_PATH"]
+__all__ = ["Context", "MaizeError", "Matrix", "default_context", "gemm", "gemm_e4m3", "gemm_skinny_static",
+           "grouped_gemm", "grouped_gemm_kn", "grouped_gemm_wgrad", "quantize_e4m3", "tile", "LIB_PATH"]

@@ -43,6 +43,8 @@ SYMBOLS = {
     "maize_grouped_gemm_bf16_kn": (_int, [_vp, _vp, _u64, _vp, _u64, _u64, _vp, _u64, _vp, _u32, _u32, _u32, _u32, _vp]),
     "maize_grouped_gemm_bf16_wgrad": (_int, [_vp, _vp, _u64, _vp, _u64, _vp, _u64, _u64, _vp, _u32, _u32, _u32, _u32,
                                              _vp]),
+    "maize_quantize_e4m3": (_int, [_vp, _vp, _u64, _u32, _u32, _u32, _vp, _u64, _vp, _u64, _vp]),
+    "maize_gemm_e4m3": (_int, [_vp, _vp, _u64, _vp, _u64, _vp, _u64, _vp, _u64, _vp, _u64, _u32, _u32, _u32, _vp]),
     "maize_gemm_bf16_host": (_int, [_vp, _vp, _u32, _u32, _vp, _u32, _u32, _vp, _u32, _u32, _vp]),
     "maize_ctx_poll": (_int, [_vp, _vp]),
     "maize_ctx_set": (_int, [_vp, ctypes.c_char_p, _i64]),

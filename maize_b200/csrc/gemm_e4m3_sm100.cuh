@@ -1,0 +1,304 @@
+// Products of e4m3 operands with a scale for each block of 128 along K:
+//
+//     C[m, n] = sum over k-blocks j of  sa[m, j] * sb[n / 128, j] * sum over k in block j of  qa[m, k] * qb[n, k]
+//
+// sa: one fp32 per row of A and k-block; sb: one fp32 per 128 x 128 block of B.  The inner sum is one tensor-core pass over
+// 128 k (four tcgen05.mma.kind::f8f6f4 of 32), the outer one runs in fp32 registers ("promotion"): any scales, no rounding
+// but fp32's until C is rounded to bf16 once.
+//
+// A CTA pair computes a 256 x 256 tile (128 x 256 per CTA).  One k-block of both operands is one 128-byte swizzle row, so
+// the ring looks like the bf16 kernel's with twice the k per byte.  TMEM holds two accumulator buffers of 256 columns, one
+// k-block each: while the MMA fills one, eight promotion warps read the other (`tcgen05.ld`), multiply by the two scales
+// and add to 128 fp32 registers per thread; they hand the buffer back as soon as its last column is in registers.
+//
+// Bound: per k-block and SM the MMA needs 512 cycles, the TMEM read 256 (512 bytes a cycle), the fp32 multiply-adds 256
+// issue slots per scheduler: the tensor pipe leads if the hand-over of buffers stays hidden.
+#pragma once
+#include "gemm_common.cuh"
+
+namespace maize {
+
+constexpr uint32_t kF8BlockK = 128;        // e4m3 elements per k-block = one 128-byte swizzle row = one scale
+constexpr uint32_t kF8UmmaK = 32;          // K per tcgen05.mma for 8-bit operands
+constexpr uint32_t kF8PromoteWarps = 8;    // two per quarter of the lanes: columns 0-127 and 128-255
+constexpr uint32_t kF8Threads = 64 + 32 * kF8PromoteWarps;
+
+struct F8Params {
+    GemmParams g;
+    const float *sa, *sb;
+    uint64_t ld_sa, ld_sb;  // row pitches of the scales
+};
+
+template <uint32_t STAGES>
+struct F8SmemLayout {
+    static constexpr uint32_t kABytes = kBlockM * kF8BlockK;
+    static constexpr uint32_t kBBytes = 128 * kF8BlockK;  // this CTA's half of the 256 columns
+    static constexpr uint32_t kStageBytes = kABytes + kBBytes;
+    static constexpr uint32_t kStagingOffset = STAGES * kStageBytes;
+    static constexpr uint32_t kStagingBytes = kF8PromoteWarps * kTmaStoreBufBytes;
+    static constexpr uint32_t kBarOffset = kStagingOffset + kStagingBytes;
+    static constexpr uint32_t kNumBars = 2 * STAGES + 4;
+    static constexpr uint32_t kTmemSlotOffset = kBarOffset + kNumBars * 8;
+    static constexpr uint32_t kAbortOffset = kTmemSlotOffset + 4;
+    static constexpr uint32_t kUsedBytes = kAbortOffset + 4;
+    static constexpr uint32_t kDynamicBytes = kUsedBytes + 1024;
+    static_assert(kDynamicBytes <= 232448, "exceeds 227 KiB of shared memory per CTA");
+    static_assert(kDynamicBytes > 116224, "two CTAs could share an SM and contend for TMEM");
+    static_assert(kStageWarpBytes <= kTmaStoreBufBytes, "the ragged epilogue's staging is carved out of the TMA one");
+};
+
+// Writes this warp's 32 rows x 128 columns of C, held as 128 fp32 per lane (lane = row).
+__device__ __forceinline__ void f8_store(const GemmParams &p, const CUtensorMap *tma_c, uint8_t *stage_gen,
+                                         uint32_t stage_u32, uint32_t lane, uint32_t row0, uint32_t col0,
+                                         const float (&acc)[128])
+{
+    if (row0 >= p.m)
+        return;
+    if (p.c_tma_ok) {
+#pragma unroll
+        for (uint32_t g = 0; g < 2; ++g) {
+            const uint32_t col = col0 + g * 64u;
+            if (col < p.n) {
+                if (lane == 0)
+                    ptx::bulk_wait_group_read<0>();  // the warp's one staging buffer has been read
+                __syncwarp();
+                const uint32_t row = stage_u32 + lane * 128u;
+                const uint32_t sw = lane & 7u;
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j) {
+                    const float *v = acc + g * 64 + 8 * j;
+                    ptx::st_shared_v4(row + ((j ^ sw) << 4), ptx::pack_bf16x2(__float_as_uint(v[0]), __float_as_uint(v[1])),
+                                      ptx::pack_bf16x2(__float_as_uint(v[2]), __float_as_uint(v[3])),
+                                      ptx::pack_bf16x2(__float_as_uint(v[4]), __float_as_uint(v[5])),
+                                      ptx::pack_bf16x2(__float_as_uint(v[6]), __float_as_uint(v[7])));
+                }
+                ptx::fence_proxy_async_shared();
+                __syncwarp();
+                if (lane == 0) {
+                    ptx::tma_store_2d(tma_c, stage_u32, static_cast<int32_t>(col), static_cast<int32_t>(row0));
+                    ptx::bulk_commit_group();
+                }
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (uint32_t g = 0; g < 4; ++g) {
+        uint32_t v[32];
+#pragma unroll
+        for (uint32_t i = 0; i < 32; ++i)
+            v[i] = __float_as_uint(acc[g * 32 + i]);
+        store_chunk(p, stage_gen, row0, col0 + g * 32u, lane, v);
+        __syncwarp();
+    }
+}
+
+template <uint32_t STAGES>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kF8Threads, 1)
+gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
+                     const __grid_constant__ CUtensorMap tma_c, const F8Params f)
+{
+    using L = F8SmemLayout<STAGES>;
+    constexpr uint32_t kTmemCols = 512;
+    constexpr uint32_t kIdesc = ptx::make_instr_desc_e4m3(2 * kBlockM, 256);
+    const GemmParams &p = f.g;
+
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
+
+    const uint32_t bar_base = smem_base + L::kBarOffset;
+    auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };
+    auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (STAGES + s); };
+    auto acc_full_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + b); };
+    auto acc_empty_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + 2 + b); };
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + L::kTmemSlotOffset);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem_gen + L::kAbortOffset);
+
+    const uint32_t warp = threadIdx.x >> 5;
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint32_t cta_rank = ptx::cluster_cta_rank();
+    const uint32_t pair = blockIdx.x >> 1;
+    const uint32_t num_pairs = gridDim.x >> 1;
+    const uint32_t num_tiles = p.tiles_m * p.tiles_n;
+    const uint32_t num_kb = (p.k + kF8BlockK - 1) / kF8BlockK;
+    const WaitCtl ctl{abort_flag, p.status, p.timeout_ns};
+
+    if (threadIdx.x == 0) {
+        ptx::prefetch_tensormap(&tma_a);
+        ptx::prefetch_tensormap(&tma_b);
+        if (p.c_tma_ok)
+            ptx::prefetch_tensormap(&tma_c);
+        for (uint32_t s = 0; s < STAGES; ++s) {
+            ptx::mbar_init(full_bar(s), 1);
+            ptx::mbar_init(empty_bar(s), 1);
+        }
+        for (uint32_t b = 0; b < 2; ++b) {
+            ptx::mbar_init(acc_full_bar(b), 1);
+            ptx::mbar_init(acc_empty_bar(b), 2 * kF8PromoteWarps);  // one lane per promotion warp of both CTAs
+        }
+        *abort_flag = 0;
+        ptx::fence_barrier_init();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc_2cta(ptx::smem_u32(const_cast<uint32_t *>(tmem_slot)), kTmemCols);
+        ptx::tmem_relinquish_2cta();
+    }
+    ptx::tcgen05_fence_before();
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+    ptx::tcgen05_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    if (p.pdl) {
+        if (threadIdx.x == 0)
+            ptx::grid_dependency_launch_dependents();
+        ptx::grid_dependency_wait();
+    }
+
+    bool role_ok = true;
+    if (warp == 0) {
+        // ------------------------------------------------------- TMA producer --
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            bool ok = true;
+            for (uint32_t t = pair; ok && t < num_tiles; t += num_pairs) {
+                const TileCoord tc = tile_coord(t, p);
+                const int32_t m0 = static_cast<int32_t>(tc.m_blk * 2 * kBlockM + cta_rank * kBlockM);
+                const int32_t n0 = static_cast<int32_t>(tc.n_blk * 256u + cta_rank * 128u);
+                for (uint32_t kb = 0; kb < num_kb; ++kb) {
+                    ok = wait_bounded<true>(empty_bar(stage), phase ^ 1u, ctl, 1);
+                    if (!ok)
+                        break;
+                    const uint32_t sa = smem_base + stage * L::kStageBytes;
+                    const uint32_t leader_full = ptx::mapa_shared(full_bar(stage), 0);
+                    if (cta_rank == 0)
+                        ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * L::kStageBytes);
+                    const int32_t kx = static_cast<int32_t>(kb * kF8BlockK);
+                    ptx::tma_load_2d_pair(sa, &tma_a, leader_full, kx, m0);
+                    ptx::tma_load_2d_pair(sa + L::kABytes, &tma_b, leader_full, kx, n0);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            role_ok = ok;
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------- MMA issuer (leader only) --
+        if (lane == 0 && cta_rank == 0) {
+            uint32_t stage = 0, phase = 0;
+            uint32_t acc = 0, acc_phase = 0;
+            bool ok = true;
+            for (uint32_t t = pair; ok && t < num_tiles; t += num_pairs) {
+                for (uint32_t kb = 0; kb < num_kb; ++kb) {
+                    ok = wait_bounded<true>(acc_empty_bar(acc), acc_phase ^ 1u, ctl, 2) &&
+                         wait_bounded<true>(full_bar(stage), phase, ctl, 2);
+                    if (!ok)
+                        break;
+                    ptx::tcgen05_fence_after();
+                    const uint32_t sa = smem_base + stage * L::kStageBytes;
+                    const uint64_t da = ptx::make_smem_desc_sw128(sa);
+                    const uint64_t db = ptx::make_smem_desc_sw128(sa + L::kABytes);
+                    const uint32_t tmem_d = tmem_base + acc * 256u;
+#pragma unroll
+                    for (uint32_t k = 0; k < kF8BlockK / kF8UmmaK; ++k)
+                        ptx::mma_f8_2cta(tmem_d, da + 2u * k, db + 2u * k, kIdesc, k != 0u ? 1u : 0u);
+                    ptx::mma_commit_2cta_mask(empty_bar(stage), 3);
+                    ptx::mma_commit_2cta_mask(acc_full_bar(acc), 3);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                    if (++acc == 2) {
+                        acc = 0;
+                        acc_phase ^= 1u;
+                    }
+                }
+            }
+            role_ok = ok;
+        }
+        __syncwarp();
+    } else {
+        // ---------------------------------------------- promotion and epilogue --
+        const uint32_t quarter = warp & 3u;
+        const uint32_t half = (warp - 2u) >> 2;
+        uint8_t *stage_gen = smem_gen + L::kStagingOffset + (warp - 2u) * kTmaStoreBufBytes;
+        const uint32_t stage_u32 = smem_base + L::kStagingOffset + (warp - 2u) * kTmaStoreBufBytes;
+        const uint32_t lane_cols = tmem_base + ((quarter * 32u) << 16) + half * 128u;
+        const uint32_t leader_empty0 = ptx::mapa_shared(acc_empty_bar(0), 0);
+        uint32_t buf = 0, buf_phase = 0;
+        bool ok = true;
+        for (uint32_t t = pair; ok && t < num_tiles; t += num_pairs) {
+            const TileCoord tc = tile_coord(t, p);
+            const uint32_t row0 = tc.m_blk * 2 * kBlockM + cta_rank * kBlockM + quarter * 32u;
+            const uint32_t col0 = tc.n_blk * 256u + half * 128u;
+            const bool row_in = row0 + lane < p.m, col_in = col0 < p.n;
+            const float *sa = f.sa + static_cast<uint64_t>(row_in ? row0 + lane : 0u) * f.ld_sa;
+            const float *sb = f.sb + static_cast<uint64_t>(col_in ? col0 / 128u : 0u) * f.ld_sb;
+            float acc[128];
+#pragma unroll
+            for (int i = 0; i < 128; ++i)
+                acc[i] = 0.0f;
+            float s_a = row_in ? __ldg(sa) : 0.0f, s_b = col_in ? __ldg(sb) : 0.0f;
+            for (uint32_t kb = 0; kb < num_kb; ++kb) {
+                const float s = s_a * s_b;
+                if (kb + 1 < num_kb) {  // the next block's scales, fetched behind this one's work
+                    s_a = row_in ? __ldg(sa + kb + 1) : 0.0f;
+                    s_b = col_in ? __ldg(sb + kb + 1) : 0.0f;
+                }
+                ok = wait_bounded<true>(acc_full_bar(buf), buf_phase, ctl, 3);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok)
+                    break;
+                ptx::tcgen05_fence_after();
+                const uint32_t taddr = lane_cols + buf * 256u;
+#pragma unroll
+                for (uint32_t c = 0; c < 4; ++c) {
+                    uint32_t v[32];
+                    ptx::tmem_ld_32x32b_x32(taddr + c * 32u, v);
+                    ptx::tmem_ld_wait();
+                    if (c == 3) {
+                        ptx::tcgen05_fence_before();
+                        __syncwarp();
+                        if (lane == 0)
+                            ptx::mbar_arrive_cluster_addr(leader_empty0 + 8u * buf);
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; ++i)
+                        acc[c * 32 + i] = fmaf(__uint_as_float(v[i]), s, acc[c * 32 + i]);
+                }
+                if (++buf == 2) {
+                    buf = 0;
+                    buf_phase ^= 1u;
+                }
+            }
+            if (!ok)
+                break;
+            f8_store(p, &tma_c, stage_gen, stage_u32, lane, row0, col0, acc);
+            __syncwarp();
+        }
+        if (p.c_tma_ok)
+            tma_store_drain(lane);
+        role_ok = ok;
+    }
+    if (!role_ok)
+        ptx::st_shared_cluster_u32(ptx::mapa_shared(ptx::smem_u32(const_cast<int *>(abort_flag)), cta_rank ^ 1u), 1u);
+
+    // ---------------------------------------------------------------- teardown --
+    __syncwarp();
+    ptx::tcgen05_fence_before();
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+    if (warp == 1) {
+        if (*abort_flag) {
+            for (int i = 0; i < 256; ++i)
+                __nanosleep(1000);
+        }
+        ptx::tcgen05_fence_after();
+        ptx::tmem_dealloc_2cta(tmem_base, kTmemCols);
+    }
+}
+
+}  // namespace maize

@@ -1,0 +1,153 @@
+// C ABI of the 8-bit products and their quantiser (declared in include/maize_gemm.h).
+#include "../../include/maize_gemm.h"
+
+#include <cstring>
+
+#include "maize_host.cuh"
+#include "gemm_e4m3_sm100.cuh"
+#include "quantize_e4m3.cuh"
+
+namespace {
+
+using maize::aligned;
+using maize::DeviceGuard;
+using maize::fail;
+using maize::fail_cuda;
+
+maize_status_t byte_map(maize_ctx_t *ctx, CUtensorMap *map, const void *base, uint64_t rows, uint64_t cols, uint64_t ld,
+                        uint32_t box_rows)
+{
+    const uint64_t dims[2] = {cols, rows}, strides[1] = {ld};
+    const uint32_t box[2] = {maize::kF8BlockK, box_rows};
+    return maize::encode_map(ctx, map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, 2, dims, strides, box,
+                             static_cast<CUtensorMapL2promotion>(ctx->tma_promotion));
+}
+
+}  // namespace
+
+extern "C" {
+
+maize_status_t maize_quantize_e4m3(maize_ctx_t *ctx, const void *x, uint64_t ldx, uint32_t rows, uint32_t cols,
+                                   uint32_t block_rows, void *q, uint64_t ldq, void *scales, uint64_t ld_scales,
+                                   void *cuda_stream)
+{
+    if (!ctx)
+        return MAIZE_ERR_INVALID_ARG;
+    ctx->err.clear();
+    if (block_rows != 1 && block_rows != maize::kQuantBlock)
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "block_rows must be 1 or 128");
+    if (rows == 0 || cols == 0)
+        return MAIZE_OK;
+    if (!x || !q || !scales)
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "null pointer");
+    if (!aligned(x, 2) || !aligned(scales, 4))
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "x must be 2-byte and scales 4-byte aligned");
+    if (rows > maize::kMaxDim || cols > maize::kMaxDim)
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "rows or cols beyond the kernel's range");
+    const uint64_t across = (uint64_t(cols) + 127) / 128;
+    if (ldx < cols || ldq < cols || ld_scales < across)
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "a leading dimension is smaller than its row");
+    maize::QuantParams p = {};
+    p.x = static_cast<const __nv_bfloat16 *>(x);
+    p.ldx = ldx;
+    p.q = static_cast<uint8_t *>(q);
+    p.ldq = ldq;
+    p.scales = static_cast<float *>(scales);
+    p.ld_scales = ld_scales;
+    p.rows = rows;
+    p.cols = cols;
+    p.pdl = ctx->pdl;
+    const bool vec = ldx % 8 == 0 && aligned(x, 16) && ldq % 8 == 0 && aligned(q, 8);
+    DeviceGuard guard(ctx->device);
+    cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    if (block_rows == 1) {
+        const uint64_t blocks = uint64_t(rows) * across;
+        const uint64_t want = (blocks + 15) / 16, cap = uint64_t(ctx->sm_count) * 8;
+        const uint32_t grid = static_cast<uint32_t>(want < cap ? want : cap);
+        return vec ? maize::launch(ctx, -1, maize::quantize_rows_kernel<true>, grid, 256, 0, stream, p)
+                   : maize::launch(ctx, -1, maize::quantize_rows_kernel<false>, grid, 256, 0, stream, p);
+    }
+    const uint64_t blocks = (uint64_t(rows) + 127) / 128 * across;
+    if (blocks > 0x7fffffffull)
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "too many blocks");
+    return vec ? maize::launch(ctx, -1, maize::quantize_blocks_kernel<true>, static_cast<uint32_t>(blocks), 256, 0, stream, p)
+               : maize::launch(ctx, -1, maize::quantize_blocks_kernel<false>, static_cast<uint32_t>(blocks), 256, 0, stream, p);
+}
+
+maize_status_t maize_gemm_e4m3(maize_ctx_t *ctx, const void *a, uint64_t lda, const void *a_scales, uint64_t ld_a_scales,
+                               const void *b, uint64_t ldb, const void *b_scales, uint64_t ld_b_scales, void *c,
+                               uint64_t ldc, uint32_t m, uint32_t n, uint32_t k, void *cuda_stream)
+{
+    if (!ctx)
+        return MAIZE_ERR_INVALID_ARG;
+    ctx->err.clear();
+    if (m == 0 || n == 0)
+        return MAIZE_OK;
+    if (!c)
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "C pointer is null");
+    if (ldc < n)
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "ldc is smaller than N");
+    if (!aligned(c, 2))
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "C must be 2-byte aligned");
+    if (m > maize::kMaxDim || n > maize::kMaxDim || k > maize::kMaxDim)
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "a dimension is beyond the kernel's range");
+    DeviceGuard guard(ctx->device);
+    cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+    if (k == 0) {
+        const cudaError_t e = cudaMemset2DAsync(c, ldc * 2, 0, size_t(n) * 2, m, stream);
+        return e == cudaSuccess ? MAIZE_OK : fail_cuda(ctx, "cudaMemset2DAsync", e);
+    }
+    if (!a || !b || !a_scales || !b_scales)
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "an operand or scale pointer is null");
+    const uint64_t kblocks = (uint64_t(k) + 127) / 128;
+    if (lda < k || ldb < k || ld_a_scales < kblocks || ld_b_scales < kblocks)
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "a leading dimension is smaller than its row");
+    if (!aligned(a_scales, 4) || !aligned(b_scales, 4))
+        return fail(ctx, MAIZE_ERR_INVALID_ARG, "scales must be 4-byte aligned");
+    if (k % 16 != 0 || lda % 16 != 0 || ldb % 16 != 0)
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "K, lda and ldb must be multiples of 16 (16-byte TMA row pitch)");
+    if (!aligned(a, 16) || !aligned(b, 16))
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "A and B must be 16-byte aligned");
+    if (lda >= (1ull << 40) || ldb >= (1ull << 40))
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "row pitch beyond the TMA limit of 2^40 bytes");
+    CUtensorMap ta, tb, tc;
+    maize_status_t st;
+    if ((st = byte_map(ctx, &ta, a, m, k, lda, maize::kBlockM)) != MAIZE_OK ||
+        (st = byte_map(ctx, &tb, b, n, k, ldb, 128)) != MAIZE_OK)
+        return st;
+    memset(&tc, 0, sizeof tc);
+    maize::F8Params f = {};
+    maize::GemmParams &p = f.g;
+    p.c = static_cast<__nv_bfloat16 *>(c);
+    p.ldc = ldc;
+    p.m = m;
+    p.n = n;
+    p.k = k;
+    p.tiles_m = static_cast<uint32_t>((uint64_t(m) + 255) / 256);
+    p.tiles_n = static_cast<uint32_t>((uint64_t(n) + 255) / 256);
+    p.group_m = (ctx->group_rows != 0 ? ctx->group_rows : 2048u) / 256u;
+    if (p.group_m == 0)
+        p.group_m = 1;
+    p.serpentine = ctx->serpentine;
+    p.pdl = ctx->pdl;
+    p.status = ctx->d_status;
+    p.timeout_ns = ctx->timeout_ns;
+    f.sa = static_cast<const float *>(a_scales);
+    f.sb = static_cast<const float *>(b_scales);
+    f.ld_sa = ld_a_scales;
+    f.ld_sb = ld_b_scales;
+    const bool c_rows_aligned = ldc % 8 == 0 && aligned(c, 16);
+    p.c_vec_ok = c_rows_aligned ? 1u : 0u;
+    if (ctx->tma_store && c_rows_aligned && n % 8 == 0 && ldc * 2 < (1ull << 40)) {
+        p.c_tma_ok = maize::matrix_map(ctx, &tc, c, m, n, ldc, 32) == MAIZE_OK;
+        ctx->err.clear();
+    }
+    const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n;
+    if (tiles > 0x7fffffffull)
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "too many output tiles");
+    const uint32_t grid = maize::persistent_grid(ctx, tiles, 2);
+    return maize::launch(ctx, maize::kAttrE4m3, maize::gemm_e4m3_sm100_2cta<6>, grid, maize::kF8Threads,
+                         maize::F8SmemLayout<6>::kDynamicBytes, stream, ta, tb, tc, f);
+}
+
+}  // extern "C"

@@ -3,10 +3,9 @@
 // everything else.
 #include "../../include/maize_gemm.h"
 
-#include <cstdio>
 #include <cstring>
 
-#include "maize_ctx.cuh"
+#include "maize_host.cuh"
 #include "gemm_sm100_grouped.cuh"
 #include "gemm_sm100_grouped_wgrad.cuh"
 
@@ -17,94 +16,12 @@ using maize::fail;
 using maize::fail_cuda;
 using maize::GroupedParams;
 
-constexpr uint32_t kMaxRows = 0x7fffff00u;  // row numbers are 32-bit offsets and TMA coordinates; room for a tile past the end
-constexpr uint32_t kMaxDim = 0x7fffff00u;
-
-// ctx->attr_experts slots
-enum { kAttrGrouped = 0, kAttrGroupedKn = 1, kAttrWgrad = 2 };
-
-bool aligned(const void *p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
-
-maize_status_t encode_map(maize_ctx_t *ctx, CUtensorMap *map, CUtensorMapDataType type, uint32_t element_bytes,
-                          const void *base, uint32_t rank, const uint64_t *dims, const uint64_t *strides,
-                          const uint32_t *box_dims, CUtensorMapL2promotion promotion)
-{
-    cuuint64_t gdim[3], gstride[2];
-    cuuint32_t box[3], estride[3] = {1, 1, 1};
-    for (uint32_t i = 0; i < rank; ++i) {
-        gdim[i] = dims[i];
-        box[i] = box_dims[i];
-        if (i + 1 < rank)
-            gstride[i] = strides[i] * element_bytes;
-    }
-    const CUresult r = ctx->encode(map, type, rank, const_cast<void *>(base), gdim, gstride, box, estride,
-                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, promotion,
-                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r == CUDA_SUCCESS)
-        return MAIZE_OK;
-    char buf[160];
-    snprintf(buf, sizeof buf, "cuTensorMapEncodeTiled failed (CUresult %d) for %llu x %llu, ld %llu", (int)r,
-             (unsigned long long)dims[1], (unsigned long long)dims[0], (unsigned long long)strides[0]);
-    return fail(ctx, MAIZE_ERR_CUDA, buf);
-}
-
-// [rows x cols] bf16, boxes of box_rows x 64.
-maize_status_t matrix_map(maize_ctx_t *ctx, CUtensorMap *map, const void *base, uint64_t rows, uint64_t cols, uint64_t ld,
-                          uint32_t box_rows)
-{
-    const uint64_t dims[2] = {cols, rows}, strides[1] = {ld};
-    const uint32_t box[2] = {maize::kBlockK, box_rows};
-    return encode_map(ctx, map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, 2, dims, strides, box,
-                      static_cast<CUtensorMapL2promotion>(ctx->tma_promotion));
-}
-
-// A stack of `count` bf16 matrices [rows x cols], `stride` elements apart, boxes of 1 x box_rows x 64.
-maize_status_t stack_map(maize_ctx_t *ctx, CUtensorMap *map, const void *base, uint64_t count, uint64_t rows, uint64_t cols,
-                         uint64_t ld, uint64_t stride, uint32_t box_rows, CUtensorMapL2promotion promotion)
-{
-    const uint64_t dims[3] = {cols, rows, count}, strides[2] = {ld, stride};
-    const uint32_t box[3] = {maize::kBlockK, box_rows, 1};
-    return encode_map(ctx, map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, 3, dims, strides, box, promotion);
-}
-
-template <typename Kernel, typename... Args>
-maize_status_t launch(maize_ctx_t *ctx, int attr_slot, Kernel kernel, uint32_t grid, uint32_t threads, uint32_t smem,
-                      cudaStream_t stream, const Args &...args)
-{
-    if (!ctx->attr_experts[attr_slot]) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess)
-            return fail_cuda(ctx, "cudaFuncSetAttribute(max dynamic smem)", e);
-        ctx->attr_experts[attr_slot] = true;
-    }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = ctx->pdl ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-    if (e != cudaSuccess)
-        return fail_cuda(ctx, "kernel launch", e);
-    ctx->launches += 1;
-    return MAIZE_OK;
-}
-
-// CTAs that may run at a time, a multiple of `unit` (the cluster size), at most what `tiles` clusters need.
-uint32_t persistent_grid(const maize_ctx_t *ctx, uint64_t tiles, uint32_t unit)
-{
-    uint32_t cap = static_cast<uint32_t>(ctx->sm_count);
-    if (ctx->max_ctas > 0 && static_cast<uint32_t>(ctx->max_ctas) < cap)
-        cap = static_cast<uint32_t>(ctx->max_ctas);
-    cap /= unit;
-    if (cap == 0)
-        cap = 1;
-    return (tiles < cap ? static_cast<uint32_t>(tiles) : cap) * unit;
-}
+using maize::aligned;
+using maize::kMaxDim;
+using maize::launch;
+using maize::matrix_map;
+using maize::persistent_grid;
+using maize::stack_map;
 
 // What the three grouped entry points check alike.
 maize_status_t check_groups(maize_ctx_t *ctx, const void *offsets, uint32_t groups, uint32_t rows)
@@ -113,7 +30,7 @@ maize_status_t check_groups(maize_ctx_t *ctx, const void *offsets, uint32_t grou
         return fail(ctx, MAIZE_ERR_INVALID_ARG, "offsets must be a 4-byte aligned device array of groups + 1 integers");
     if (groups > maize::kGroupedMaxGroups)
         return fail(ctx, MAIZE_ERR_UNSUPPORTED, "more than 1024 groups");
-    if (rows > kMaxRows)
+    if (rows > kMaxDim)
         return fail(ctx, MAIZE_ERR_UNSUPPORTED, "too many rows for 32-bit offsets");
     return MAIZE_OK;
 }
@@ -194,9 +111,9 @@ maize_status_t grouped_impl(maize_ctx_t *ctx, const void *a, uint64_t lda, const
     const uint64_t row_tiles = rows / maize::kGroupedTileRows + (rows < groups ? rows : groups);
     const uint32_t grid = persistent_grid(ctx, row_tiles * n_blocks, 2);
     using L = maize::GroupedSmemLayout<6>;
-    return b_kn ? launch(ctx, kAttrGroupedKn, maize::gemm_bf16_sm100_grouped<true, 6>, grid, maize::kNumThreads,
+    return b_kn ? launch(ctx, maize::kAttrGroupedKn, maize::gemm_bf16_sm100_grouped<true, 6>, grid, maize::kNumThreads,
                          L::kDynamicBytes, stream, ta, tw, p)
-                : launch(ctx, kAttrGrouped, maize::gemm_bf16_sm100_grouped<false, 6>, grid, maize::kNumThreads,
+                : launch(ctx, maize::kAttrGrouped, maize::gemm_bf16_sm100_grouped<false, 6>, grid, maize::kNumThreads,
                          L::kDynamicBytes, stream, ta, tw, p);
 }
 
@@ -294,7 +211,7 @@ maize_status_t maize_grouped_gemm_bf16_wgrad(maize_ctx_t *ctx, const void *a, ui
         ctx->err.clear();
     }
     const uint32_t grid = persistent_grid(ctx, tiles, 2);
-    return launch(ctx, kAttrWgrad, maize::gemm_bf16_sm100_grouped_wgrad<5>, grid, maize::kWgradThreads,
+    return launch(ctx, maize::kAttrWgrad, maize::gemm_bf16_sm100_grouped_wgrad<5>, grid, maize::kWgradThreads,
                   maize::WgradSmemLayout<5>::kDynamicBytes, stream, tdc, ta, tdw, p);
 }
 

@@ -330,6 +330,63 @@ class Context:
             out.stride(0), offsets.data_ptr(), groups, rows, n, k, self._stream(stream)))
         return out
 
+    # ------------------------------------------------------ 8-bit products --
+    def quantize_e4m3(self, x, block_rows: int = 1, out=None, scales=None, stream=None):
+        """bf16 rows x cols -> (e4m3 tensor of the same shape, fp32 scales), with a power-of-two scale for each 1 x 128
+        (``block_rows`` = 1: activations) or 128 x 128 block (``block_rows`` = 128: weights): ``x ~ q * scale``."""
+        import torch
+        self._own("x", x, 2, torch.bfloat16)
+        rows, cols = x.shape
+        if block_rows not in (1, 128):
+            raise MaizeError(_ffi.INVALID_ARG, "block_rows must be 1 or 128")
+        shape = (-(-rows // block_rows), -(-cols // 128))
+        if out is None:
+            out = self._new((rows, cols), torch.float8_e4m3fn, stream)
+        else:
+            self._own("out", out, 2, torch.float8_e4m3fn)
+            if out.shape != x.shape:
+                raise MaizeError(_ffi.INVALID_ARG, f"out: expected {rows} x {cols}")
+        if scales is None:
+            scales = self._new(shape, torch.float32, stream)
+        else:
+            self._own("scales", scales, 2, torch.float32)
+            if scales.shape != shape:
+                raise MaizeError(_ffi.INVALID_ARG, f"scales: expected {shape[0]} x {shape[1]}")
+        self._check(self._lib.maize_quantize_e4m3(
+            self._h, x.data_ptr(), x.stride(0) if rows > 1 else max(cols, 1), rows, cols, block_rows, out.data_ptr(),
+            out.stride(0) if rows > 1 else max(cols, 1), scales.data_ptr(),
+            scales.stride(0) if shape[0] > 1 else max(shape[1], 1), self._stream(stream)))
+        return out, scales
+
+    def gemm_e4m3(self, a, a_scales, b, b_scales, out=None, stream=None):
+        """``out = (a * a_scales) @ (b * b_scales).T`` in bf16 for e4m3 a (M x K) with a scale for each 1 x 128 block
+        (M x ceil(K/128), fp32) and e4m3 b (N x K) with one for each 128 x 128 block (ceil(N/128) x ceil(K/128))."""
+        import torch
+        f8 = torch.float8_e4m3fn
+        self._own("a", a, 2, f8)
+        self._own("b", b, 2, f8)
+        self._own("a_scales", a_scales, 2, torch.float32)
+        self._own("b_scales", b_scales, 2, torch.float32)
+        m, k = a.shape
+        n, kb = b.shape
+        if k != kb:
+            raise MaizeError(_ffi.INVALID_ARG, "a.shape[1] != b.shape[1] (b is stored N x K)")
+        blocks = -(-k // 128)
+        if a_scales.shape != (m, blocks) or b_scales.shape != (-(-n // 128), blocks):
+            raise MaizeError(_ffi.INVALID_ARG, f"scales: expected {m} x {blocks} for a, {-(-n // 128)} x {blocks} for b")
+        if out is None:
+            out = self._new((m, n), torch.bfloat16, stream)
+        else:
+            self._own("out", out, 2, torch.bfloat16)
+            if out.shape != (m, n):
+                raise MaizeError(_ffi.INVALID_ARG, f"out: expected {m} x {n}")
+        self._check(self._lib.maize_gemm_e4m3(
+            self._h, a.data_ptr(), a.stride(0) if m > 1 else k, a_scales.data_ptr(),
+            a_scales.stride(0) if m > 1 else blocks, b.data_ptr(), b.stride(0) if n > 1 else k, b_scales.data_ptr(),
+            b_scales.stride(0) if n > 128 else blocks, out.data_ptr(), out.stride(0) if m > 1 else max(n, 1), m, n, k,
+            self._stream(stream)))
+        return out
+
     def debug_wait_expires(self, budget_ns: int, stream=None) -> None:
         self._check(self._lib.maize_debug_wait_expires(self._h, int(budget_ns), _stream_handle(stream)))
 
@@ -371,6 +428,16 @@ def grouped_gemm_kn(a, b, offsets, out=None, stream=None):
 def grouped_gemm_wgrad(a, dc, offsets, out=None, stream=None):
     """``Context.grouped_gemm_wgrad`` over a cached Context of a's device."""
     return _context_of(a).grouped_gemm_wgrad(a, dc, offsets, out, stream)
+
+
+def quantize_e4m3(x, block_rows: int = 1, out=None, scales=None, stream=None):
+    """``Context.quantize_e4m3`` over a cached Context of x's device."""
+    return _context_of(x).quantize_e4m3(x, block_rows, out, scales, stream)
+
+
+def gemm_e4m3(a, a_scales, b, b_scales, out=None, stream=None):
+    """``Context.gemm_e4m3`` over a cached Context of a's device."""
+    return _context_of(a).gemm_e4m3(a, a_scales, b, b_scales, out, stream)
 
 
 def gemm_skinny_static(a, b, out, stream=None, device_status=None):
