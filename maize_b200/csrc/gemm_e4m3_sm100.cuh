@@ -21,7 +21,12 @@ namespace maize {
 constexpr uint32_t kF8BlockK = 128;        // e4m3 elements per k-block = one 128-byte swizzle row = one scale
 constexpr uint32_t kF8UmmaK = 32;          // K per tcgen05.mma for 8-bit operands
 constexpr uint32_t kF8PromoteWarps = 8;    // two per quarter of the lanes: columns 0-127 and 128-255
-constexpr uint32_t kF8Threads = 64 + 32 * kF8PromoteWarps;
+constexpr uint32_t kF8ControlWarps = 4;    // producer, MMA issuer, two idle: a whole warpgroup, so that it can give registers away
+constexpr uint32_t kF8Threads = 32 * (kF8ControlWarps + kF8PromoteWarps);
+// 384 threads are launched with 168 registers each (504 over the three warpgroups); the control warpgroup keeps 72, the two
+// promotion warpgroups take 216 each: 72 + 2 * 216 = 504.
+constexpr int kF8ControlRegs = 56;
+constexpr int kF8PromoteRegs = 224;
 
 struct F8Params {
     GemmParams g;
@@ -50,7 +55,7 @@ struct F8SmemLayout {
 // Writes this warp's 32 rows x 128 columns of C, held as 128 fp32 per lane (lane = row).
 __device__ __forceinline__ void f8_store(const GemmParams &p, const CUtensorMap *tma_c, uint8_t *stage_gen,
                                          uint32_t stage_u32, uint32_t lane, uint32_t row0, uint32_t col0,
-                                         const float (&acc)[128])
+                                         const uint64_t (&acc)[64])
 {
     if (row0 >= p.m)
         return;
@@ -66,11 +71,14 @@ __device__ __forceinline__ void f8_store(const GemmParams &p, const CUtensorMap 
                 const uint32_t sw = lane & 7u;
 #pragma unroll
                 for (uint32_t j = 0; j < 8; ++j) {
-                    const float *v = acc + g * 64 + 8 * j;
-                    ptx::st_shared_v4(row + ((j ^ sw) << 4), ptx::pack_bf16x2(__float_as_uint(v[0]), __float_as_uint(v[1])),
-                                      ptx::pack_bf16x2(__float_as_uint(v[2]), __float_as_uint(v[3])),
-                                      ptx::pack_bf16x2(__float_as_uint(v[4]), __float_as_uint(v[5])),
-                                      ptx::pack_bf16x2(__float_as_uint(v[6]), __float_as_uint(v[7])));
+                    uint32_t w[4];
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        uint32_t lo, hi;
+                        ptx::unpack_f32x2(acc[g * 32 + 4 * j + i], lo, hi);
+                        w[i] = ptx::pack_bf16x2(lo, hi);
+                    }
+                    ptx::st_shared_v4(row + ((j ^ sw) << 4), w[0], w[1], w[2], w[3]);
                 }
                 ptx::fence_proxy_async_shared();
                 __syncwarp();
@@ -86,8 +94,8 @@ __device__ __forceinline__ void f8_store(const GemmParams &p, const CUtensorMap 
     for (uint32_t g = 0; g < 4; ++g) {
         uint32_t v[32];
 #pragma unroll
-        for (uint32_t i = 0; i < 32; ++i)
-            v[i] = __float_as_uint(acc[g * 32 + i]);
+        for (uint32_t i = 0; i < 16; ++i)
+            ptx::unpack_f32x2(acc[g * 16 + i], v[2 * i], v[2 * i + 1]);
         store_chunk(p, stage_gen, row0, col0 + g * 32u, lane, v);
         __syncwarp();
     }
@@ -156,6 +164,8 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
     }
 
     bool role_ok = true;
+    if (warp < kF8ControlWarps) {
+        ptx::setmaxnreg_dec<kF8ControlRegs>();
     if (warp == 0) {
         // ------------------------------------------------------- TMA producer --
         if (lane == 0) {
@@ -220,12 +230,14 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
             role_ok = ok;
         }
         __syncwarp();
+    }
     } else {
+        ptx::setmaxnreg_inc<kF8PromoteRegs>();
         // ---------------------------------------------- promotion and epilogue --
         const uint32_t quarter = warp & 3u;
-        const uint32_t half = (warp - 2u) >> 2;
-        uint8_t *stage_gen = smem_gen + L::kStagingOffset + (warp - 2u) * kTmaStoreBufBytes;
-        const uint32_t stage_u32 = smem_base + L::kStagingOffset + (warp - 2u) * kTmaStoreBufBytes;
+        const uint32_t half = (warp - kF8ControlWarps) >> 2;
+        uint8_t *stage_gen = smem_gen + L::kStagingOffset + (warp - kF8ControlWarps) * kTmaStoreBufBytes;
+        const uint32_t stage_u32 = smem_base + L::kStagingOffset + (warp - kF8ControlWarps) * kTmaStoreBufBytes;
         const uint32_t lane_cols = tmem_base + ((quarter * 32u) << 16) + half * 128u;
         const uint32_t leader_empty0 = ptx::mapa_shared(acc_empty_bar(0), 0);
         uint32_t buf = 0, buf_phase = 0;
@@ -237,10 +249,10 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
             const bool row_in = row0 + lane < p.m, col_in = col0 < p.n;
             const float *sa = f.sa + static_cast<uint64_t>(row_in ? row0 + lane : 0u) * f.ld_sa;
             const float *sb = f.sb + static_cast<uint64_t>(col_in ? col0 / 128u : 0u) * f.ld_sb;
-            float acc[128];
+            uint64_t acc[64];  // 128 fp32 in pairs of neighbouring columns
 #pragma unroll
-            for (int i = 0; i < 128; ++i)
-                acc[i] = 0.0f;
+            for (int i = 0; i < 64; ++i)
+                acc[i] = 0ull;
             float s_a = row_in ? __ldg(sa) : 0.0f, s_b = col_in ? __ldg(sb) : 0.0f;
             for (uint32_t kb = 0; kb < num_kb; ++kb) {
                 const float s = s_a * s_b;
@@ -254,20 +266,25 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
                     break;
                 ptx::tcgen05_fence_after();
                 const uint32_t taddr = lane_cols + buf * 256u;
+                const uint64_t ss = ptx::pack_f32x2(__float_as_uint(s), __float_as_uint(s));
+                // the next 32 columns are on their way while these are multiplied and added
+                uint32_t v[2][32];
+                ptx::tmem_ld_32x32b_x32(taddr, v[0]);
 #pragma unroll
                 for (uint32_t c = 0; c < 4; ++c) {
-                    uint32_t v[32];
-                    ptx::tmem_ld_32x32b_x32(taddr + c * 32u, v);
                     ptx::tmem_ld_wait();
-                    if (c == 3) {
+                    if (c < 3) {
+                        ptx::tmem_ld_32x32b_x32(taddr + (c + 1) * 32u, v[(c + 1) & 1]);
+                    } else {
+                        // all columns are in registers: the buffer goes back
                         ptx::tcgen05_fence_before();
                         __syncwarp();
                         if (lane == 0)
-                            ptx::mbar_arrive_cluster_addr(leader_empty0 + 8u * buf);
+                            ptx::mbar_arrive_cluster_addr_relaxed(leader_empty0 + 8u * buf);
                     }
 #pragma unroll
-                    for (uint32_t i = 0; i < 32; ++i)
-                        acc[c * 32 + i] = fmaf(__uint_as_float(v[i]), s, acc[c * 32 + i]);
+                    for (uint32_t i = 0; i < 16; ++i)
+                        ptx::fma_f32x2(acc[c * 16 + i], ptx::pack_f32x2(v[c & 1][2 * i], v[c & 1][2 * i + 1]), ss);
                 }
                 if (++buf == 2) {
                     buf = 0;

@@ -226,6 +226,13 @@ __device__ __forceinline__ void mbar_arrive_cluster_addr(uint32_t bar_cluster_ad
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
 }
 
+// The same without release: for hand-overs whose earlier accesses are complete by themselves (tensor-memory loads after
+// tcgen05.wait::ld).  A release at cluster scope holds the thread until all its earlier accesses are performed.
+__device__ __forceinline__ void mbar_arrive_cluster_addr_relaxed(uint32_t bar_cluster_addr)
+{
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+}
+
 __device__ __forceinline__ void st_shared_cluster_u32(uint32_t cluster_addr, uint32_t value)
 {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(value) : "memory");
@@ -477,6 +484,37 @@ __device__ __forceinline__ uint32_t pack_bf16x2(uint32_t lo_f32_bits, uint32_t h
     uint32_t d;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(__uint_as_float(hi_f32_bits)), "f"(__uint_as_float(lo_f32_bits)));
     return d;
+}
+
+// Two fp32 in one 64-bit register pair, and the multiply-add of two pairs in one instruction.
+__device__ __forceinline__ uint64_t pack_f32x2(uint32_t lo, uint32_t hi)
+{
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+    return d;
+}
+
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, uint32_t &lo, uint32_t &hi)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
+}
+
+__device__ __forceinline__ void fma_f32x2(uint64_t &acc, uint64_t a, uint64_t b)
+{
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
+}
+
+// Registers of the executing warpgroup (all four warps): handed back to, or taken from, what the block was launched with.
+template <int N>
+__device__ __forceinline__ void setmaxnreg_dec()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+template <int N>
+__device__ __forceinline__ void setmaxnreg_inc()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // Programmatic dependent launch.  launch_dependents: this CTA no longer objects to the next kernel of the
