@@ -504,6 +504,14 @@ __device__ __forceinline__ void fma_f32x2(uint64_t &acc, uint64_t a, uint64_t b)
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
 }
 
+// Read-only load that stays where it is written (the compiler may sink an ordinary one to its use).
+__device__ __forceinline__ float ld_f32_nc(const float *p)
+{
+    float v;
+    asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    return v;
+}
+
 // Registers of the executing warpgroup (all four warps): handed back to, or taken from, what the block was launched with.
 template <int N>
 __device__ __forceinline__ void setmaxnreg_dec()
