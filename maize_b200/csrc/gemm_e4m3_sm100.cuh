@@ -37,13 +37,12 @@ struct F8Params {
 template <uint32_t STAGES>
 struct F8SmemLayout {
     static constexpr uint32_t kABytes = kBlockM * kF8BlockK;
-    static constexpr uint32_t kBHalfBytes = 64 * kF8BlockK;  // this CTA's rows of B for one half of the tile's columns
-    static constexpr uint32_t kBBytes = 2 * kBHalfBytes;
+    static constexpr uint32_t kBBytes = 128 * kF8BlockK;  // this CTA's half of the 256 columns
     static constexpr uint32_t kStageBytes = kABytes + kBBytes;
     static constexpr uint32_t kStagingOffset = STAGES * kStageBytes;
     static constexpr uint32_t kStagingBytes = kF8PromoteWarps * kTmaStoreBufBytes;
     static constexpr uint32_t kBarOffset = kStagingOffset + kStagingBytes;
-    static constexpr uint32_t kNumBars = 2 * STAGES + 8;
+    static constexpr uint32_t kNumBars = 2 * STAGES + 4;
     static constexpr uint32_t kTmemSlotOffset = kBarOffset + kNumBars * 8;
     static constexpr uint32_t kAbortOffset = kTmemSlotOffset + 4;
     static constexpr uint32_t kUsedBytes = kAbortOffset + 4;
@@ -109,7 +108,7 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
 {
     using L = F8SmemLayout<STAGES>;
     constexpr uint32_t kTmemCols = 512;
-    constexpr uint32_t kIdesc = ptx::make_instr_desc_e4m3(2 * kBlockM, 128);
+    constexpr uint32_t kIdesc = ptx::make_instr_desc_e4m3(2 * kBlockM, 256);
     const GemmParams &p = f.g;
 
     extern __shared__ uint8_t smem_raw[];
@@ -119,8 +118,8 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
     const uint32_t bar_base = smem_base + L::kBarOffset;
     auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };
     auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (STAGES + s); };
-    auto acc_full_bar = [&](uint32_t half, uint32_t b) { return bar_base + 8u * (2 * STAGES + 2 * half + b); };
-    auto acc_empty_bar = [&](uint32_t half, uint32_t b) { return bar_base + 8u * (2 * STAGES + 4 + 2 * half + b); };
+    auto acc_full_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + b); };
+    auto acc_empty_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + 2 + b); };
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + L::kTmemSlotOffset);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem_gen + L::kAbortOffset);
 
@@ -142,11 +141,10 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
             ptx::mbar_init(full_bar(s), 1);
             ptx::mbar_init(empty_bar(s), 1);
         }
-        for (uint32_t h = 0; h < 2; ++h)
-            for (uint32_t b = 0; b < 2; ++b) {
-                ptx::mbar_init(acc_full_bar(h, b), 1);
-                ptx::mbar_init(acc_empty_bar(h, b), kF8PromoteWarps);  // one lane per warp of the half's group, both CTAs
-            }
+        for (uint32_t b = 0; b < 2; ++b) {
+            ptx::mbar_init(acc_full_bar(b), 1);
+            ptx::mbar_init(acc_empty_bar(b), 2 * kF8PromoteWarps);  // one lane per promotion warp of both CTAs
+        }
         *abort_flag = 0;
         ptx::fence_barrier_init();
     }
@@ -176,7 +174,7 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
             for (uint32_t t = pair; ok && t < num_tiles; t += num_pairs) {
                 const TileCoord tc = tile_coord(t, p);
                 const int32_t m0 = static_cast<int32_t>(tc.m_blk * 2 * kBlockM + cta_rank * kBlockM);
-                const int32_t n0 = static_cast<int32_t>(tc.n_blk * 256u + cta_rank * 64u);
+                const int32_t n0 = static_cast<int32_t>(tc.n_blk * 256u + cta_rank * 128u);
                 for (uint32_t kb = 0; kb < num_kb; ++kb) {
                     ok = wait_bounded<true>(empty_bar(stage), phase ^ 1u, ctl, 1);
                     if (!ok)
@@ -187,9 +185,7 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
                         ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * L::kStageBytes);
                     const int32_t kx = static_cast<int32_t>(kb * kF8BlockK);
                     ptx::tma_load_2d_pair(sa, &tma_a, leader_full, kx, m0);
-                    // 64 rows of B for each half of the tile's columns
                     ptx::tma_load_2d_pair(sa + L::kABytes, &tma_b, leader_full, kx, n0);
-                    ptx::tma_load_2d_pair(sa + L::kABytes + L::kBHalfBytes, &tma_b, leader_full, kx, n0 + 128);
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1u;
@@ -207,24 +203,19 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
             bool ok = true;
             for (uint32_t t = pair; ok && t < num_tiles; t += num_pairs) {
                 for (uint32_t kb = 0; kb < num_kb; ++kb) {
-                    ok = wait_bounded<true>(full_bar(stage), phase, ctl, 2);
-                    const uint32_t sa = smem_base + stage * L::kStageBytes;
-                    const uint64_t da = ptx::make_smem_desc_sw128(sa);
-#pragma unroll
-                    for (uint32_t h = 0; h < 2; ++h) {
-                        ok = ok && wait_bounded<true>(acc_empty_bar(h, acc), acc_phase ^ 1u, ctl, 2);
-                        if (!ok)
-                            break;
-                        ptx::tcgen05_fence_after();
-                        const uint64_t db = ptx::make_smem_desc_sw128(sa + L::kABytes + h * L::kBHalfBytes);
-                        const uint32_t tmem_d = tmem_base + h * 256u + acc * 128u;
-#pragma unroll
-                        for (uint32_t k = 0; k < kF8BlockK / kF8UmmaK; ++k)
-                            ptx::mma_f8_2cta(tmem_d, da + 2u * k, db + 2u * k, kIdesc, k != 0u ? 1u : 0u);
-                        ptx::mma_commit_2cta_mask(acc_full_bar(h, acc), 3);
-                    }
+                    ok = wait_bounded<true>(full_bar(stage), phase, ctl, 2) &&
+                         wait_bounded<true>(acc_empty_bar(acc), acc_phase ^ 1u, ctl, 2);
                     if (!ok)
                         break;
+                    ptx::tcgen05_fence_after();
+                    const uint32_t sa = smem_base + stage * L::kStageBytes;
+                    const uint64_t da = ptx::make_smem_desc_sw128(sa);
+                    const uint64_t db = ptx::make_smem_desc_sw128(sa + L::kABytes);
+                    const uint32_t tmem_d = tmem_base + acc * 256u;
+#pragma unroll
+                    for (uint32_t k = 0; k < kF8BlockK / kF8UmmaK; ++k)
+                        ptx::mma_f8_2cta(tmem_d, da + 2u * k, db + 2u * k, kIdesc, k != 0u ? 1u : 0u);
+                    ptx::mma_commit_2cta_mask(acc_full_bar(acc), 3);
                     ptx::mma_commit_2cta_mask(empty_bar(stage), 3);
                     if (++stage == STAGES) {
                         stage = 0;
@@ -247,8 +238,8 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
         const uint32_t half = (warp - kF8ControlWarps) >> 2;
         uint8_t *stage_gen = smem_gen + L::kStagingOffset + (warp - kF8ControlWarps) * kTmaStoreBufBytes;
         const uint32_t stage_u32 = smem_base + L::kStagingOffset + (warp - kF8ControlWarps) * kTmaStoreBufBytes;
-        const uint32_t lane_cols = tmem_base + ((quarter * 32u) << 16) + half * 256u;
-        const uint32_t leader_empty0 = ptx::mapa_shared(acc_empty_bar(half, 0), 0);
+        const uint32_t lane_cols = tmem_base + ((quarter * 32u) << 16) + half * 128u;
+        const uint32_t leader_empty0 = ptx::mapa_shared(acc_empty_bar(0), 0);
         uint32_t buf = 0, buf_phase = 0;
         bool ok = true;
         for (uint32_t t = pair; ok && t < num_tiles; t += num_pairs) {
@@ -271,12 +262,12 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
                 a0 = a1, b0 = b1;
                 a1 = ptx::ld_f32_nc(sa + min(kb + 2, last));
                 b1 = ptx::ld_f32_nc(sb + min(kb + 2, last));
-                ok = wait_bounded<true>(acc_full_bar(half, buf), buf_phase, ctl, 3);
+                ok = wait_bounded(acc_full_bar(buf), buf_phase, ctl, 3);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok)
                     break;
                 ptx::tcgen05_fence_after();
-                const uint32_t taddr = lane_cols + buf * 128u;
+                const uint32_t taddr = lane_cols + buf * 256u;
                 const uint64_t ss = ptx::pack_f32x2(__float_as_uint(s), __float_as_uint(s));
                 // the next 32 columns are on their way while these are multiplied and added
                 uint32_t v[2][32];

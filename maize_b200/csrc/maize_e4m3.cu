@@ -113,7 +113,7 @@ maize_status_t maize_gemm_e4m3(maize_ctx_t *ctx, const void *a, uint64_t lda, co
     CUtensorMap ta, tb, tc;
     maize_status_t st;
     if ((st = byte_map(ctx, &ta, a, m, k, lda, maize::kBlockM)) != MAIZE_OK ||
-        (st = byte_map(ctx, &tb, b, n, k, ldb, 64)) != MAIZE_OK)
+        (st = byte_map(ctx, &tb, b, n, k, ldb, 128)) != MAIZE_OK)
         return st;
     memset(&tc, 0, sizeof tc);
     maize::F8Params f = {};
