@@ -101,6 +101,14 @@ __device__ __forceinline__ void f8_store(const GemmParams &p, const CUtensorMap 
     }
 }
 
+// acc[first .. first + 15] += v * ss: 32 columns of one row, in pairs.
+__device__ __forceinline__ void f8_promote(uint64_t (&acc)[64], int first, const uint32_t (&v)[32], uint64_t ss)
+{
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        ptx::fma_f32x2(acc[first + i], ptx::pack_f32x2(v[2 * i], v[2 * i + 1]), ss);
+}
+
 template <uint32_t STAGES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kF8Threads, 1)
 gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
@@ -269,25 +277,24 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
                 ptx::tcgen05_fence_after();
                 const uint32_t taddr = lane_cols + buf * 256u;
                 const uint64_t ss = ptx::pack_f32x2(__float_as_uint(s), __float_as_uint(s));
-                // the next 32 columns are on their way while these are multiplied and added
-                uint32_t v[2][32];
-                ptx::tmem_ld_32x32b_x32(taddr, v[0]);
-#pragma unroll
-                for (uint32_t c = 0; c < 4; ++c) {
-                    ptx::tmem_ld_wait();
-                    if (c < 3) {
-                        ptx::tmem_ld_32x32b_x32(taddr + (c + 1) * 32u, v[(c + 1) & 1]);
-                    } else {
-                        // all columns are in registers: the buffer goes back
-                        ptx::tcgen05_fence_before();
-                        __syncwarp();
-                        if (lane == 0)
-                            ptx::mbar_arrive_cluster_addr_relaxed(leader_empty0 + 8u * buf);
-                    }
-#pragma unroll
-                    for (uint32_t i = 0; i < 16; ++i)
-                        ptx::fma_f32x2(acc[c * 16 + i], ptx::pack_f32x2(v[c & 1][2 * i], v[c & 1][2 * i + 1]), ss);
-                }
+                // Two loads of 32 columns in flight at a time: a load's latency, not its transfer, is what a warp waits for,
+                // and tcgen05.wait::ld waits for all of them.
+                uint32_t v0[32], v1[32];
+                ptx::tmem_ld_32x32b_x32(taddr, v0);
+                ptx::tmem_ld_32x32b_x32(taddr + 32u, v1);
+                ptx::tmem_ld_wait();
+                f8_promote(acc, 0, v0, ss);
+                ptx::tmem_ld_32x32b_x32(taddr + 64u, v0);
+                f8_promote(acc, 16, v1, ss);
+                ptx::tmem_ld_32x32b_x32(taddr + 96u, v1);
+                ptx::tmem_ld_wait();
+                // all columns are in registers: the buffer goes back
+                ptx::tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    ptx::mbar_arrive_cluster_addr_relaxed(leader_empty0 + 8u * buf);
+                f8_promote(acc, 32, v0, ss);
+                f8_promote(acc, 48, v1, ss);
                 if (++buf == 2) {
                     buf = 0;
                     buf_phase ^= 1u;
