@@ -228,7 +228,6 @@ gemm_bf16_sm100_grouped(const __grid_constant__ RowMaps tma_a, const __grid_cons
 
     if (threadIdx.x == 0) {
         ptx::prefetch_tensormap(&tma_w);
-        ptx::prefetch_tensormap(&tma_a.box[3]);
         for (uint32_t s = 0; s < STAGES; ++s) {
             ptx::mbar_init(full_bar(s), 1);   // the leader's producer; bytes of both CTAs
             ptx::mbar_init(empty_bar(s), 1);  // one tcgen05.commit of the leader

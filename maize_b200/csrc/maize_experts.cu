@@ -95,8 +95,9 @@ maize_status_t grouped_impl(maize_ctx_t *ctx, const void *a, uint64_t lda, const
     if (lda * 2 >= (1ull << 40) || ldb * 2 >= (1ull << 40) || b_stride * 2 >= (1ull << 40))
         return fail(ctx, MAIZE_ERR_UNSUPPORTED, "pitch beyond the TMA limit of 2^40 bytes");
 
-    maize::RowMaps ta;
-    for (uint32_t i = 0; i < 4; ++i)
+    // a CTA brings in half a tile's rows: no box is used that is longer than half of all rows, rounded up
+    maize::RowMaps ta = {};
+    for (uint32_t i = 0; i < 4 && (i == 0 || (8u << i) < (rows + 31) / 32 * 16); ++i)
         if ((st = matrix_map(ctx, &ta.box[i], a, rows, k, lda, 16u << i)) != MAIZE_OK)
             return st;
     CUtensorMap tw;

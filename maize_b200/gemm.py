@@ -54,6 +54,21 @@ def _stream_handle(stream) -> Optional[int]:
     return stream.cuda_stream
 
 
+_torch = None
+_raw_stream = None
+
+
+def _types():
+    """The torch module (imported with the first call that has tensors to look at), and the shortest way to the current
+    stream's handle where this torch has it."""
+    global _torch, _raw_stream
+    if _torch is None:
+        import torch
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _torch = torch
+    return _torch
+
+
 class Context:
     """One per host thread / stream; owns the device status word and tunables."""
 
@@ -240,151 +255,161 @@ class Context:
         return out
 
     # ------------------------------------------- products grouped by expert --
-    def _own(self, name: str, t, dims: int, dtype) -> None:
-        """The checks every operand of the calls below shares: kind, device, unit stride along the rows."""
-        if (t.dim() != dims or t.dtype != dtype or not t.is_cuda or t.device.index != self.device
-                or (t.shape[-1] > 1 and t.stride(-1) != 1)):
-            raise MaizeError(_ffi.INVALID_ARG, f"{name}: expected a {dims}-D {dtype} tensor with unit column stride on "
-                                               f"cuda:{self.device}")
+    # Small calls are bound by the host, so these checks take each property of a tensor once.
+    def _own(self, name: str, t, dims: int, dtype):
+        """The checks every operand of the calls below shares: kind, device, unit stride along the rows.  Returns the
+        strides."""
+        if t.dtype is dtype and t.dim() == dims and t.get_device() == self.device:
+            strides = t.stride()
+            if strides[-1] == 1 or t.shape[-1] <= 1:
+                return strides
+        raise MaizeError(_ffi.INVALID_ARG, f"{name}: expected a {dims}-D {dtype} tensor with unit column stride on "
+                                           f"cuda:{self.device}")
 
     def _stream(self, stream) -> int:
         """Handle of the stream a call runs on: the given one, or the current stream of the context's device."""
         if stream is None:
             import torch
-            return torch.cuda.current_stream(self.device).cuda_stream
+            return torch.cuda.current_stream(self.device).cuda_stream if _raw_stream is None else _raw_stream(self.device)
         return stream if isinstance(stream, int) else stream.cuda_stream
 
-    def _new(self, shape, dtype, stream):
-        """An output tensor, allocated for the stream the call runs on."""
-        import torch
+    def _new(self, like, shape, dtype, stream):
+        """An output tensor on the device of `like`, allocated for the stream the call runs on."""
         if stream is None:
-            return torch.empty(shape, dtype=dtype, device=torch.device("cuda", self.device))
+            return like.new_empty(shape, dtype=dtype)
+        import torch
         if isinstance(stream, int):
             stream = torch.cuda.ExternalStream(stream, device=self.device)
         with torch.cuda.stream(stream):
-            return torch.empty(shape, dtype=dtype, device=torch.device("cuda", self.device))
+            return like.new_empty(shape, dtype=dtype)
 
-    def _offsets(self, offsets, groups: int) -> None:
-        import torch
-        if (offsets.dim() != 1 or offsets.dtype != torch.int32 or not offsets.is_cuda
-                or offsets.device.index != self.device or offsets.shape[0] != groups + 1 or not offsets.is_contiguous()):
-            raise MaizeError(_ffi.INVALID_ARG, f"offsets: expected {groups + 1} contiguous int32 values on cuda:{self.device}")
+    def _offsets(self, offsets, groups: int) -> int:
+        if (offsets.dtype is _types().int32 and offsets.dim() == 1 and offsets.shape[0] == groups + 1
+                and offsets.get_device() == self.device and offsets.is_contiguous()):
+            return offsets.data_ptr()
+        raise MaizeError(_ffi.INVALID_ARG, f"offsets: expected {groups + 1} contiguous int32 values on cuda:{self.device}")
 
-    def _grouped(self, entry, a, b, offsets, out, stream, n: int, kb: int):
-        import torch
-        bf16 = torch.bfloat16
-        self._own("a", a, 2, bf16)
-        self._own("b", b, 3, bf16)
+    def _grouped(self, entry, a, b, offsets, out, stream, kn: bool):
+        bf16 = _types().bfloat16
+        sa, sb = self._own("a", a, 2, bf16), self._own("b", b, 3, bf16)
         rows, k = a.shape
-        groups = b.shape[0]
+        groups, b_rows, b_cols = b.shape
+        n, kb = (b_cols, b_rows) if kn else (b_rows, b_cols)
         if k != kb:
             raise MaizeError(_ffi.INVALID_ARG, f"a has {k} columns, the matrices of b a K of {kb}")
-        self._offsets(offsets, groups)
+        at = self._offsets(offsets, groups)
         if out is None:
-            out = self._new((rows, n), bf16, stream)
+            out = self._new(a, (rows, n), bf16, stream)
+            ldc = n
         else:
-            self._own("out", out, 2, bf16)
+            ldc = self._own("out", out, 2, bf16)[0]
             if out.shape != (rows, n):
                 raise MaizeError(_ffi.INVALID_ARG, f"out: expected {rows} x {n}")
-        self._check(entry(self._h, a.data_ptr(), a.stride(0) if rows > 1 else max(k, -(-k // 8) * 8), b.data_ptr(),
-                          b.stride(1) if b.shape[1] > 1 else -(-b.shape[2] // 8) * 8, b.stride(0), out.data_ptr(),
-                          out.stride(0) if rows > 1 else max(n, 1), offsets.data_ptr(), groups, rows, n, k,
-                          self._stream(stream)))
+        # the stride of a dimension of one is not used and may be anything
+        st = entry(self._h, a.data_ptr(), sa[0] if rows > 1 else -(-k // 8) * 8, b.data_ptr(),
+                   sb[1] if b_rows > 1 else -(-b_cols // 8) * 8, sb[0], out.data_ptr(), ldc if rows > 1 else n, at,
+                   groups, rows, n, k, self._stream(stream))
+        if st != _ffi.OK:
+            self._check(st)
         return out
 
     def grouped_gemm(self, a, b, offsets, out=None, stream=None):
         """``out[r] = a[r] @ b[g].T`` for the rows ``offsets[g] <= r < offsets[g + 1]`` of every group g: a is rows x K,
         b is groups x N x K (one weight matrix per expert), offsets int32 on the device, ascending, groups + 1 of them.
         Rows outside all groups are left as they were.  Groups may be empty; their sizes are never read on the host."""
-        return self._grouped(self._lib.maize_grouped_gemm_bf16, a, b, offsets, out, stream, b.shape[-2], b.shape[-1])
+        return self._grouped(self._lib.maize_grouped_gemm_bf16, a, b, offsets, out, stream, False)
 
     def grouped_gemm_kn(self, a, b, offsets, out=None, stream=None):
         """``out[r] = a[r] @ b[g]`` with b given groups x K x N.  With ``a`` the gradient of ``grouped_gemm``'s result and
         the same b this is the gradient of its input."""
-        return self._grouped(self._lib.maize_grouped_gemm_bf16_kn, a, b, offsets, out, stream, b.shape[-1], b.shape[-2])
+        return self._grouped(self._lib.maize_grouped_gemm_bf16_kn, a, b, offsets, out, stream, True)
 
     def grouped_gemm_wgrad(self, a, dc, offsets, out=None, stream=None):
         """``out[g] = dc[rows of g].T @ a[rows of g]``: the gradient of ``grouped_gemm``'s b (groups x N x K) from its
         input ``a`` (rows x K) and the gradient ``dc`` (rows x N) of its result.  A group without rows gets zeros."""
-        import torch
-        bf16 = torch.bfloat16
-        self._own("a", a, 2, bf16)
-        self._own("dc", dc, 2, bf16)
+        bf16 = _types().bfloat16
+        sa, sd = self._own("a", a, 2, bf16), self._own("dc", dc, 2, bf16)
         rows, k = a.shape
-        n = dc.shape[1]
-        if dc.shape[0] != rows:
-            raise MaizeError(_ffi.INVALID_ARG, f"a has {rows} rows, dc {dc.shape[0]}")
-        if offsets.dim() != 1 or offsets.shape[0] < 1:
+        rows_dc, n = dc.shape
+        if rows_dc != rows:
+            raise MaizeError(_ffi.INVALID_ARG, f"a has {rows} rows, dc {rows_dc}")
+        groups = offsets.shape[0] - 1 if offsets.dim() == 1 else -1
+        if groups < 0:
             raise MaizeError(_ffi.INVALID_ARG, "offsets: expected groups + 1 int32 values")
-        groups = offsets.shape[0] - 1
-        self._offsets(offsets, groups)
+        at = self._offsets(offsets, groups)
         if out is None:
-            out = self._new((groups, n, k), bf16, stream)
+            out = self._new(a, (groups, n, k), bf16, stream)
+            so = (n * k, k)
         else:
-            self._own("out", out, 3, bf16)
+            so = self._own("out", out, 3, bf16)
             if out.shape != (groups, n, k):
                 raise MaizeError(_ffi.INVALID_ARG, f"out: expected {groups} x {n} x {k}")
-        self._check(self._lib.maize_grouped_gemm_bf16_wgrad(
-            self._h, a.data_ptr(), a.stride(0) if rows > 1 else -(-k // 8) * 8, dc.data_ptr(),
-            dc.stride(0) if rows > 1 else -(-n // 8) * 8, out.data_ptr(), out.stride(1) if n > 1 else max(k, 1),
-            out.stride(0), offsets.data_ptr(), groups, rows, n, k, self._stream(stream)))
+        st = self._lib.maize_grouped_gemm_bf16_wgrad(
+            self._h, a.data_ptr(), sa[0] if rows > 1 else -(-k // 8) * 8, dc.data_ptr(),
+            sd[0] if rows > 1 else -(-n // 8) * 8, out.data_ptr(), so[1] if n > 1 else k, so[0], at, groups, rows, n, k,
+            self._stream(stream))
+        if st != _ffi.OK:
+            self._check(st)
         return out
 
     # ------------------------------------------------------ 8-bit products --
     def quantize_e4m3(self, x, block_rows: int = 1, out=None, scales=None, stream=None):
         """bf16 rows x cols -> (e4m3 tensor of the same shape, fp32 scales), with a power-of-two scale for each 1 x 128
         (``block_rows`` = 1: activations) or 128 x 128 block (``block_rows`` = 128: weights): ``x ~ q * scale``."""
-        import torch
-        self._own("x", x, 2, torch.bfloat16)
+        torch = _types()
+        sx = self._own("x", x, 2, torch.bfloat16)
         rows, cols = x.shape
-        if block_rows not in (1, 128):
+        if block_rows != 1 and block_rows != 128:
             raise MaizeError(_ffi.INVALID_ARG, "block_rows must be 1 or 128")
-        shape = (-(-rows // block_rows), -(-cols // 128))
+        down, across = -(-rows // block_rows), -(-cols // 128)
         if out is None:
-            out = self._new((rows, cols), torch.float8_e4m3fn, stream)
+            out = self._new(x, (rows, cols), torch.float8_e4m3fn, stream)
+            ldq = cols
         else:
-            self._own("out", out, 2, torch.float8_e4m3fn)
-            if out.shape != x.shape:
+            ldq = self._own("out", out, 2, torch.float8_e4m3fn)[0]
+            if out.shape != (rows, cols):
                 raise MaizeError(_ffi.INVALID_ARG, f"out: expected {rows} x {cols}")
         if scales is None:
-            scales = self._new(shape, torch.float32, stream)
+            scales = self._new(x, (down, across), torch.float32, stream)
+            lds = across
         else:
-            self._own("scales", scales, 2, torch.float32)
-            if scales.shape != shape:
-                raise MaizeError(_ffi.INVALID_ARG, f"scales: expected {shape[0]} x {shape[1]}")
-        self._check(self._lib.maize_quantize_e4m3(
-            self._h, x.data_ptr(), x.stride(0) if rows > 1 else max(cols, 1), rows, cols, block_rows, out.data_ptr(),
-            out.stride(0) if rows > 1 else max(cols, 1), scales.data_ptr(),
-            scales.stride(0) if shape[0] > 1 else max(shape[1], 1), self._stream(stream)))
+            lds = self._own("scales", scales, 2, torch.float32)[0]
+            if scales.shape != (down, across):
+                raise MaizeError(_ffi.INVALID_ARG, f"scales: expected {down} x {across}")
+        st = self._lib.maize_quantize_e4m3(self._h, x.data_ptr(), sx[0] if rows > 1 else cols, rows, cols, block_rows,
+                                           out.data_ptr(), ldq if rows > 1 else cols, scales.data_ptr(),
+                                           lds if down > 1 else across, self._stream(stream))
+        if st != _ffi.OK:
+            self._check(st)
         return out, scales
 
     def gemm_e4m3(self, a, a_scales, b, b_scales, out=None, stream=None):
         """``out = (a * a_scales) @ (b * b_scales).T`` in bf16 for e4m3 a (M x K) with a scale for each 1 x 128 block
         (M x ceil(K/128), fp32) and e4m3 b (N x K) with one for each 128 x 128 block (ceil(N/128) x ceil(K/128))."""
-        import torch
-        f8 = torch.float8_e4m3fn
-        self._own("a", a, 2, f8)
-        self._own("b", b, 2, f8)
-        self._own("a_scales", a_scales, 2, torch.float32)
-        self._own("b_scales", b_scales, 2, torch.float32)
+        torch = _types()
+        f8, f32 = torch.float8_e4m3fn, torch.float32
+        sa, sb = self._own("a", a, 2, f8), self._own("b", b, 2, f8)
+        ssa, ssb = self._own("a_scales", a_scales, 2, f32), self._own("b_scales", b_scales, 2, f32)
         m, k = a.shape
         n, kb = b.shape
         if k != kb:
             raise MaizeError(_ffi.INVALID_ARG, "a.shape[1] != b.shape[1] (b is stored N x K)")
-        blocks = -(-k // 128)
-        if a_scales.shape != (m, blocks) or b_scales.shape != (-(-n // 128), blocks):
-            raise MaizeError(_ffi.INVALID_ARG, f"scales: expected {m} x {blocks} for a, {-(-n // 128)} x {blocks} for b")
+        blocks, down = -(-k // 128), -(-n // 128)
+        if a_scales.shape != (m, blocks) or b_scales.shape != (down, blocks):
+            raise MaizeError(_ffi.INVALID_ARG, f"scales: expected {m} x {blocks} for a, {down} x {blocks} for b")
         if out is None:
-            out = self._new((m, n), torch.bfloat16, stream)
+            out = self._new(a, (m, n), torch.bfloat16, stream)
+            ldc = n
         else:
-            self._own("out", out, 2, torch.bfloat16)
+            ldc = self._own("out", out, 2, torch.bfloat16)[0]
             if out.shape != (m, n):
                 raise MaizeError(_ffi.INVALID_ARG, f"out: expected {m} x {n}")
-        self._check(self._lib.maize_gemm_e4m3(
-            self._h, a.data_ptr(), a.stride(0) if m > 1 else k, a_scales.data_ptr(),
-            a_scales.stride(0) if m > 1 else blocks, b.data_ptr(), b.stride(0) if n > 1 else k, b_scales.data_ptr(),
-            b_scales.stride(0) if n > 128 else blocks, out.data_ptr(), out.stride(0) if m > 1 else max(n, 1), m, n, k,
-            self._stream(stream)))
+        st = self._lib.maize_gemm_e4m3(self._h, a.data_ptr(), sa[0] if m > 1 else k, a_scales.data_ptr(),
+                                       ssa[0] if m > 1 else blocks, b.data_ptr(), sb[0] if n > 1 else k,
+                                       b_scales.data_ptr(), ssb[0] if down > 1 else blocks, out.data_ptr(),
+                                       ldc if m > 1 else n, m, n, k, self._stream(stream))
+        if st != _ffi.OK:
+            self._check(st)
         return out
 
     def debug_wait_expires(self, budget_ns: int, stream=None) -> None:
@@ -410,9 +435,10 @@ def gemm(a, b, out=None, stream=None):
 
 
 def _context_of(t) -> Context:
-    if not t.is_cuda:
+    device = t.get_device()
+    if device < 0:
         raise MaizeError(_ffi.INVALID_ARG, "expected CUDA tensors")
-    return default_context(t.device.index)
+    return _default_ctx.get(device) or default_context(device)
 
 
 def grouped_gemm(a, b, offsets, out=None, stream=None):
