@@ -62,10 +62,11 @@ maize_status_t maize_quantize_e4m3(maize_ctx_t *ctx, const void *x, uint64_t ldx
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     if (block_rows == 1) {
         const uint64_t blocks = uint64_t(rows) * across;
-        const uint64_t want = (blocks + 15) / 16, cap = uint64_t(ctx->sm_count) * 8;
+        // one block per half warp until the SMs are full, then several in flight
+        const uint64_t want = (blocks + 15) / 16, cap = uint64_t(ctx->sm_count) * 6;
         const uint32_t grid = static_cast<uint32_t>(want < cap ? want : cap);
-        return vec ? maize::launch(ctx, -1, maize::quantize_rows_kernel<true>, grid, 256, 0, stream, p)
-                   : maize::launch(ctx, -1, maize::quantize_rows_kernel<false>, grid, 256, 0, stream, p);
+        return vec ? maize::launch(ctx, -1, maize::quantize_rows_kernel<true, 4>, grid, 256, 0, stream, p)
+                   : maize::launch(ctx, -1, maize::quantize_rows_kernel<false, 2>, grid, 256, 0, stream, p);
     }
     const uint64_t blocks = (uint64_t(rows) + 127) / 128 * across;
     if (blocks > 0x7fffffffull)
