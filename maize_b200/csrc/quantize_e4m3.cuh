@@ -61,39 +61,53 @@ __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w 
 
 constexpr uint32_t kBf16Inf = 0x7f80u;
 
-// Largest finite magnitude of the eight, as bf16 bits (they order like integers).  `odd` is set where one is infinite or
-// NaN; only then are the elements looked at one by one.
-__device__ __forceinline__ uint32_t eight_top(const Eight &v, bool &odd)
+// The eight one by one, where one of them is infinite or NaN: the largest finite magnitude, and the conversion with NaN in
+// their places (the conversion instruction would saturate infinities).  Out of line: nearly no data comes here.
+static __device__ __noinline__ uint32_t odd_eight_top(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3)
 {
-    constexpr uint32_t kAbs = 0x7fff7fffu;
-    const uint32_t m2 = max_s16x2(max_s16x2(v.w[0] & kAbs, v.w[1] & kAbs), max_s16x2(v.w[2] & kAbs, v.w[3] & kAbs));
-    uint32_t m = max(m2 & 0xffffu, m2 >> 16);
-    if (m >= kBf16Inf) {
-        odd = true;
-        m = 0;
+    const uint32_t w[4] = {w0, w1, w2, w3};
+    uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t lo = v.w[i] & 0x7fffu, hi = (v.w[i] >> 16) & 0x7fffu;
-            m = max(m, max(lo < kBf16Inf ? lo : 0u, hi < kBf16Inf ? hi : 0u));
-        }
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = w[i] & 0x7fffu, hi = (w[i] >> 16) & 0x7fffu;
+        m = max(m, max(lo < kBf16Inf ? lo : 0u, hi < kBf16Inf ? hi : 0u));
     }
     return m;
 }
 
-__device__ __forceinline__ uint2 eight_convert(const Eight &v, float inverse, bool odd)
+static __device__ __noinline__ uint2 odd_eight_convert(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, float inverse)
 {
+    const uint32_t w[4] = {w0, w1, w2, w3};
     uint32_t h[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        float lo = bf16_lo(v.w[i]) * inverse, hi = bf16_hi(v.w[i]) * inverse;
-        if (odd) {  // the conversion saturates infinities: they become NaN here
-            if ((v.w[i] & 0x7fffu) >= kBf16Inf)
-                lo = __uint_as_float(0x7fffffffu);
-            if (((v.w[i] >> 16) & 0x7fffu) >= kBf16Inf)
-                hi = __uint_as_float(0x7fffffffu);
-        }
-        h[i] = to_e4m3x2(lo, hi);
+        const float nan = __uint_as_float(0x7fffffffu);
+        h[i] = to_e4m3x2((w[i] & 0x7fffu) >= kBf16Inf ? nan : bf16_lo(w[i]) * inverse,
+                         ((w[i] >> 16) & 0x7fffu) >= kBf16Inf ? nan : bf16_hi(w[i]) * inverse);
     }
+    return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+}
+
+// Largest finite magnitude of the eight, as bf16 bits (they order like integers); `odd` is set where one is not finite.
+__device__ __forceinline__ uint32_t eight_top(const Eight &v, bool &odd)
+{
+    constexpr uint32_t kAbs = 0x7fff7fffu;
+    const uint32_t m2 = max_s16x2(max_s16x2(v.w[0] & kAbs, v.w[1] & kAbs), max_s16x2(v.w[2] & kAbs, v.w[3] & kAbs));
+    const uint32_t m = max(m2 & 0xffffu, m2 >> 16);
+    if (m < kBf16Inf)
+        return m;
+    odd = true;
+    return odd_eight_top(v.w[0], v.w[1], v.w[2], v.w[3]);
+}
+
+__device__ __forceinline__ uint2 eight_convert(const Eight &v, float inverse, bool odd)
+{
+    if (odd)
+        return odd_eight_convert(v.w[0], v.w[1], v.w[2], v.w[3], inverse);
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        h[i] = to_e4m3x2(bf16_lo(v.w[i]) * inverse, bf16_hi(v.w[i]) * inverse);
     return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 
@@ -232,25 +246,32 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
         ptx::grid_dependency_wait();
     }
     const uint32_t across = (p.cols + kQuantBlock - 1) / kQuantBlock;
-    const uint64_t blocks = static_cast<uint64_t>(p.rows) * across;
     const uint32_t lane16 = threadIdx.x & 15u;
-    const uint64_t step = static_cast<uint64_t>(gridDim.x) * (blockDim.x / 16);
-    const uint64_t first = (static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / 16;
-    // whole warps go round: the shuffles need both halves of one
-    for (uint64_t round = 0; round * step < blocks; round += UNROLL) {
+    // Half warp i takes the blocks i, i + step, ... in row order; the row and the block within it are carried along.
+    const uint32_t step = gridDim.x * (blockDim.x / 16);
+    const uint32_t first = (blockIdx.x * blockDim.x + threadIdx.x) / 16;
+    const uint32_t step_rows = step / across, step_blks = step - step_rows * across;
+    uint32_t row = first / across, blk = first - row * across;
+    // whole warps go round (the shuffles need both halves of one): the warp's first half has the lower block
+    for (uint32_t lead = __shfl_sync(0xffffffffu, row, 0); lead < p.rows; lead = __shfl_sync(0xffffffffu, row, 0)) {
         Eight v[UNROLL];
-        uint32_t row[UNROLL], blk[UNROLL];
-        bool mine[UNROLL];
+        uint32_t at_row[UNROLL], at_blk[UNROLL];
 #pragma unroll
         for (uint32_t u = 0; u < UNROLL; ++u) {
-            const uint64_t b = first + (round + u) * step;
-            mine[u] = b < blocks;
-            row[u] = mine[u] ? (blocks >> 32 ? static_cast<uint32_t>(b / across) : static_cast<uint32_t>(b) / across) : 0u;
-            blk[u] = mine[u] ? static_cast<uint32_t>(b - static_cast<uint64_t>(row[u]) * across) : 0u;
-            v[u] = load_block_row<VEC>(p.x + static_cast<uint64_t>(row[u]) * p.ldx, blk[u] * kQuantBlock, p.cols, lane16, mine[u]);
+            at_row[u] = row;
+            at_blk[u] = blk;
+            const bool mine = row < p.rows;
+            v[u] = load_block_row<VEC>(p.x + static_cast<uint64_t>(mine ? row : 0u) * p.ldx, blk * kQuantBlock, p.cols, lane16, mine);
+            row += step_rows;
+            blk += step_blks;
+            if (blk >= across) {
+                blk -= across;
+                ++row;
+            }
         }
 #pragma unroll
         for (uint32_t u = 0; u < UNROLL; ++u) {
+            const bool mine = at_row[u] < p.rows;
             bool odd = false;
             uint32_t top = eight_top(v[u], odd);
 #pragma unroll
@@ -258,10 +279,10 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
             float scale, inverse;
             block_scale(top, scale, inverse);
-            store_block_row<VEC>(p.q + static_cast<uint64_t>(row[u]) * p.ldq, blk[u] * kQuantBlock, p.cols, lane16, mine[u],
-                                 eight_convert(v[u], inverse, odd));
-            if (mine[u] && lane16 == 0)
-                p.scales[static_cast<uint64_t>(row[u]) * p.ld_scales + blk[u]] = scale;
+            store_block_row<VEC>(p.q + static_cast<uint64_t>(mine ? at_row[u] : 0u) * p.ldq, at_blk[u] * kQuantBlock, p.cols, lane16,
+                                 mine, eight_convert(v[u], inverse, odd));
+            if (mine && lane16 == 0)
+                p.scales[static_cast<uint64_t>(at_row[u]) * p.ld_scales + at_blk[u]] = scale;
         }
     }
 }
