@@ -57,22 +57,24 @@ maize_status_t maize_quantize_e4m3(maize_ctx_t *ctx, const void *x, uint64_t ldx
     p.rows = rows;
     p.cols = cols;
     p.pdl = ctx->pdl;
-    const bool vec = ldx % 8 == 0 && aligned(x, 16) && ldq % 8 == 0 && aligned(q, 8);
+    // rows of X that loads of 16 bytes take as they are; rows of Q for stores of 16 bytes
+    const bool xvec = ldx % 8 == 0 && aligned(x, 16), qvec = ldq % 16 == 0 && aligned(q, 16);
     DeviceGuard guard(ctx->device);
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     if (block_rows == 1) {
-        const uint64_t blocks = uint64_t(rows) * across;
-        // one block per half warp until the SMs are full, then several in flight
-        const uint64_t want = (blocks + 15) / 16, cap = uint64_t(ctx->sm_count) * 6;
+        // one block per group of eight lanes until the SMs are full, then several in flight
+        const uint64_t want = (uint64_t(rows) * across + 31) / 32, cap = uint64_t(ctx->sm_count) * 6;
         const uint32_t grid = static_cast<uint32_t>(want < cap ? want : cap);
-        return vec ? maize::launch(ctx, -1, maize::quantize_rows_kernel<true, 4>, grid, 256, 0, stream, p)
-                   : maize::launch(ctx, -1, maize::quantize_rows_kernel<false, 2>, grid, 256, 0, stream, p);
+        auto kernel = xvec ? (qvec ? maize::quantize_rows_kernel<true, true, 2> : maize::quantize_rows_kernel<true, false, 2>)
+                           : maize::quantize_rows_kernel<false, false, 2>;
+        return maize::launch(ctx, -1, kernel, grid, 256, 0, stream, p);
     }
     const uint64_t blocks = (uint64_t(rows) + 127) / 128 * across;
     if (blocks > 0x7fffffffull)
         return fail(ctx, MAIZE_ERR_UNSUPPORTED, "too many blocks");
-    return vec ? maize::launch(ctx, -1, maize::quantize_blocks_kernel<true>, static_cast<uint32_t>(blocks), 256, 0, stream, p)
-               : maize::launch(ctx, -1, maize::quantize_blocks_kernel<false>, static_cast<uint32_t>(blocks), 256, 0, stream, p);
+    auto kernel = xvec ? (qvec ? maize::quantize_blocks_kernel<true, true> : maize::quantize_blocks_kernel<true, false>)
+                       : maize::quantize_blocks_kernel<false, false>;
+    return maize::launch(ctx, -1, kernel, static_cast<uint32_t>(blocks), 256, 0, stream, p);
 }
 
 maize_status_t maize_gemm_e4m3(maize_ctx_t *ctx, const void *a, uint64_t lda, const void *a_scales, uint64_t ld_a_scales,

@@ -51,194 +51,190 @@ __device__ __forceinline__ uint32_t max_s16x2(uint32_t a, uint32_t b)
     return r;
 }
 
-// Eight bf16 in four words.
-struct Eight {
-    uint32_t w[4];
+// Sixteen bf16 in eight words: what a lane holds.  Eight lanes hold a row of a block.
+struct Sixteen {
+    uint32_t w[8];
 };
+constexpr uint32_t kLaneElements = 16;
 
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
 constexpr uint32_t kBf16Inf = 0x7f80u;
 
-// The eight one by one, where one of them is infinite or NaN: the largest finite magnitude, and the conversion with NaN in
+// The sixteen one by one, where one of them is infinite or NaN: the largest finite magnitude, and the conversion with NaN in
 // their places (the conversion instruction would saturate infinities).  Out of line: nearly no data comes here.
-static __device__ __noinline__ uint32_t odd_eight_top(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3)
+static __device__ __noinline__ uint32_t odd_top(const Sixteen v)
 {
-    const uint32_t w[4] = {w0, w1, w2, w3};
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t lo = w[i] & 0x7fffu, hi = (w[i] >> 16) & 0x7fffu;
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t lo = v.w[i] & 0x7fffu, hi = (v.w[i] >> 16) & 0x7fffu;
         m = max(m, max(lo < kBf16Inf ? lo : 0u, hi < kBf16Inf ? hi : 0u));
     }
     return m;
 }
 
-static __device__ __noinline__ uint2 odd_eight_convert(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, float inverse)
+static __device__ __noinline__ uint4 odd_convert(const Sixteen v, float inverse)
 {
-    const uint32_t w[4] = {w0, w1, w2, w3};
-    uint32_t h[4];
+    uint32_t h[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
         const float nan = __uint_as_float(0x7fffffffu);
-        h[i] = to_e4m3x2((w[i] & 0x7fffu) >= kBf16Inf ? nan : bf16_lo(w[i]) * inverse,
-                         ((w[i] >> 16) & 0x7fffu) >= kBf16Inf ? nan : bf16_hi(w[i]) * inverse);
+        h[i] = to_e4m3x2((v.w[i] & 0x7fffu) >= kBf16Inf ? nan : bf16_lo(v.w[i]) * inverse,
+                         ((v.w[i] >> 16) & 0x7fffu) >= kBf16Inf ? nan : bf16_hi(v.w[i]) * inverse);
     }
-    return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+    return make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
 }
 
-// Largest finite magnitude of the eight, as bf16 bits (they order like integers); `odd` is set where one is not finite.
-__device__ __forceinline__ uint32_t eight_top(const Eight &v, bool &odd)
+// Largest finite magnitude of the sixteen, as bf16 bits (they order like integers); `odd` is set where one is not finite.
+__device__ __forceinline__ uint32_t lane_top(const Sixteen &v, bool &odd)
 {
     constexpr uint32_t kAbs = 0x7fff7fffu;
-    const uint32_t m2 = max_s16x2(max_s16x2(v.w[0] & kAbs, v.w[1] & kAbs), max_s16x2(v.w[2] & kAbs, v.w[3] & kAbs));
+    uint32_t m2 = v.w[0] & kAbs;
+#pragma unroll
+    for (int i = 1; i < 8; ++i)
+        m2 = max_s16x2(m2, v.w[i] & kAbs);
     const uint32_t m = max(m2 & 0xffffu, m2 >> 16);
     if (m < kBf16Inf)
         return m;
     odd = true;
-    return odd_eight_top(v.w[0], v.w[1], v.w[2], v.w[3]);
+    return odd_top(v);
 }
 
-__device__ __forceinline__ uint2 eight_convert(const Eight &v, float inverse, bool odd)
+__device__ __forceinline__ uint4 lane_convert(const Sixteen &v, float inverse, bool odd)
 {
     if (odd)
-        return odd_eight_convert(v.w[0], v.w[1], v.w[2], v.w[3], inverse);
-    uint32_t h[4];
+        return odd_convert(v, inverse);
+    uint32_t h[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 8; ++i)
         h[i] = to_e4m3x2(bf16_lo(v.w[i]) * inverse, bf16_hi(v.w[i]) * inverse);
-    return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+    return make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
 }
 
-__device__ __forceinline__ uint32_t element(const __nv_bfloat16 *p)
+// Elements c .. c+7 of a row of `cols` as four words; those outside [0, cols) are zeros and not read.
+__device__ __forceinline__ uint4 load_elements(const __nv_bfloat16 *row, int64_t c, uint32_t cols)
 {
-    return __ldg(reinterpret_cast<const uint16_t *>(p));
-}
-
-// Elements col .. col+7 of a row of `cols`, one by one, zeros past the end.
-__device__ __forceinline__ Eight load_elements(const __nv_bfloat16 *row, uint32_t col, uint32_t cols)
-{
-    Eight v;
+    uint32_t h[8];
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t c = col + 2 * i;
-        const uint32_t lo = c < cols ? element(row + c) : 0u;
-        const uint32_t hi = c + 1 < cols ? element(row + c + 1) : 0u;
-        v.w[i] = lo | (hi << 16);
-    }
-    return v;
+    for (int j = 0; j < 8; ++j)
+        h[j] = (c + j >= 0 && c + j < static_cast<int64_t>(cols)) ? __ldg(reinterpret_cast<const uint16_t *>(row + c + j)) : 0u;
+    return make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
 }
 
-// Sixteen lanes load the 128 elements from `col0` of a row, lane i the eight from col0 + 8i (zeros past the row's end).
-// VEC: the row starts 16-byte aligned.  Otherwise every lane loads the aligned 16-byte piece its eight begin in, takes the
-// next piece from its neighbour (the last lane loads it) and shifts; pieces that reach beyond the row's own elements are
-// loaded element by element, so nothing outside the row is read.  All 32 lanes of the warp take part; `mine` = this half
-// warp has a row.
+// Elements c .. c+7 where row + c is 16-byte aligned: one load where all of them are the row's own, else one by one.
+__device__ __forceinline__ uint4 load_piece(const __nv_bfloat16 *row, int64_t c, uint32_t cols)
+{
+    if (c >= 0 && c + 8 <= static_cast<int64_t>(cols))
+        return __ldg(reinterpret_cast<const uint4 *>(row + c));
+    if (c + 8 > 0 && c < static_cast<int64_t>(cols))
+        return load_elements(row, c, cols);
+    return make_uint4(0u, 0u, 0u, 0u);
+}
+
+// Eight lanes load the 128 elements from `col0` of a row, lane i the sixteen from col0 + 16i (zeros past the row's end).
+// VEC: the row starts 16-byte aligned.  Otherwise every lane loads the two aligned 16-byte pieces its sixteen begin in,
+// takes the next piece from its neighbour (the last lane loads it) and shifts; nothing outside the row is read.  All 32
+// lanes of the warp take part; `mine` = this group of eight has a row.
 template <bool VEC>
-__device__ __forceinline__ Eight load_block_row(const __nv_bfloat16 *row, uint32_t col0, uint32_t cols, uint32_t lane16,
-                                                bool mine)
+__device__ __forceinline__ Sixteen load_block_row(const __nv_bfloat16 *row, uint32_t col0, uint32_t cols, uint32_t lane8, bool mine)
 {
-    const uint32_t col = col0 + lane16 * 8u;
-    Eight v{};
-    if (VEC) {
-        if (mine) {
-            if (col + 8 <= cols) {
-                const uint4 u = __ldg(reinterpret_cast<const uint4 *>(row + col));
-                v.w[0] = u.x, v.w[1] = u.y, v.w[2] = u.z, v.w[3] = u.w;
-            } else {
-                v = load_elements(row, col, cols);
-            }
-        }
-        return v;
-    }
-    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row + col0) & 15u) / 2u;  // elements past an aligned piece
-    // piece i holds the elements first + 8i .. of the row, first = col0 - off (it may lie before the row)
-    auto piece = [&](uint32_t i) {
-        const int64_t c = static_cast<int64_t>(col0) - off + 8 * static_cast<int64_t>(i);
-        uint4 u = make_uint4(0u, 0u, 0u, 0u);
-        if (c >= 0 && c + 8 <= static_cast<int64_t>(cols)) {
-            u = __ldg(reinterpret_cast<const uint4 *>(row + c));
-        } else if (c + 8 > 0 && c < static_cast<int64_t>(cols)) {
-            uint32_t h[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                h[j] = (c + j >= 0 && c + j < static_cast<int64_t>(cols)) ? element(row + c + j) : 0u;
-            u = make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
-        }
-        return u;
-    };
-    uint4 a = make_uint4(0u, 0u, 0u, 0u), last = a;
+    uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
+    const uint32_t off = VEC ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row + col0) & 15u) / 2u;
+    // the first aligned piece, in elements of the row (it may begin before the row)
+    const int64_t c = static_cast<int64_t>(col0 + lane8 * kLaneElements) - off;
     if (mine) {
-        a = piece(lane16);
-        if (lane16 == 15u && off != 0u)
-            last = piece(16u);
+        a = load_piece(row, c, cols);
+        b = load_piece(row, c + 8, cols);
     }
-    uint4 b;
-    b.x = __shfl_down_sync(0xffffffffu, a.x, 1, 16);
-    b.y = __shfl_down_sync(0xffffffffu, a.y, 1, 16);
-    b.z = __shfl_down_sync(0xffffffffu, a.z, 1, 16);
-    b.w = __shfl_down_sync(0xffffffffu, a.w, 1, 16);
-    if (lane16 == 15u)
-        b = last;
-    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (VEC)
+        return Sixteen{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+    uint4 n;
+    n.x = __shfl_down_sync(0xffffffffu, a.x, 1, 8);
+    n.y = __shfl_down_sync(0xffffffffu, a.y, 1, 8);
+    n.z = __shfl_down_sync(0xffffffffu, a.z, 1, 8);
+    n.w = __shfl_down_sync(0xffffffffu, a.w, 1, 8);
+    if (lane8 == 7u)
+        n = (mine && off != 0u) ? load_piece(row, c + 16, cols) : make_uint4(0u, 0u, 0u, 0u);
+    uint32_t w[12] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, n.x, n.y, n.z, n.w};
     if (off & 4u) {
 #pragma unroll
-        for (int i = 0; i < 6; ++i)
+        for (int i = 0; i < 10; ++i)
             w[i] = w[i + 2];
     }
     if (off & 2u) {
 #pragma unroll
-        for (int i = 0; i < 5; ++i)
+        for (int i = 0; i < 9; ++i)
             w[i] = w[i + 1];
     }
+    Sixteen v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 8; ++i)
         v.w[i] = (off & 1u) ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
     return v;
 }
 
-// Sixteen lanes store 128 bytes from `col0` of a row of Q, lane i the eight from col0 + 8i (none past the row's end).
-// VEC: the row starts 8-byte aligned.  Otherwise each lane stores the two aligned words that end with its bytes, the first
-// of them with its neighbour's last bytes; the ends of the run go byte by byte.  All 32 lanes take part.
+// The lane's sixteen bytes b to row + col .. (none past the row's end).  VEC: the row starts 16-byte aligned.  Otherwise a
+// lane stores the aligned sixteen bytes that end with its own, the first of them its neighbour's last; the ends of a run go
+// byte by byte.  `joined`: the lane before this one holds the sixteen bytes before these; `follows`: the lane after it holds
+// the next ones, if the row has all of them.  All 32 lanes take part.
 template <bool VEC>
-__device__ __forceinline__ void store_block_row(uint8_t *row, uint32_t col0, uint32_t cols, uint32_t lane16, bool mine, uint2 b)
+__device__ __forceinline__ void store_lane(uint8_t *row, uint32_t col, uint32_t cols, bool mine, bool joined, bool follows, uint4 b)
 {
-    const uint32_t col = col0 + lane16 * 8u;
     auto bytes = [&](uint32_t from, uint32_t to) {
+        const uint32_t w[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i)
+        for (uint32_t i = 0; i < 16; ++i)
             if (i >= from && i < to)
-                row[col + i] = static_cast<uint8_t>((i < 4 ? b.x : b.y) >> (8 * (i & 3u)));
+                row[col + i] = static_cast<uint8_t>(w[i / 4] >> (8 * (i & 3u)));
     };
-    const bool full = col + 8 <= cols;
+    const bool full = col + 16 <= cols;
     if (VEC) {
         if (mine && full)
-            *reinterpret_cast<uint2 *>(row + col) = b;
+            *reinterpret_cast<uint4 *>(row + col) = b;
         else if (mine && col < cols)
             bytes(0u, cols - col);
         return;
     }
-    const uint32_t before = __shfl_up_sync(0xffffffffu, b.y, 1, 16);
+    uint32_t w[8] = {__shfl_up_sync(0xffffffffu, b.x, 1), __shfl_up_sync(0xffffffffu, b.y, 1), __shfl_up_sync(0xffffffffu, b.z, 1),
+                     __shfl_up_sync(0xffffffffu, b.w, 1), b.x, b.y, b.z, b.w};
     if (!mine || col >= cols)
         return;
     if (!full) {
+        // the neighbour's store ends where it ends: these go byte by byte, with its last ones (it has no follower)
         bytes(0u, cols - col);
         return;
     }
-    const uint32_t s = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row + col) & 3u);
-    uint32_t *word = reinterpret_cast<uint32_t *>(row + col - s);
-    if (s == 0u || lane16 != 0u)
-        word[0] = __funnelshift_l(before, b.x, 8u * s);
-    else
-        bytes(0u, 4u - s);
-    word[1] = __funnelshift_l(b.x, b.y, 8u * s);
-    if (s != 0u && (lane16 == 15u || col + 16 > cols))
-        bytes(8u - s, 8u);
+    const uint32_t s = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row + col) & 15u);
+    if (s == 0u) {
+        *reinterpret_cast<uint4 *>(row + col) = b;
+        return;
+    }
+    if (joined) {
+        const uint32_t t = 16u - s;  // bytes of the sixteen before that come first
+        if (t & 8u) {
+#pragma unroll
+            for (int i = 0; i < 6; ++i)
+                w[i] = w[i + 2];
+        }
+        if (t & 4u) {
+#pragma unroll
+            for (int i = 0; i < 5; ++i)
+                w[i] = w[i + 1];
+        }
+        const uint32_t r = 8u * (t & 3u);
+        *reinterpret_cast<uint4 *>(row + col - s) = make_uint4(__funnelshift_r(w[0], w[1], r), __funnelshift_r(w[1], w[2], r),
+                                                               __funnelshift_r(w[2], w[3], r), __funnelshift_r(w[3], w[4], r));
+    } else {
+        bytes(0u, 16u - s);
+    }
+    if (!(follows && col + 32 <= cols))
+        bytes(16u - s, 16u);
 }
 
-// 1 x 128 blocks: 16 lanes of a warp hold one block, eight elements each; every half warp keeps UNROLL blocks in flight.
-template <bool VEC, uint32_t UNROLL>
+// 1 x 128 blocks: eight lanes hold a block; every group of eight keeps UNROLL blocks in flight.
+template <bool XVEC, bool QVEC, uint32_t UNROLL>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
 {
     if (p.pdl) {
@@ -246,22 +242,22 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
         ptx::grid_dependency_wait();
     }
     const uint32_t across = (p.cols + kQuantBlock - 1) / kQuantBlock;
-    const uint32_t lane16 = threadIdx.x & 15u;
-    // Half warp i takes the blocks i, i + step, ... in row order; the row and the block within it are carried along.
-    const uint32_t step = gridDim.x * (blockDim.x / 16);
-    const uint32_t first = (blockIdx.x * blockDim.x + threadIdx.x) / 16;
+    const uint32_t lane = threadIdx.x & 31u, lane8 = threadIdx.x & 7u;
+    // Group i takes the blocks i, i + step, ... in row order; the row and the block within it are carried along.
+    const uint32_t step = gridDim.x * (blockDim.x / 8);
+    const uint32_t first = (blockIdx.x * blockDim.x + threadIdx.x) / 8;
     const uint32_t step_rows = step / across, step_blks = step - step_rows * across;
     uint32_t row = first / across, blk = first - row * across;
-    // whole warps go round (the shuffles need both halves of one): the warp's first half has the lower block
-    for (uint32_t lead = __shfl_sync(0xffffffffu, row, 0); lead < p.rows; lead = __shfl_sync(0xffffffffu, row, 0)) {
-        Eight v[UNROLL];
+    // whole warps go round (the shuffles need every group of one): the warp's first group has the lowest block
+    while (__shfl_sync(0xffffffffu, row, 0) < p.rows) {
+        Sixteen v[UNROLL];
         uint32_t at_row[UNROLL], at_blk[UNROLL];
 #pragma unroll
         for (uint32_t u = 0; u < UNROLL; ++u) {
             at_row[u] = row;
             at_blk[u] = blk;
             const bool mine = row < p.rows;
-            v[u] = load_block_row<VEC>(p.x + static_cast<uint64_t>(mine ? row : 0u) * p.ldx, blk * kQuantBlock, p.cols, lane16, mine);
+            v[u] = load_block_row<XVEC>(p.x + static_cast<uint64_t>(mine ? row : 0u) * p.ldx, blk * kQuantBlock, p.cols, lane8, mine);
             row += step_rows;
             blk += step_blks;
             if (blk >= across) {
@@ -273,22 +269,24 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
         for (uint32_t u = 0; u < UNROLL; ++u) {
             const bool mine = at_row[u] < p.rows;
             bool odd = false;
-            uint32_t top = eight_top(v[u], odd);
+            uint32_t top = lane_top(v[u], odd);
 #pragma unroll
-            for (uint32_t d = 8; d > 0; d >>= 1)
+            for (uint32_t d = 4; d > 0; d >>= 1)
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
             float scale, inverse;
             block_scale(top, scale, inverse);
-            store_block_row<VEC>(p.q + static_cast<uint64_t>(mine ? at_row[u] : 0u) * p.ldq, at_blk[u] * kQuantBlock, p.cols, lane16,
-                                 mine, eight_convert(v[u], inverse, odd));
-            if (mine && lane16 == 0)
+            // neighbouring groups of a warp have neighbouring blocks: runs go on across them within a row
+            store_lane<QVEC>(p.q + static_cast<uint64_t>(mine ? at_row[u] : 0u) * p.ldq, at_blk[u] * kQuantBlock + lane8 * kLaneElements,
+                             p.cols, mine, lane != 0u && (lane8 != 0u || at_blk[u] != 0u), lane != 31u,
+                             lane_convert(v[u], inverse, odd));
+            if (mine && lane8 == 0)
                 p.scales[static_cast<uint64_t>(at_row[u]) * p.ld_scales + at_blk[u]] = scale;
         }
     }
 }
 
-// 128 x 128 blocks: one CTA per block, 16 threads per row, eight rows per thread.
-template <bool VEC>
+// 128 x 128 blocks: one CTA per block, eight threads per row, four rows per thread.
+template <bool XVEC, bool QVEC>
 __global__ void __launch_bounds__(256) quantize_blocks_kernel(const QuantParams p)
 {
     __shared__ uint32_t warp_top[8];
@@ -298,20 +296,20 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const QuantParams 
     }
     const uint32_t across = (p.cols + kQuantBlock - 1) / kQuantBlock;
     const uint32_t down = blockIdx.x / across, blk = blockIdx.x - down * across;
-    const uint32_t lane16 = threadIdx.x & 15u;
-    const uint32_t row0 = down * kQuantBlock + threadIdx.x / 16u;
-    Eight v[8];
+    const uint32_t lane8 = threadIdx.x & 7u;
+    const uint32_t row0 = down * kQuantBlock + threadIdx.x / 8u;
+    Sixteen v[4];
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-        const uint32_t row = row0 + 16u * i;
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t row = row0 + 32u * i;
         const bool mine = row < p.rows;
-        v[i] = load_block_row<VEC>(p.x + static_cast<uint64_t>(mine ? row : 0u) * p.ldx, blk * kQuantBlock, p.cols, lane16, mine);
+        v[i] = load_block_row<XVEC>(p.x + static_cast<uint64_t>(mine ? row : 0u) * p.ldx, blk * kQuantBlock, p.cols, lane8, mine);
     }
     bool odd = false;
     uint32_t top = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i)
-        top = max(top, eight_top(v[i], odd));
+    for (uint32_t i = 0; i < 4; ++i)
+        top = max(top, lane_top(v[i], odd));
 #pragma unroll
     for (uint32_t d = 16; d > 0; d >>= 1)
         top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
@@ -324,11 +322,11 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const QuantParams 
     float scale, inverse;
     block_scale(top, scale, inverse);
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-        const uint32_t row = row0 + 16u * i;
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t row = row0 + 32u * i;
         const bool mine = row < p.rows;
-        store_block_row<VEC>(p.q + static_cast<uint64_t>(mine ? row : 0u) * p.ldq, blk * kQuantBlock, p.cols, lane16, mine,
-                             eight_convert(v[i], inverse, odd));
+        store_lane<QVEC>(p.q + static_cast<uint64_t>(mine ? row : 0u) * p.ldq, blk * kQuantBlock + lane8 * kLaneElements, p.cols, mine,
+                         lane8 != 0u, lane8 != 7u, lane_convert(v[i], inverse, odd));
     }
     if (threadIdx.x == 0)
         p.scales[static_cast<uint64_t>(down) * p.ld_scales + blk] = scale;
