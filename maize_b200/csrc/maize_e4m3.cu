@@ -58,15 +58,21 @@ maize_status_t maize_quantize_e4m3(maize_ctx_t *ctx, const void *x, uint64_t ldx
     p.cols = cols;
     p.pdl = ctx->pdl;
     // rows of X that loads of 16 bytes take as they are; rows of Q for stores of 16 bytes
-    const bool xvec = ldx % 8 == 0 && aligned(x, 16), qvec = ldq % 16 == 0 && aligned(q, 16);
+    const bool xvec = ldx % 8 == 0 && aligned(x, 16), qvec = xvec && ldq % 16 == 0 && aligned(q, 16);
     DeviceGuard guard(ctx->device);
     cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
     if (block_rows == 1) {
-        // one block per group of eight lanes until the SMs are full, then several in flight
-        const uint64_t want = (uint64_t(rows) * across + 31) / 32, cap = uint64_t(ctx->sm_count) * 6;
+        // A call that does not fill the SMs gives each warp four blocks; a larger one runs of eight (sixteen where the ends of
+        // a run cost more).  More CTAs than fit at a time even out the last round: 8191 x 8191 takes 56 us with 16 per SM, 70
+        // with the 5 that fit; 8192 x 8192 takes 34 with either.
+        const uint64_t blocks = uint64_t(rows) * across, sms = uint64_t(ctx->sm_count);
+        const bool small = blocks <= sms * 6 * 32;
+        const uint32_t run = small ? 4 : (qvec ? 8 : 16);
+        const uint64_t want = (blocks + run * 8 - 1) / (run * 8), cap = sms * 16;
         const uint32_t grid = static_cast<uint32_t>(want < cap ? want : cap);
-        auto kernel = xvec ? (qvec ? maize::quantize_rows_kernel<true, true, 2> : maize::quantize_rows_kernel<true, false, 2>)
-                           : maize::quantize_rows_kernel<false, false, 2>;
+        auto kernel = xvec ? (qvec ? (small ? maize::quantize_rows_kernel<true, true, 1> : maize::quantize_rows_kernel<true, true, 2>)
+                                   : (small ? maize::quantize_rows_kernel<true, false, 1> : maize::quantize_rows_kernel<true, false, 4>))
+                           : (small ? maize::quantize_rows_kernel<false, false, 1> : maize::quantize_rows_kernel<false, false, 4>);
         return maize::launch(ctx, -1, kernel, grid, 256, 0, stream, p);
     }
     const uint64_t blocks = (uint64_t(rows) + 127) / 128 * across;

@@ -114,49 +114,66 @@ __device__ __forceinline__ uint4 lane_convert(const Sixteen &v, float inverse, b
 }
 
 // Elements c .. c+7 of a row of `cols` as four words; those outside [0, cols) are zeros and not read.
-__device__ __forceinline__ uint4 load_elements(const __nv_bfloat16 *row, int64_t c, uint32_t cols)
+__device__ __forceinline__ uint4 load_elements(const __nv_bfloat16 *row, int32_t c, int32_t cols)
 {
     uint32_t h[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-        h[j] = (c + j >= 0 && c + j < static_cast<int64_t>(cols)) ? __ldg(reinterpret_cast<const uint16_t *>(row + c + j)) : 0u;
+        h[j] = (c + j >= 0 && c + j < cols) ? __ldg(reinterpret_cast<const uint16_t *>(row + c + j)) : 0u;
     return make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
 }
 
 // Elements c .. c+7 where row + c is 16-byte aligned: one load where all of them are the row's own, else one by one.
-__device__ __forceinline__ uint4 load_piece(const __nv_bfloat16 *row, int64_t c, uint32_t cols)
+__device__ __forceinline__ uint4 load_piece(const __nv_bfloat16 *row, int32_t c, int32_t cols)
 {
-    if (c >= 0 && c + 8 <= static_cast<int64_t>(cols))
+    if (c >= 0 && c + 8 <= cols)
         return __ldg(reinterpret_cast<const uint4 *>(row + c));
-    if (c + 8 > 0 && c < static_cast<int64_t>(cols))
+    if (c + 8 > 0 && c < cols)
         return load_elements(row, c, cols);
     return make_uint4(0u, 0u, 0u, 0u);
 }
 
 // Eight lanes load the 128 elements from `col0` of a row, lane i the sixteen from col0 + 16i (zeros past the row's end).
-// VEC: the row starts 16-byte aligned.  Otherwise every lane loads the two aligned 16-byte pieces its sixteen begin in,
-// takes the next piece from its neighbour (the last lane loads it) and shifts; nothing outside the row is read.  All 32
-// lanes of the warp take part; `mine` = this group of eight has a row.
-template <bool VEC>
-__device__ __forceinline__ Sixteen load_block_row(const __nv_bfloat16 *row, uint32_t col0, uint32_t cols, uint32_t lane8, bool mine)
+// Where the row starts 16-byte aligned, two loads bring them.  Otherwise every lane loads the two aligned 16-byte pieces its
+// sixteen begin in (load_pair), gets the next piece from the lane that holds it, or loads it, and shifts (shift_pair);
+// nothing outside the row is read.
+struct Pair {
+    uint4 a, b;
+};
+
+// Elements of the row by which the block's first element is past an aligned piece.
+__device__ __forceinline__ uint32_t piece_offset(const __nv_bfloat16 *row, uint32_t col0)
 {
-    uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
-    const uint32_t off = VEC ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row + col0) & 15u) / 2u;
-    // the first aligned piece, in elements of the row (it may begin before the row)
-    const int64_t c = static_cast<int64_t>(col0 + lane8 * kLaneElements) - off;
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row + col0) & 15u) / 2u;
+}
+
+__device__ __forceinline__ Pair load_pair(const __nv_bfloat16 *row, uint32_t col0, uint32_t cols, uint32_t lane8, uint32_t off, bool mine)
+{
+    Pair r{make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+    // the first piece in elements of the row: it may begin before the row
+    const int32_t c = static_cast<int32_t>(col0 + lane8 * kLaneElements - off), end = static_cast<int32_t>(cols);
     if (mine) {
-        a = load_piece(row, c, cols);
-        b = load_piece(row, c + 8, cols);
+        r.a = load_piece(row, c, end);
+        r.b = load_piece(row, c + 8, end);
     }
-    if (VEC)
-        return Sixteen{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
-    uint4 n;
-    n.x = __shfl_down_sync(0xffffffffu, a.x, 1, 8);
-    n.y = __shfl_down_sync(0xffffffffu, a.y, 1, 8);
-    n.z = __shfl_down_sync(0xffffffffu, a.z, 1, 8);
-    n.w = __shfl_down_sync(0xffffffffu, a.w, 1, 8);
-    if (lane8 == 7u)
-        n = (mine && off != 0u) ? load_piece(row, c + 16, cols) : make_uint4(0u, 0u, 0u, 0u);
+    return r;
+}
+
+__device__ __forceinline__ uint4 shfl_down4(const uint4 &v)
+{
+    return make_uint4(__shfl_down_sync(0xffffffffu, v.x, 1), __shfl_down_sync(0xffffffffu, v.y, 1),
+                      __shfl_down_sync(0xffffffffu, v.z, 1), __shfl_down_sync(0xffffffffu, v.w, 1));
+}
+
+__device__ __forceinline__ uint4 shfl4(const uint4 &v, int lane)
+{
+    return make_uint4(__shfl_sync(0xffffffffu, v.x, lane), __shfl_sync(0xffffffffu, v.y, lane), __shfl_sync(0xffffffffu, v.z, lane),
+                      __shfl_sync(0xffffffffu, v.w, lane));
+}
+
+__device__ __forceinline__ Sixteen shift_pair(const Pair &r, const uint4 &n, uint32_t off)
+{
+    const uint4 a = r.a, b = r.b;
     uint32_t w[12] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, n.x, n.y, n.z, n.w};
     if (off & 4u) {
 #pragma unroll
@@ -175,35 +192,42 @@ __device__ __forceinline__ Sixteen load_block_row(const __nv_bfloat16 *row, uint
     return v;
 }
 
-// The lane's sixteen bytes b to row + col .. (none past the row's end).  VEC: the row starts 16-byte aligned.  Otherwise a
-// lane stores the aligned sixteen bytes that end with its own, the first of them its neighbour's last; the ends of a run go
-// byte by byte.  `joined`: the lane before this one holds the sixteen bytes before these; `follows`: the lane after it holds
-// the next ones, if the row has all of them.  All 32 lanes take part.
-template <bool VEC>
-__device__ __forceinline__ void store_lane(uint8_t *row, uint32_t col, uint32_t cols, bool mine, bool joined, bool follows, uint4 b)
+__device__ __forceinline__ uint4 shfl_up4(const uint4 &v)
 {
-    auto bytes = [&](uint32_t from, uint32_t to) {
+    return make_uint4(__shfl_up_sync(0xffffffffu, v.x, 1), __shfl_up_sync(0xffffffffu, v.y, 1), __shfl_up_sync(0xffffffffu, v.z, 1),
+                      __shfl_up_sync(0xffffffffu, v.w, 1));
+}
+
+// The lane's sixteen bytes b to row + col .. (none past the row's end).  VEC: the row starts 16-byte aligned.  Otherwise a
+// lane stores the aligned sixteen bytes that end with its own, the first of them the last of `before`, the sixteen in front
+// of its own (`joined`: the row has them and a lane of this warp holds them); the ends of a run go in pieces.  `follows`: a
+// lane of this warp holds the next sixteen, if the row has all of them.
+template <bool VEC>
+__device__ __forceinline__ void store_lane(uint8_t *row, uint32_t col, uint32_t cols, bool mine, bool joined, bool follows,
+                                           const uint4 &before, const uint4 &b)
+{
+    auto bytes = [&](uint32_t count) {  // the first `count`
         const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (uint32_t i = 0; i < 16; ++i)
-            if (i >= from && i < to)
-                row[col + i] = static_cast<uint8_t>(w[i / 4] >> (8 * (i & 3u)));
+#pragma unroll 1
+        for (uint32_t i = 0; i < count; ++i) {
+            const uint32_t word = (i & 8u) ? ((i & 4u) ? w[3] : w[2]) : ((i & 4u) ? w[1] : w[0]);
+            row[col + i] = static_cast<uint8_t>(word >> (8 * (i & 3u)));
+        }
     };
     const bool full = col + 16 <= cols;
     if (VEC) {
         if (mine && full)
             *reinterpret_cast<uint4 *>(row + col) = b;
         else if (mine && col < cols)
-            bytes(0u, cols - col);
+            bytes(cols - col);
         return;
     }
-    uint32_t w[8] = {__shfl_up_sync(0xffffffffu, b.x, 1), __shfl_up_sync(0xffffffffu, b.y, 1), __shfl_up_sync(0xffffffffu, b.z, 1),
-                     __shfl_up_sync(0xffffffffu, b.w, 1), b.x, b.y, b.z, b.w};
+    uint32_t w[8] = {before.x, before.y, before.z, before.w, b.x, b.y, b.z, b.w};
     if (!mine || col >= cols)
         return;
     if (!full) {
         // the neighbour's store ends where it ends: these go byte by byte, with its last ones (it has no follower)
-        bytes(0u, cols - col);
+        bytes(cols - col);
         return;
     }
     const uint32_t s = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row + col) & 15u);
@@ -227,13 +251,67 @@ __device__ __forceinline__ void store_lane(uint8_t *row, uint32_t col, uint32_t 
         *reinterpret_cast<uint4 *>(row + col - s) = make_uint4(__funnelshift_r(w[0], w[1], r), __funnelshift_r(w[1], w[2], r),
                                                                __funnelshift_r(w[2], w[3], r), __funnelshift_r(w[3], w[4], r));
     } else {
-        bytes(0u, 16u - s);
+        // the first 16 - s bytes, up to an aligned address: 1, 2, 4, 8 as the count has them
+        uint32_t v[4] = {b.x, b.y, b.z, b.w};
+        uint8_t *to = row + col;
+        const uint32_t t = 16u - s;
+        if (t & 1u) {
+            *to = static_cast<uint8_t>(v[0]);
+            to += 1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[i] = __funnelshift_r(v[i], i < 3 ? v[i + 1] : 0u, 8);
+        }
+        if (t & 2u) {
+            *reinterpret_cast<uint16_t *>(to) = static_cast<uint16_t>(v[0]);
+            to += 2;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[i] = __funnelshift_r(v[i], i < 3 ? v[i + 1] : 0u, 16);
+        }
+        if (t & 4u) {
+            *reinterpret_cast<uint32_t *>(to) = v[0];
+            to += 4;
+            v[0] = v[1], v[1] = v[2];
+        }
+        if (t & 8u)
+            *reinterpret_cast<uint2 *>(to) = make_uint2(v[0], v[1]);
     }
-    if (!(follows && col + 32 <= cols))
-        bytes(16u - s, 16u);
+    if (!(follows && col + 32 <= cols)) {
+        // the last s bytes, from an aligned address: 8, 4, 2, 1.  They are the top of the sixteen: shifted down first.
+        uint32_t v[7] = {b.x, b.y, b.z, b.w, 0u, 0u, 0u};
+        const uint32_t t = 16u - s;
+        if (t & 8u)
+            v[0] = v[2], v[1] = v[3], v[2] = 0u, v[3] = 0u;
+        if (t & 4u)
+            v[0] = v[1], v[1] = v[2], v[2] = v[3], v[3] = 0u;
+        const uint32_t r = 8u * (t & 3u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            v[i] = __funnelshift_r(v[i], v[i + 1], r);
+        uint8_t *to = row + col + t;
+        if (s & 8u) {
+            *reinterpret_cast<uint2 *>(to) = make_uint2(v[0], v[1]);
+            to += 8;
+            v[0] = v[2], v[1] = v[3];
+        }
+        if (s & 4u) {
+            *reinterpret_cast<uint32_t *>(to) = v[0];
+            to += 4;
+            v[0] = v[1];
+        }
+        if (s & 2u) {
+            *reinterpret_cast<uint16_t *>(to) = static_cast<uint16_t>(v[0]);
+            to += 2;
+            v[0] >>= 16;
+        }
+        if (s & 1u)
+            *to = static_cast<uint8_t>(v[0]);
+    }
 }
 
-// 1 x 128 blocks: eight lanes hold a block; every group of eight keeps UNROLL blocks in flight.
+// 1 x 128 blocks: eight lanes hold a block, a warp four neighbouring ones at a time and UNROLL times that in a run; only at
+// the ends of a run are rows of Q that start anywhere stored in pieces.
 template <bool XVEC, bool QVEC, uint32_t UNROLL>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
 {
@@ -243,28 +321,60 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
     }
     const uint32_t across = (p.cols + kQuantBlock - 1) / kQuantBlock;
     const uint32_t lane = threadIdx.x & 31u, lane8 = threadIdx.x & 7u;
-    // Group i takes the blocks i, i + step, ... in row order; the row and the block within it are carried along.
-    const uint32_t step = gridDim.x * (blockDim.x / 8);
-    const uint32_t first = (blockIdx.x * blockDim.x + threadIdx.x) / 8;
+    const uint32_t warps = gridDim.x * (blockDim.x / 32), warp = (blockIdx.x * blockDim.x + threadIdx.x) / 32;
+    // from one run of this warp to its next, in rows and blocks (a division here, none below)
+    const uint32_t step = (warps - 1) * UNROLL * 4;
     const uint32_t step_rows = step / across, step_blks = step - step_rows * across;
-    uint32_t row = first / across, blk = first - row * across;
+    const uint32_t four_rows = 4u / across, four_blks = 4u - four_rows * across;
+    const uint64_t first = static_cast<uint64_t>(warp) * UNROLL * 4 + lane / 8u;
+    uint32_t row = static_cast<uint32_t>(first / across), blk = static_cast<uint32_t>(first - static_cast<uint64_t>(row) * across);
+    auto advance = [&](uint32_t rows, uint32_t blks) {
+        row += rows;
+        blk += blks;
+        if (blk >= across) {
+            blk -= across;
+            ++row;
+        }
+    };
     // whole warps go round (the shuffles need every group of one): the warp's first group has the lowest block
     while (__shfl_sync(0xffffffffu, row, 0) < p.rows) {
+        Pair raw[UNROLL];
         Sixteen v[UNROLL];
-        uint32_t at_row[UNROLL], at_blk[UNROLL];
+        uint32_t at_row[UNROLL], at_blk[UNROLL], off[UNROLL];
 #pragma unroll
         for (uint32_t u = 0; u < UNROLL; ++u) {
             at_row[u] = row;
             at_blk[u] = blk;
             const bool mine = row < p.rows;
-            v[u] = load_block_row<XVEC>(p.x + static_cast<uint64_t>(mine ? row : 0u) * p.ldx, blk * kQuantBlock, p.cols, lane8, mine);
-            row += step_rows;
-            blk += step_blks;
-            if (blk >= across) {
-                blk -= across;
-                ++row;
-            }
+            const __nv_bfloat16 *x = p.x + static_cast<uint64_t>(mine ? row : 0u) * p.ldx;
+            off[u] = XVEC ? 0u : piece_offset(x, blk * kQuantBlock);
+            raw[u] = load_pair(x, blk * kQuantBlock, p.cols, lane8, off[u], mine);
+            advance(four_rows, four_blks);
         }
+        advance(step_rows, step_blks);
+#pragma unroll
+        for (uint32_t u = 0; u < UNROLL; ++u) {
+            if (XVEC) {
+                v[u] = Sixteen{{raw[u].a.x, raw[u].a.y, raw[u].a.z, raw[u].a.w, raw[u].b.x, raw[u].b.y, raw[u].b.z, raw[u].b.w}};
+                continue;
+            }
+            // the next piece: the lane after holds it, for the last lane the first one of the run's next four blocks
+            uint4 n = shfl_down4(raw[u].a);
+            if (u + 1 < UNROLL) {
+                const uint4 next = shfl4(raw[u + 1].a, 0);
+                if (lane == 31u)
+                    n = next;
+            }
+            if (lane8 == 7u && ((u + 1 == UNROLL && lane == 31u) || at_blk[u] + 1 == across)) {
+                n = make_uint4(0u, 0u, 0u, 0u);
+                if (at_row[u] < p.rows && off[u] != 0u)
+                    n = load_piece(p.x + static_cast<uint64_t>(at_row[u]) * p.ldx,
+                                   static_cast<int32_t>(at_blk[u] * kQuantBlock + 8u * kLaneElements - off[u]),
+                                   static_cast<int32_t>(p.cols));
+            }
+            v[u] = shift_pair(raw[u], n, off[u]);
+        }
+        uint4 last = make_uint4(0u, 0u, 0u, 0u);  // lane 31's bytes of the four blocks before
 #pragma unroll
         for (uint32_t u = 0; u < UNROLL; ++u) {
             const bool mine = at_row[u] < p.rows;
@@ -275,10 +385,18 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
             float scale, inverse;
             block_scale(top, scale, inverse);
-            // neighbouring groups of a warp have neighbouring blocks: runs go on across them within a row
+            const uint4 b = lane_convert(v[u], inverse, odd);
+            uint4 before = last;
+            if (!QVEC) {
+                const uint4 up = shfl_up4(b);
+                if (lane != 0u)
+                    before = up;
+                if (u + 1 < UNROLL)
+                    last = shfl4(b, 31);
+            }
             store_lane<QVEC>(p.q + static_cast<uint64_t>(mine ? at_row[u] : 0u) * p.ldq, at_blk[u] * kQuantBlock + lane8 * kLaneElements,
-                             p.cols, mine, lane != 0u && (lane8 != 0u || at_blk[u] != 0u), lane != 31u,
-                             lane_convert(v[u], inverse, odd));
+                             p.cols, mine, (lane != 0u || u != 0u) && (lane8 != 0u || at_blk[u] != 0u), lane != 31u || u + 1 < UNROLL,
+                             before, b);
             if (mine && lane8 == 0)
                 p.scales[static_cast<uint64_t>(at_row[u]) * p.ld_scales + at_blk[u]] = scale;
         }
@@ -298,12 +416,31 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const QuantParams 
     const uint32_t down = blockIdx.x / across, blk = blockIdx.x - down * across;
     const uint32_t lane8 = threadIdx.x & 7u;
     const uint32_t row0 = down * kQuantBlock + threadIdx.x / 8u;
+    Pair raw[4];
     Sixteen v[4];
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
         const uint32_t row = row0 + 32u * i;
         const bool mine = row < p.rows;
-        v[i] = load_block_row<XVEC>(p.x + static_cast<uint64_t>(mine ? row : 0u) * p.ldx, blk * kQuantBlock, p.cols, lane8, mine);
+        const __nv_bfloat16 *x = p.x + static_cast<uint64_t>(mine ? row : 0u) * p.ldx;
+        raw[i] = load_pair(x, blk * kQuantBlock, p.cols, lane8, XVEC ? 0u : piece_offset(x, blk * kQuantBlock), mine);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        if (XVEC) {
+            v[i] = Sixteen{{raw[i].a.x, raw[i].a.y, raw[i].a.z, raw[i].a.w, raw[i].b.x, raw[i].b.y, raw[i].b.z, raw[i].b.w}};
+            continue;
+        }
+        const uint32_t row = row0 + 32u * i;
+        const __nv_bfloat16 *x = p.x + static_cast<uint64_t>(row < p.rows ? row : 0u) * p.ldx;
+        const uint32_t off = piece_offset(x, blk * kQuantBlock);
+        uint4 n = shfl_down4(raw[i].a);
+        if (lane8 == 7u) {
+            n = make_uint4(0u, 0u, 0u, 0u);
+            if (row < p.rows && off != 0u)
+                n = load_piece(x, static_cast<int32_t>(blk * kQuantBlock + 8u * kLaneElements - off), static_cast<int32_t>(p.cols));
+        }
+        v[i] = shift_pair(raw[i], n, off);
     }
     bool odd = false;
     uint32_t top = 0;
@@ -325,8 +462,9 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const QuantParams 
     for (uint32_t i = 0; i < 4; ++i) {
         const uint32_t row = row0 + 32u * i;
         const bool mine = row < p.rows;
+        const uint4 b = lane_convert(v[i], inverse, odd);
         store_lane<QVEC>(p.q + static_cast<uint64_t>(mine ? row : 0u) * p.ldq, blk * kQuantBlock + lane8 * kLaneElements, p.cols, mine,
-                         lane8 != 0u, lane8 != 7u, lane_convert(v[i], inverse, odd));
+                         lane8 != 0u, lane8 != 7u, QVEC ? b : shfl_up4(b), b);
     }
     if (threadIdx.x == 0)
         p.scales[static_cast<uint64_t>(down) * p.ld_scales + blk] = scale;
