@@ -5,6 +5,7 @@
 
 #include "maize_host.cuh"
 #include "gemm_e4m3_sm100.cuh"
+#include "gemm_e4m3_sm100_skinny.cuh"
 #include "quantize_e4m3.cuh"
 
 namespace {
@@ -21,6 +22,55 @@ maize_status_t byte_map(maize_ctx_t *ctx, CUtensorMap *map, const void *base, ui
     const uint32_t box[2] = {maize::kF8BlockK, box_rows};
     return maize::encode_map(ctx, map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, 2, dims, strides, box,
                              static_cast<CUtensorMapL2promotion>(ctx->tma_promotion));
+}
+
+template <uint32_t NT, uint32_t STAGES>
+maize_status_t launch_skinny(maize_ctx_t *ctx, int slot, const CUtensorMap &ta, const CUtensorMap &tb,
+                             const maize::F8SkinnyParams &f, uint32_t grid, cudaStream_t stream)
+{
+    return maize::launch(ctx, slot, maize::gemm_e4m3_sm100_skinny<NT, STAGES>, grid, maize::kNumThreads,
+                         maize::F8SkinnySmemLayout<NT, STAGES>::kDynamicBytes, stream, ta, tb, f);
+}
+
+// M <= 128: tiles of up to 128 rows of B, as tall as fills whole rounds of the CTA pairs (never below 32 rows: a shorter
+// tile reads the rows of A more often than it gains).
+maize_status_t skinny(maize_ctx_t *ctx, const void *a, uint64_t lda, const float *sa, uint64_t ld_sa, const void *b, uint64_t ldb,
+                      const float *sb, uint64_t ld_sb, void *c, uint64_t ldc, uint32_t m, uint32_t n, uint32_t k, cudaStream_t stream)
+{
+    const uint32_t nt = m <= 16 ? 16 : (m <= 32 ? 32 : (m <= 64 ? 64 : 128));
+    const uint64_t pairs = maize::persistent_grid(ctx, 0xffffffffull, 2) / 2;
+    const uint64_t rounds = (uint64_t(n) + pairs * 128 - 1) / (pairs * 128);
+    uint32_t rows = static_cast<uint32_t>((uint64_t(n) + pairs * rounds - 1) / (pairs * rounds));
+    rows = (rows + 7) / 8 * 8;
+    if (rows < 32)
+        rows = 32;
+    maize::F8SkinnyParams f = {};
+    f.c.c = static_cast<__nv_bfloat16 *>(c);
+    f.c.ldc = ldc;
+    f.c.rows = m;
+    f.c.n = n;
+    f.c.k = k;
+    f.c.c_pair_ok = (ldc % 2 == 0 && aligned(c, 4)) ? 1u : 0u;
+    f.c.pdl = ctx->pdl;
+    f.c.status = ctx->d_status;
+    f.c.timeout_ns = ctx->timeout_ns;
+    f.sa = sa;
+    f.sb = sb;
+    f.ld_sa = ld_sa;
+    f.ld_sb = ld_sb;
+    f.tile_rows = rows;
+    f.tiles = (n + rows - 1) / rows;
+    CUtensorMap ta, tb;
+    maize_status_t st;
+    if ((st = byte_map(ctx, &ta, a, m, k, lda, nt)) != MAIZE_OK || (st = byte_map(ctx, &tb, b, n, k, ldb, rows)) != MAIZE_OK)
+        return st;
+    const uint32_t grid = maize::persistent_grid(ctx, f.tiles, 2);
+    switch (nt) {
+    case 16: return launch_skinny<16, 11>(ctx, maize::kAttrE4m3Skinny, ta, tb, f, grid, stream);
+    case 32: return launch_skinny<32, 10>(ctx, maize::kAttrE4m3Skinny + 1, ta, tb, f, grid, stream);
+    case 64: return launch_skinny<64, 7>(ctx, maize::kAttrE4m3Skinny + 2, ta, tb, f, grid, stream);
+    default: return launch_skinny<128, 4>(ctx, maize::kAttrE4m3Skinny + 3, ta, tb, f, grid, stream);
+    }
 }
 
 }  // namespace
@@ -119,6 +169,9 @@ maize_status_t maize_gemm_e4m3(maize_ctx_t *ctx, const void *a, uint64_t lda, co
         return fail(ctx, MAIZE_ERR_UNSUPPORTED, "A and B must be 16-byte aligned");
     if (lda >= (1ull << 40) || ldb >= (1ull << 40))
         return fail(ctx, MAIZE_ERR_UNSUPPORTED, "row pitch beyond the TMA limit of 2^40 bytes");
+    if (m <= 128 && kblocks <= 2 * maize::kF8SkinnyMaxKb)
+        return skinny(ctx, a, lda, static_cast<const float *>(a_scales), ld_a_scales, b, ldb, static_cast<const float *>(b_scales),
+                      ld_b_scales, c, ldc, m, n, k, stream);
     CUtensorMap ta, tb, tc;
     maize_status_t st;
     if ((st = byte_map(ctx, &ta, a, m, k, lda, maize::kBlockM)) != MAIZE_OK ||
