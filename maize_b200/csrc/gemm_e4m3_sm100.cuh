@@ -102,7 +102,8 @@ __device__ __forceinline__ void f8_store(const GemmParams &p, const CUtensorMap 
 }
 
 // acc[first .. first + 15] += v * ss: 32 columns of one row, in pairs.
-__device__ __forceinline__ void f8_promote(uint64_t (&acc)[64], int first, const uint32_t (&v)[32], uint64_t ss)
+template <uint32_t PAIRS>
+__device__ __forceinline__ void f8_promote(uint64_t (&acc)[PAIRS], int first, const uint32_t (&v)[32], uint64_t ss)
 {
 #pragma unroll
     for (int i = 0; i < 16; ++i)

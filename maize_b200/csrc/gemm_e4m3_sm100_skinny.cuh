@@ -1,79 +1,69 @@
 // The e4m3 product for few rows of A (M <= 128): bound by reading B once.
 //
-// As in the grouped product, B is the M side of the MMA (up to 128 of its rows per tile) and the rows of A its N side
-// (NT = 16, 32, 64 or 128).  A cluster of two CTAs shares a tile and splits K: each takes half of the k-blocks, promotes
-// them in registers (lane = row of B, one register per row of A) and sends the other CTA half of its sums through
-// distributed shared memory; each then rounds and stores half of the rows of A.  No global scratch, a fixed order of sums.
+// Rows of A are the M side of the MMA, up to 256 rows of B its N side: an MMA takes about 128 cycles for the 32 k of its 128
+// M-side rows whatever its N, so the operand that has to stream belongs on the N side (with B on the M side 16 x 16384 x 4096
+// took 16.6 us, bound by the MMAs; 11.3 this way, 6.0 TB/s).  For M <= 32 (64) the rows of A are loaded four times (twice)
+// into the 128 lanes, so that every promotion warp has lanes with all rows and only some of the columns: REPL copies.  Only
+// the m rows there are are loaded (a box that reaches past the end of A takes longer: 17 against 11 us for one row of A);
+// what lies in the other lanes is never stored.  For 64 < M the tile is 128 wide, so that four accumulator buffers fit and
+// the MMA does not wait for hand-overs.
 //
-// The tile's height is chosen by the host so that the tiles fill whole rounds of CTA pairs (16384 rows over 74 pairs: two
-// rounds of 112 rows); a tile may then touch two scale blocks of B, so the scale of B is per lane.  The scales of A for this
-// CTA's k-blocks are read once into shared memory, transposed.
+// A cluster of S = 2 or 4 CTAs shares a tile and splits K: each promotes the k-blocks of its part in registers (lane = row
+// of A, one register per row of B), then sends every other CTA the sums of that CTA's share of the columns through distributed
+// shared memory; each adds its share in the order of the parts, rounds once and stores.  No global scratch, a fixed order.
+// (Eight parts lost more in the exchange and in clusters that do not fit beside each other than they gained.)
 //
-// NT columns of TMEM per k-block leave room for four accumulator buffers, so the MMA never waits for a hand-over; the ring
-// holds 6 to 10 stages of 128 k (128 bytes per row).
+// The host picks the tile's width so that the tiles fill whole rounds of clusters (16384 rows over 74 pairs: one round of
+// 224).  The columns of a warp lie in at most two scale blocks of B, each chunk of 32 in one.
 #pragma once
 #include "gemm_e4m3_sm100.cuh"
-#include "gemm_sm100_grouped.cuh"
 
 namespace maize {
 
-constexpr uint32_t kF8SkinnyMaxKb = 64;  // k-blocks per CTA whose scales fit in shared memory: K <= 16384
+constexpr uint32_t kF8SkinnyThreads = 64 + 32 * 8;
 
 struct F8SkinnyParams {
-    GroupedParams c;   // C, its pitch and alignment, n = N, k = K, rows = M (no offsets)
+    GemmParams g;  // C and the sizes; tiles_n = tiles
     const float *sa, *sb;
     uint64_t ld_sa, ld_sb;
-    uint32_t tile_rows;  // rows of B per tile, a multiple of 8, at most 128
-    uint32_t tiles;
+    uint32_t bn;  // rows of B per tile, a multiple of 32, at most 256
 };
 
-template <uint32_t NT, uint32_t STAGES>
-struct F8SkinnySmemLayout {
-    static constexpr uint32_t kBBytes = 128 * kF8BlockK;
-    static constexpr uint32_t kABytes = NT * kF8BlockK;
-    static constexpr uint32_t kStageBytes = kBBytes + kABytes;
-    static constexpr uint32_t kExchangeOffset = STAGES * kStageBytes;  // the other CTA's sums for this CTA's half of the rows
-    static constexpr uint32_t kExchangeBytes = 128 * (NT / 2) * 4;
-    static constexpr uint32_t kScaleAOffset = kExchangeOffset + kExchangeBytes;
-    static constexpr uint32_t kScaleABytes = kF8SkinnyMaxKb * NT * 4;
-    static constexpr uint32_t kScaleBOffset = kScaleAOffset + kScaleABytes;  // two scale blocks x k-blocks, for two tiles
-    static constexpr uint32_t kScaleBBytes = 2 * 2 * kF8SkinnyMaxKb * 4;
-    static constexpr uint32_t kBarOffset = kScaleBOffset + kScaleBBytes;
-    static constexpr uint32_t kNumBars = 2 * STAGES + 8 + 2;
+template <uint32_t REPL, uint32_t S, uint32_t STAGES>
+struct F8SkinnyLayout {
+    static_assert(REPL == 1 || REPL == 2 || REPL == 4, "copies of the rows of A");
+    static constexpr uint32_t kRows = 128 / REPL;                       // rows of A
+    static constexpr uint32_t kWarps = 8;                               // promotion warps, two per quarter of the lanes
+    static constexpr uint32_t kTileCols = REPL == 1 ? 128 : 256;        // rows of B per tile at most
+    static constexpr uint32_t kBuffers = 512 / kTileCols;               // accumulator buffers that fill tensor memory
+    static constexpr uint32_t kWarpCols = REPL == 4 ? 32 : 64;
+    static constexpr uint32_t kShare = kWarpCols / S;                   // columns of a warp that one CTA finishes
+    static constexpr uint32_t kABytes = kBlockM * kF8BlockK;
+    static constexpr uint32_t kBBytes = kTileCols * kF8BlockK;
+    static constexpr uint32_t kStageBytes = kABytes + kBBytes;
+    static constexpr uint32_t kExchangeOffset = STAGES * kStageBytes;   // from each other CTA: [warp][4 columns][lane]
+    static constexpr uint32_t kPartBytes = kWarps * kShare * 32 * 4;
+    static constexpr uint32_t kExchangeBytes = (S - 1) * kPartBytes;
+    static constexpr uint32_t kBarOffset = kExchangeOffset + kExchangeBytes;
+    static constexpr uint32_t kNumBars = 2 * STAGES + 2 * kBuffers + 2;
     static constexpr uint32_t kTmemSlotOffset = kBarOffset + kNumBars * 8;
     static constexpr uint32_t kAbortOffset = kTmemSlotOffset + 4;
     static constexpr uint32_t kUsedBytes = kAbortOffset + 4;
     static constexpr uint32_t kDynamicBytes = kUsedBytes + 1024;
     static_assert(kDynamicBytes <= 232448, "exceeds 227 KiB of shared memory per CTA");
     static_assert(kDynamicBytes > 116224, "two CTAs could share an SM and contend for TMEM");
+    static_assert(kShare < 32 || kShare * 128 >= kStageWarpBytes, "a warp's part of the exchange serves as its staging buffer");
 };
 
-// sum[i] += v[i] * (scale of row i of A * scale of this lane's row of B)
-template <int N>
-__device__ __forceinline__ void f8_skinny_promote(float *sum, const uint32_t (&v)[N], const float4 *sa, float sb)
-{
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-        const float4 s = sa[i];
-        sum[4 * i + 0] = fmaf(__uint_as_float(v[4 * i + 0]), s.x * sb, sum[4 * i + 0]);
-        sum[4 * i + 1] = fmaf(__uint_as_float(v[4 * i + 1]), s.y * sb, sum[4 * i + 1]);
-        sum[4 * i + 2] = fmaf(__uint_as_float(v[4 * i + 2]), s.z * sb, sum[4 * i + 2]);
-        sum[4 * i + 3] = fmaf(__uint_as_float(v[4 * i + 3]), s.w * sb, sum[4 * i + 3]);
-    }
-}
-
-template <uint32_t NT, uint32_t STAGES>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNumThreads, 1)
+template <uint32_t REPL, uint32_t S, uint32_t STAGES>
+__global__ void __launch_bounds__(kF8SkinnyThreads, 1)
 gemm_e4m3_sm100_skinny(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                        const F8SkinnyParams f)
 {
-    using L = F8SkinnySmemLayout<NT, STAGES>;
-    static_assert(NT == 16 || NT == 32 || NT == 64 || NT == 128, "rows of A per launch");
-    constexpr uint32_t kBuffers = 4;
-    constexpr uint32_t kTmemCols = kBuffers * NT;  // 64 .. 512
-    constexpr uint32_t kIdesc = ptx::make_instr_desc_e4m3(kBlockM, NT);
-    constexpr uint32_t kHalf = NT / 2;
-    const GroupedParams &p = f.c;
+    using L = F8SkinnyLayout<REPL, S, STAGES>;
+    constexpr uint32_t kTmemCols = 512;
+    constexpr uint32_t kChunks = L::kWarpCols / 32;
+    const GemmParams &p = f.g;
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -83,21 +73,21 @@ gemm_e4m3_sm100_skinny(const __grid_constant__ CUtensorMap tma_a, const __grid_c
     auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };
     auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (STAGES + s); };
     auto acc_full_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + b); };
-    auto acc_empty_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + kBuffers + b); };
-    const uint32_t sums_full_bar = bar_base + 8u * (2 * STAGES + 2 * kBuffers);        // the peer's sums are here
-    const uint32_t sums_taken_bar = bar_base + 8u * (2 * STAGES + 2 * kBuffers + 1);   // the peer has read what this CTA sent
+    auto acc_empty_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + L::kBuffers + b); };
+    const uint32_t sums_full_bar = bar_base + 8u * (2 * STAGES + 2 * L::kBuffers);       // the other CTAs' sums are here
+    const uint32_t sums_taken_bar = bar_base + 8u * (2 * STAGES + 2 * L::kBuffers + 1);  // the others have read what this CTA sent
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + L::kTmemSlotOffset);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem_gen + L::kAbortOffset);
 
     const uint32_t warp = threadIdx.x >> 5;
     const uint32_t lane = threadIdx.x & 31u;
-    const uint32_t cta_rank = ptx::cluster_cta_rank();
-    const uint32_t pair = blockIdx.x >> 1;
-    const uint32_t num_pairs = gridDim.x >> 1;
+    const uint32_t rank = ptx::cluster_cta_rank();
+    const uint32_t cluster = blockIdx.x / S;
+    const uint32_t num_clusters = gridDim.x / S;
     const uint32_t all_kb = (p.k + kF8BlockK - 1) / kF8BlockK;
-    const uint32_t first_half = (all_kb + 1) / 2;
-    const uint32_t kb0 = cta_rank == 0 ? 0u : first_half;
-    const uint32_t num_kb = cta_rank == 0 ? first_half : all_kb - first_half;  // 0 in the second CTA if K is one block
+    const uint32_t per_cta = (all_kb + S - 1) / S;
+    const uint32_t kb0 = min(rank * per_cta, all_kb);
+    const uint32_t num_kb = min(per_cta, all_kb - kb0);  // may be 0 in the last CTAs
     const WaitCtl ctl{abort_flag, p.status, p.timeout_ns};
 
     if (threadIdx.x == 0) {
@@ -107,12 +97,12 @@ gemm_e4m3_sm100_skinny(const __grid_constant__ CUtensorMap tma_a, const __grid_c
             ptx::mbar_init(full_bar(s), 1);
             ptx::mbar_init(empty_bar(s), 1);
         }
-        for (uint32_t b = 0; b < kBuffers; ++b) {
+        for (uint32_t b = 0; b < L::kBuffers; ++b) {
             ptx::mbar_init(acc_full_bar(b), 1);
-            ptx::mbar_init(acc_empty_bar(b), kNumEpilogueWarps);
+            ptx::mbar_init(acc_empty_bar(b), L::kWarps);
         }
-        ptx::mbar_init(sums_full_bar, kNumEpilogueWarps);
-        ptx::mbar_init(sums_taken_bar, kNumEpilogueWarps);
+        ptx::mbar_init(sums_full_bar, (S - 1) * L::kWarps);
+        ptx::mbar_init(sums_taken_bar, (S - 1) * L::kWarps);
         *abort_flag = 0;
         ptx::fence_barrier_init();
     }
@@ -133,21 +123,23 @@ gemm_e4m3_sm100_skinny(const __grid_constant__ CUtensorMap tma_a, const __grid_c
 
     bool role_ok = true;
     if (warp == 0) {
-        // ------------------------------------------------------- TMA producer --
+        // --------------------------------------------------- TMA producer --
         if (lane == 0) {
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            const uint32_t bytes = f.tile_rows * kF8BlockK + L::kABytes;
-            for (uint32_t t = pair; ok && t < f.tiles; t += num_pairs) {
+            const uint32_t bytes = (f.bn + REPL * p.m) * kF8BlockK;
+            for (uint32_t t = cluster; ok && t < p.tiles_n; t += num_clusters) {
                 for (uint32_t kb = 0; kb < num_kb; ++kb) {
                     ok = wait_bounded(empty_bar(stage), phase ^ 1u, ctl, 1);
                     if (!ok)
                         break;
-                    const uint32_t sb = smem_base + stage * L::kStageBytes;
+                    const uint32_t sa = smem_base + stage * L::kStageBytes;
                     const int32_t kx = static_cast<int32_t>((kb0 + kb) * kF8BlockK);
                     ptx::mbar_arrive_expect_tx(full_bar(stage), bytes);
-                    ptx::tma_load_2d(sb, &tma_b, full_bar(stage), kx, static_cast<int32_t>(t * f.tile_rows));
-                    ptx::tma_load_2d(sb + L::kBBytes, &tma_a, full_bar(stage), kx, 0);
+                    ptx::tma_load_2d(sa + L::kABytes, &tma_b, full_bar(stage), kx, static_cast<int32_t>(t * f.bn));
+#pragma unroll
+                    for (uint32_t r = 0; r < REPL; ++r)
+                        ptx::tma_load_2d(sa + r * L::kRows * kF8BlockK, &tma_a, full_bar(stage), kx, 0);
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1u;
@@ -158,31 +150,32 @@ gemm_e4m3_sm100_skinny(const __grid_constant__ CUtensorMap tma_a, const __grid_c
         }
         __syncwarp();
     } else if (warp == 1) {
-        // -------------------------------------------------------- MMA issuer --
+        // ---------------------------------------------------- MMA issuer --
         if (lane == 0) {
             uint32_t stage = 0, phase = 0;
             uint32_t acc = 0, acc_phase = 0;
             bool ok = true;
-            for (uint32_t t = pair; ok && t < f.tiles; t += num_pairs) {
+            const uint32_t idesc = ptx::make_instr_desc_e4m3(kBlockM, f.bn);
+            for (uint32_t t = cluster; ok && t < p.tiles_n; t += num_clusters) {
                 for (uint32_t kb = 0; kb < num_kb; ++kb) {
                     ok = wait_bounded(full_bar(stage), phase, ctl, 2) &&
                          wait_bounded(acc_empty_bar(acc), acc_phase ^ 1u, ctl, 2);
                     if (!ok)
                         break;
                     ptx::tcgen05_fence_after();
-                    const uint32_t sb = smem_base + stage * L::kStageBytes;
-                    const uint64_t db = ptx::make_smem_desc_sw128(sb);
-                    const uint64_t da = ptx::make_smem_desc_sw128(sb + L::kBBytes);
+                    const uint32_t sa = smem_base + stage * L::kStageBytes;
+                    const uint64_t da = ptx::make_smem_desc_sw128(sa);
+                    const uint64_t db = ptx::make_smem_desc_sw128(sa + L::kABytes);
 #pragma unroll
                     for (uint32_t k = 0; k < kF8BlockK / kF8UmmaK; ++k)
-                        ptx::mma_f8_1cta(tmem_base + acc * NT, db + 2u * k, da + 2u * k, kIdesc, k != 0u ? 1u : 0u);
+                        ptx::mma_f8_1cta(tmem_base + acc * L::kTileCols, da + 2u * k, db + 2u * k, idesc, k != 0u ? 1u : 0u);
                     ptx::mma_commit_1cta(acc_full_bar(acc));
                     ptx::mma_commit_1cta(empty_bar(stage));
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1u;
                     }
-                    if (++acc == kBuffers) {
+                    if (++acc == L::kBuffers) {
                         acc = 0;
                         acc_phase ^= 1u;
                     }
@@ -193,144 +186,177 @@ gemm_e4m3_sm100_skinny(const __grid_constant__ CUtensorMap tma_a, const __grid_c
         __syncwarp();
     } else {
         // ---------------------------------------------- promotion and epilogue --
-        const uint32_t quarter = warp & 3u;
-        const uint32_t row = quarter * 32u + lane;  // of the tile's rows of B
-        const uint32_t tid = threadIdx.x - 64u;     // 0 .. 127
-        float *scale_a = reinterpret_cast<float *>(smem_gen + L::kScaleAOffset);  // [k-block][row of A]
-        float *scale_b = reinterpret_cast<float *>(smem_gen + L::kScaleBOffset);  // [tile parity][scale block][k-block]
-        float *sums_in = reinterpret_cast<float *>(smem_gen + L::kExchangeOffset);  // [row of A][128]
-        const uint32_t sums_out = ptx::mapa_shared(smem_base + L::kExchangeOffset, cta_rank ^ 1u);
-        const uint32_t peer_full = ptx::mapa_shared(sums_full_bar, cta_rank ^ 1u);
-        const uint32_t peer_taken = ptx::mapa_shared(sums_taken_bar, cta_rank ^ 1u);
-        const uint32_t last_block = (p.n - 1) / 128u;
-        // thread i < 2 * 64 fetches scale block i / 64, k-block i % 64 of a tile
-        auto fetch_scale_b = [&](uint32_t t) {
-            const uint32_t kb = tid & (kF8SkinnyMaxKb - 1);
-            const uint32_t block = min(t * f.tile_rows / 128u + tid / kF8SkinnyMaxKb, last_block);
-            return t < f.tiles && kb < num_kb ? __ldg(f.sb + static_cast<uint64_t>(block) * f.ld_sb + kb0 + kb) : 0.0f;
-        };
-        float next_b = fetch_scale_b(pair);
-        // eight loads in flight per thread: one after the other they cost 16 latencies for 128 rows and 16 k-blocks
-        for (uint32_t base = tid; base < num_kb * NT; base += 8u * 128u) {
-            float v[8];
-#pragma unroll
-            for (uint32_t u = 0; u < 8; ++u) {
-                const uint32_t i = base + u * 128u, m = i / num_kb, kb = i - m * num_kb;
-                v[u] = m < p.rows && i < num_kb * NT ? __ldg(f.sa + static_cast<uint64_t>(m) * f.ld_sa + kb0 + kb) : 0.0f;
-            }
-#pragma unroll
-            for (uint32_t u = 0; u < 8; ++u) {
-                const uint32_t i = base + u * 128u, m = i / num_kb, kb = i - m * num_kb;
-                if (i < num_kb * NT)
-                    scale_a[kb * NT + m] = v[u];
-            }
-        }
+        const uint32_t quarter = warp & 3u, w = warp - 2u;
+        // this warp's rows of A and columns of the tile
+        const uint32_t row0 = REPL == 4 ? 0u : (REPL == 2 ? (quarter & 1u) * 32u : quarter * 32u);
+        const uint32_t col0 = (REPL == 4 ? quarter * 64u : (REPL == 2 ? (quarter >> 1) * 128u : 0u)) + (w >> 2) * L::kWarpCols;
+        const uint32_t lane_addr = tmem_base + ((quarter * 32u) << 16) + col0;
+        const float *sa = f.sa + static_cast<uint64_t>(min(row0 + lane, p.m - 1)) * f.ld_sa + kb0;
+        const uint32_t last_block = (p.n - 1) / 128u, last_kb = num_kb > 0 ? num_kb - 1 : 0u;
+        const uint32_t exchange = smem_base + L::kExchangeOffset;
         uint32_t acc = 0, acc_phase = 0, parity = 0;
         bool ok = true;
-        for (uint32_t t = pair; ok && t < f.tiles; t += num_pairs, parity ^= 1u) {
-            const uint32_t n0 = t * f.tile_rows;
-            float *my_b = scale_b + parity * 2 * kF8SkinnyMaxKb;
-            my_b[tid] = next_b;
-            asm volatile("bar.sync 1, 128;" ::: "memory");  // the scales of this tile (and of A) are in place
-            next_b = fetch_scale_b(t + num_pairs);
-            const float *lane_b = my_b + ((n0 + row) / 128u - n0 / 128u) * kF8SkinnyMaxKb;
-            float sum[NT];
+        for (uint32_t t = cluster; ok && t < p.tiles_n; t += num_clusters, parity ^= 1u) {
+            const uint32_t n0 = t * f.bn;
+            // the (at most two) scale blocks of this warp's columns; bit c of `second`: chunk c lies in the second
+            const uint32_t block0 = (n0 + col0) / 128u;
+            uint32_t second = 0;
 #pragma unroll
-            for (uint32_t i = 0; i < NT; ++i)
-                sum[i] = 0.0f;
+            for (uint32_t c = 0; c < kChunks; ++c)
+                second |= (n0 + col0 + 32u * c) / 128u != block0 ? 1u << c : 0u;
+            const float *sb0 = f.sb + static_cast<uint64_t>(min(block0, last_block)) * f.ld_sb + kb0;
+            const float *sb1 = f.sb + static_cast<uint64_t>(min(block0 + 1u, last_block)) * f.ld_sb + kb0;
+            const uint32_t cols = f.bn > col0 ? min(L::kWarpCols, f.bn - col0) : 0u;  // of this warp in the tile
+            uint64_t sum[L::kWarpCols / 2];
+#pragma unroll
+            for (uint32_t i = 0; i < L::kWarpCols / 2; ++i)
+                sum[i] = 0ull;
+            float a0 = 0.0f, a1 = 0.0f, x0 = 0.0f, x1 = 0.0f, y0 = 0.0f, y1 = 0.0f;
+            if (num_kb > 0) {  // the scales of the next two k-blocks are on their way behind this one's work
+                const uint32_t one = min(1u, last_kb);
+                a0 = ptx::ld_f32_nc(sa), x0 = ptx::ld_f32_nc(sb0), y0 = ptx::ld_f32_nc(sb1);
+                a1 = ptx::ld_f32_nc(sa + one), x1 = ptx::ld_f32_nc(sb0 + one), y1 = ptx::ld_f32_nc(sb1 + one);
+            }
             for (uint32_t kb = 0; kb < num_kb; ++kb) {
+                const float s0 = a0 * x0, s1 = a0 * y0;
+                const uint32_t ahead = min(kb + 2, last_kb);
+                a0 = a1, x0 = x1, y0 = y1;
+                a1 = ptx::ld_f32_nc(sa + ahead), x1 = ptx::ld_f32_nc(sb0 + ahead), y1 = ptx::ld_f32_nc(sb1 + ahead);
                 ok = wait_bounded(acc_full_bar(acc), acc_phase, ctl, 3);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok)
                     break;
                 ptx::tcgen05_fence_after();
-                const uint32_t taddr = tmem_base + acc * NT + ((quarter * 32u) << 16);
-                const float sb = lane_b[kb];
-                const float4 *sa = reinterpret_cast<const float4 *>(scale_a + kb * NT);
-                auto hand_back = [&]() {
-                    ptx::tcgen05_fence_before();
-                    __syncwarp();
-                    if (lane == 0)
-                        ptx::mbar_arrive(acc_empty_bar(acc));
+                const uint32_t taddr = lane_addr + acc * L::kTileCols;
+                auto scale = [&](uint32_t c) {
+                    const uint32_t bits = __float_as_uint((second >> c) & 1u ? s1 : s0);
+                    return ptx::pack_f32x2(bits, bits);
                 };
-                if constexpr (NT == 16) {
-                    uint32_t v[16];
-                    ptx::tmem_ld_32x32b_x16(taddr, v);
-                    ptx::tmem_ld_wait();
-                    hand_back();
-                    f8_skinny_promote(sum, v, sa, sb);
-                } else {
-                    // at most two loads of 32 columns in flight, the buffer back as soon as the last is in registers
-                    uint32_t v0[32], v1[32];
+                uint32_t v0[32], v1[32];
+                if (cols > 0) {
                     ptx::tmem_ld_32x32b_x32(taddr, v0);
-                    if constexpr (NT >= 64)
+                    if (kChunks == 2 && cols > 32)
                         ptx::tmem_ld_32x32b_x32(taddr + 32u, v1);
                     ptx::tmem_ld_wait();
-                    if constexpr (NT == 128) {
-                        f8_skinny_promote(sum, v0, sa, sb);
-                        ptx::tmem_ld_32x32b_x32(taddr + 64u, v0);
-                        f8_skinny_promote(sum + 32, v1, sa + 8, sb);
-                        ptx::tmem_ld_32x32b_x32(taddr + 96u, v1);
-                        ptx::tmem_ld_wait();
-                    }
-                    hand_back();
-                    constexpr uint32_t kDone = NT == 128 ? 64u : 0u;
-                    f8_skinny_promote(sum + kDone, v0, sa + kDone / 4, sb);
-                    if constexpr (NT >= 64)
-                        f8_skinny_promote(sum + kDone + 32, v1, sa + kDone / 4 + 8, sb);
                 }
-                if (++acc == kBuffers) {
+                // all columns are in registers: the buffer goes back
+                ptx::tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    ptx::mbar_arrive(acc_empty_bar(acc));
+                if (cols > 0) {
+                    f8_promote<L::kWarpCols / 2>(sum, 0, v0, scale(0));
+                    if constexpr (kChunks == 2)
+                        if (cols > 32)
+                            f8_promote<L::kWarpCols / 2>(sum, 16, v1, scale(1));
+                }
+                if (++acc == L::kBuffers) {
                     acc = 0;
                     acc_phase ^= 1u;
                 }
             }
             if (!ok)
                 break;
-            // The sums of the other CTA's half of the rows of A go there; the exchange buffer has been read since the last tile.
+            // Every CTA finishes its share of each warp's columns: the others' sums of it come here, what this CTA has of theirs
+            // goes there, once they have read what it sent for its tile before.
             ok = wait_bounded<true>(sums_taken_bar, parity ^ 1u, ctl, 7);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok)
                 break;
 #pragma unroll
-            for (uint32_t i = 0; i < kHalf; ++i)
-                ptx::st_shared_cluster_u32(sums_out + (i * 128u + row) * 4u,
-                                           __float_as_uint(cta_rank == 0 ? sum[kHalf + i] : sum[i]));
+            for (uint32_t d = 0; d < S; ++d) {
+                if (d == rank)
+                    continue;
+                // the slot of this CTA among the others of CTA d
+                const uint32_t slot = rank - (rank > d ? 1u : 0u);
+                const uint32_t to = ptx::mapa_shared(exchange + slot * L::kPartBytes + w * (L::kShare * 128u) + lane * 16u, d);
+#pragma unroll
+                for (uint32_t i = 0; i < L::kShare / 4; ++i) {
+                    uint32_t q[4];
+                    ptx::unpack_f32x2(sum[d * (L::kShare / 2) + 2 * i], q[0], q[1]);
+                    ptx::unpack_f32x2(sum[d * (L::kShare / 2) + 2 * i + 1], q[2], q[3]);
+                    ptx::st_shared_cluster_v4(to + i * 512u, q[0], q[1], q[2], q[3]);
+                }
+            }
             __syncwarp();
-            if (lane == 0)
-                ptx::mbar_arrive_cluster_addr(peer_full);
+            // one lane per CTA: each release at cluster scope waits for what was stored, one after the other they would add up
+            if (lane < S && lane != rank)
+                ptx::mbar_arrive_cluster_addr(ptx::mapa_shared(sums_full_bar, lane));
+            float mine[L::kShare];
+#pragma unroll
+            for (uint32_t d = 0; d < S; ++d)
+                if (d == rank) {
+#pragma unroll
+                    for (uint32_t i = 0; i < L::kShare / 2; ++i) {
+                        uint32_t lo, hi;
+                        ptx::unpack_f32x2(sum[d * (L::kShare / 2) + i], lo, hi);
+                        mine[2 * i] = __uint_as_float(lo), mine[2 * i + 1] = __uint_as_float(hi);
+                    }
+                }
             ok = wait_bounded<true>(sums_full_bar, parity, ctl, 7);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok)
                 break;
-            uint32_t out[kHalf < 32 ? 32 : kHalf] = {};
+            // in the order of the parts of K, whoever adds
+            const uint8_t *from = smem_gen + L::kExchangeOffset + w * (L::kShare * 128u) + lane * 16u;
+            uint32_t out[L::kShare];
 #pragma unroll
-            for (uint32_t i = 0; i < kHalf; ++i) {
-                const float mine = cta_rank == 0 ? sum[i] : sum[kHalf + i], theirs = sums_in[i * 128u + row];
-                // k order: the first CTA's blocks come first
-                out[i] = __float_as_uint(cta_rank == 0 ? mine + theirs : theirs + mine);
+            for (uint32_t i = 0; i < L::kShare / 4; ++i) {
+                float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (uint32_t d = 0; d < S; ++d) {
+                    float4 part = make_float4(mine[4 * i], mine[4 * i + 1], mine[4 * i + 2], mine[4 * i + 3]);
+                    if (d != rank)
+                        part = *reinterpret_cast<const float4 *>(from + (d - (d > rank ? 1u : 0u)) * L::kPartBytes + i * 512u);
+                    total.x += part.x, total.y += part.y, total.z += part.z, total.w += part.w;
+                }
+                out[4 * i] = __float_as_uint(total.x), out[4 * i + 1] = __float_as_uint(total.y);
+                out[4 * i + 2] = __float_as_uint(total.z), out[4 * i + 3] = __float_as_uint(total.w);
             }
             __syncwarp();
-            if (lane == 0)
-                ptx::mbar_arrive_cluster_addr(peer_taken);
-            GroupedParams q = p;
-            q.n = min(p.n, n0 + f.tile_rows);
-            const uint32_t m0 = cta_rank * kHalf;
+            // ---- store this CTA's share: kShare columns of 32 rows
+            const uint32_t end = min(p.n, n0 + f.bn), out_col = n0 + col0 + rank * L::kShare;
+            if constexpr (L::kShare >= 32) {
+                GemmParams q = p;
+                q.n = end;
+                uint8_t *staging = smem_gen + L::kExchangeOffset + w * (L::kShare * 128u);  // what came has been read
 #pragma unroll
-            for (uint32_t c = 0; c < kHalf; c += 32) {
-                if (m0 + c < p.rows && n0 + quarter * 32u < q.n) {
+                for (uint32_t c = 0; c < L::kShare; c += 32) {
                     uint32_t v[32];
 #pragma unroll
                     for (uint32_t i = 0; i < 32; ++i)
                         v[i] = out[c + i];
-                    store_transposed_chunk(q, m0 + c, min(min(32u, kHalf), p.rows - m0 - c), n0 + row, lane, v);
+                    store_chunk(q, staging, row0, out_col + c, lane, v);
+                    __syncwarp();
                 }
-                __syncwarp();
+            } else if (row0 + lane < p.m) {
+                __nv_bfloat16 *dst = p.c + static_cast<uint64_t>(row0 + lane) * p.ldc + out_col;
+#pragma unroll
+                for (uint32_t i = 0; i < L::kShare; i += 8) {
+                    if (p.c_vec_ok && out_col + i + 8 <= end) {
+                        *reinterpret_cast<uint4 *>(dst + i) =
+                            make_uint4(ptx::pack_bf16x2(out[i], out[i + 1]), ptx::pack_bf16x2(out[i + 2], out[i + 3]),
+                                       ptx::pack_bf16x2(out[i + 4], out[i + 5]), ptx::pack_bf16x2(out[i + 6], out[i + 7]));
+                    } else {
+#pragma unroll
+                        for (uint32_t j = 0; j < 8; ++j)
+                            if (out_col + i + j < end)
+                                dst[i + j] = __float2bfloat16_rn(__uint_as_float(out[i + j]));
+                    }
+                }
             }
+            __syncwarp();
+            if (lane < S && lane != rank)
+                ptx::mbar_arrive_cluster_addr(ptx::mapa_shared(sums_taken_bar, lane));
         }
         role_ok = ok;
     }
-    if (!role_ok)
-        ptx::st_shared_cluster_u32(ptx::mapa_shared(ptx::smem_u32(const_cast<int *>(abort_flag)), cta_rank ^ 1u), 1u);
+    if (!role_ok) {
+        // tell the other CTAs, so that their roles stop waiting on us
+        for (uint32_t d = 0; d < S; ++d)
+            if (d != rank)
+                ptx::st_shared_cluster_u32(ptx::mapa_shared(ptx::smem_u32(const_cast<int *>(abort_flag)), d), 1u);
+    }
 
     // ---------------------------------------------------------------- teardown --
     __syncwarp();

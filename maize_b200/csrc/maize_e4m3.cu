@@ -24,53 +24,80 @@ maize_status_t byte_map(maize_ctx_t *ctx, CUtensorMap *map, const void *base, ui
                              static_cast<CUtensorMapL2promotion>(ctx->tma_promotion));
 }
 
-template <uint32_t NT, uint32_t STAGES>
-maize_status_t launch_skinny(maize_ctx_t *ctx, int slot, const CUtensorMap &ta, const CUtensorMap &tb,
-                             const maize::F8SkinnyParams &f, uint32_t grid, cudaStream_t stream)
+template <uint32_t REPL, uint32_t S, uint32_t STAGES>
+maize_status_t launch_skinny(maize_ctx_t *ctx, int slot, uint32_t clusters, const CUtensorMap &ta, const CUtensorMap &tb,
+                             const maize::F8SkinnyParams &f, cudaStream_t stream)
 {
-    return maize::launch(ctx, slot, maize::gemm_e4m3_sm100_skinny<NT, STAGES>, grid, maize::kNumThreads,
-                         maize::F8SkinnySmemLayout<NT, STAGES>::kDynamicBytes, stream, ta, tb, f);
+    using L = maize::F8SkinnyLayout<REPL, S, STAGES>;
+    const uint32_t grid = (f.g.tiles_n < clusters ? f.g.tiles_n : clusters) * S;
+    return maize::launch_clusters(ctx, slot, maize::gemm_e4m3_sm100_skinny<REPL, S, STAGES>, grid, S, maize::kF8SkinnyThreads,
+                                  L::kDynamicBytes, stream, ta, tb, f);
 }
 
-// M <= 128: tiles of up to 128 rows of B, as tall as fills whole rounds of the CTA pairs (never below 32 rows: a shorter
-// tile reads the rows of A more often than it gains).
+// How the tiles of a skinny product are cut: `parts` CTAs share a tile's K, `bn` rows of B per tile.
+struct SkinnyPlan {
+    uint32_t parts, clusters, bn;
+    double cost;  // microseconds, for comparison only
+};
+
+// One round of clusters covers clusters * widest rows of B; the tiles are as wide as fills whole rounds.  A k-block costs a
+// CTA 0.34 us (four MMAs of 128 rows and their hand-over) or its bytes at 80 GB/s per SM, measured; joining four parts about
+// 0.8 us more than joining two.  16 x 512 x 8192: 9.8 us in four parts, 14.7 in two; 5 x 9001 x 2048: 12.8 and 7.8.
+SkinnyPlan skinny_plan(uint32_t ctas, uint32_t parts, uint32_t widest, uint32_t rows_loaded, uint32_t n, uint32_t kblocks)
+{
+    SkinnyPlan q;
+    q.parts = parts;
+    // clusters of four fit only within a GPC: of the 37 that 148 SMs would make, 32 are counted on
+    q.clusters = parts == 2 ? ctas / 2 : ctas * 32 / 148;
+    if (q.clusters == 0)
+        q.clusters = 1;
+    const uint64_t rounds = (uint64_t(n) + uint64_t(q.clusters) * widest - 1) / (uint64_t(q.clusters) * widest);
+    q.bn = static_cast<uint32_t>((uint64_t(n) + q.clusters * rounds - 1) / (q.clusters * rounds) + 31) / 32 * 32;
+    const double bytes = (q.bn + rows_loaded) * 128.0, block = bytes / 80e3 > 0.34 ? bytes / 80e3 : 0.34;
+    q.cost = double(rounds) * ((kblocks + parts - 1) / parts) * block + (parts == 2 ? 0.0 : 0.8);
+    return q;
+}
+
 maize_status_t skinny(maize_ctx_t *ctx, const void *a, uint64_t lda, const float *sa, uint64_t ld_sa, const void *b, uint64_t ldb,
                       const float *sb, uint64_t ld_sb, void *c, uint64_t ldc, uint32_t m, uint32_t n, uint32_t k, cudaStream_t stream)
 {
-    const uint32_t nt = m <= 16 ? 16 : (m <= 32 ? 32 : (m <= 64 ? 64 : 128));
-    const uint64_t pairs = maize::persistent_grid(ctx, 0xffffffffull, 2) / 2;
-    const uint64_t rounds = (uint64_t(n) + pairs * 128 - 1) / (pairs * 128);
-    uint32_t rows = static_cast<uint32_t>((uint64_t(n) + pairs * rounds - 1) / (pairs * rounds));
-    rows = (rows + 7) / 8 * 8;
-    if (rows < 32)
-        rows = 32;
+    const uint32_t copies = m <= 32 ? 4 : (m <= 64 ? 2 : 1), widest = copies == 1 ? 128 : 256;
+    const uint32_t kblocks = (k + 127) / 128, ctas = maize::persistent_grid(ctx, 0xffffffffull, 1);
+    SkinnyPlan plan = skinny_plan(ctas, 2, widest, copies * m, n, kblocks);
+    const SkinnyPlan four = skinny_plan(ctas, 4, widest, copies * m, n, kblocks);
+    if (four.cost < plan.cost)
+        plan = four;
+    const uint32_t bn = plan.bn;
     maize::F8SkinnyParams f = {};
-    f.c.c = static_cast<__nv_bfloat16 *>(c);
-    f.c.ldc = ldc;
-    f.c.rows = m;
-    f.c.n = n;
-    f.c.k = k;
-    f.c.c_pair_ok = (ldc % 2 == 0 && aligned(c, 4)) ? 1u : 0u;
-    f.c.pdl = ctx->pdl;
-    f.c.status = ctx->d_status;
-    f.c.timeout_ns = ctx->timeout_ns;
+    f.g.c = static_cast<__nv_bfloat16 *>(c);
+    f.g.ldc = ldc;
+    f.g.m = m;
+    f.g.n = n;
+    f.g.k = k;
+    f.g.tiles_n = (n + bn - 1) / bn;
+    f.g.c_vec_ok = (ldc % 8 == 0 && aligned(c, 16)) ? 1u : 0u;
+    f.g.pdl = ctx->pdl;
+    f.g.status = ctx->d_status;
+    f.g.timeout_ns = ctx->timeout_ns;
     f.sa = sa;
     f.sb = sb;
     f.ld_sa = ld_sa;
     f.ld_sb = ld_sb;
-    f.tile_rows = rows;
-    f.tiles = (n + rows - 1) / rows;
+    f.bn = bn;
     CUtensorMap ta, tb;
     maize_status_t st;
-    if ((st = byte_map(ctx, &ta, a, m, k, lda, nt)) != MAIZE_OK || (st = byte_map(ctx, &tb, b, n, k, ldb, rows)) != MAIZE_OK)
+    if ((st = byte_map(ctx, &ta, a, m, k, lda, m)) != MAIZE_OK || (st = byte_map(ctx, &tb, b, n, k, ldb, bn)) != MAIZE_OK)
         return st;
-    const uint32_t grid = maize::persistent_grid(ctx, f.tiles, 2);
-    switch (nt) {
-    case 16: return launch_skinny<16, 11>(ctx, maize::kAttrE4m3Skinny, ta, tb, f, grid, stream);
-    case 32: return launch_skinny<32, 10>(ctx, maize::kAttrE4m3Skinny + 1, ta, tb, f, grid, stream);
-    case 64: return launch_skinny<64, 7>(ctx, maize::kAttrE4m3Skinny + 2, ta, tb, f, grid, stream);
-    default: return launch_skinny<128, 4>(ctx, maize::kAttrE4m3Skinny + 3, ta, tb, f, grid, stream);
-    }
+    const int slot = maize::kAttrE4m3Skinny;
+    const bool two = plan.parts == 2;
+    if (copies == 1)
+        return two ? launch_skinny<1, 2, 6>(ctx, slot, plan.clusters, ta, tb, f, stream)
+                   : launch_skinny<1, 4, 5>(ctx, slot + 1, plan.clusters, ta, tb, f, stream);
+    if (copies == 2)
+        return two ? launch_skinny<2, 2, 4>(ctx, slot + 2, plan.clusters, ta, tb, f, stream)
+                   : launch_skinny<2, 4, 3>(ctx, slot + 3, plan.clusters, ta, tb, f, stream);
+    return two ? launch_skinny<4, 2, 4>(ctx, slot + 4, plan.clusters, ta, tb, f, stream)
+               : launch_skinny<4, 4, 4>(ctx, slot + 5, plan.clusters, ta, tb, f, stream);
 }
 
 }  // namespace
@@ -169,7 +196,7 @@ maize_status_t maize_gemm_e4m3(maize_ctx_t *ctx, const void *a, uint64_t lda, co
         return fail(ctx, MAIZE_ERR_UNSUPPORTED, "A and B must be 16-byte aligned");
     if (lda >= (1ull << 40) || ldb >= (1ull << 40))
         return fail(ctx, MAIZE_ERR_UNSUPPORTED, "row pitch beyond the TMA limit of 2^40 bytes");
-    if (m <= 128 && kblocks <= 2 * maize::kF8SkinnyMaxKb)
+    if (m <= 128)
         return skinny(ctx, a, lda, static_cast<const float *>(a_scales), ld_a_scales, b, ldb, static_cast<const float *>(b_scales),
                       ld_b_scales, c, ldc, m, n, k, stream);
     CUtensorMap ta, tb, tc;

@@ -9,7 +9,7 @@ namespace maize {
 constexpr uint32_t kMaxDim = 0x7fffff00u;  // sizes are TMA coordinates (int32); room for a tile past the end
 
 // ctx->attr_experts slots: kernels whose shared-memory limit has been raised on the context's device
-enum { kAttrGrouped = 0, kAttrGroupedKn = 1, kAttrWgrad = 2, kAttrE4m3 = 3, kAttrE4m3Skinny = 4 /* .. 7 */ };
+enum { kAttrGrouped = 0, kAttrGroupedKn = 1, kAttrWgrad = 2, kAttrE4m3 = 3, kAttrE4m3Skinny = 4 /* .. 9 */ };
 
 inline bool aligned(const void *p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
@@ -55,10 +55,11 @@ inline maize_status_t stack_map(maize_ctx_t *ctx, CUtensorMap *map, const void *
     return encode_map(ctx, map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, 3, dims, strides, box, promotion);
 }
 
-// `attr_slot` < 0: a kernel that needs no more shared memory than any may have.
+// Kernels launched in clusters of `cluster` CTAs (0: as the kernel itself says).  `attr_slot` < 0: a kernel that needs no
+// more shared memory than any may have.
 template <typename Kernel, typename... Args>
-maize_status_t launch(maize_ctx_t *ctx, int attr_slot, Kernel kernel, uint32_t grid, uint32_t threads, uint32_t smem,
-                      cudaStream_t stream, const Args &...args)
+maize_status_t launch_clusters(maize_ctx_t *ctx, int attr_slot, Kernel kernel, uint32_t grid, uint32_t cluster, uint32_t threads,
+                               uint32_t smem, cudaStream_t stream, const Args &...args)
 {
     if (attr_slot >= 0 && !ctx->attr_experts[attr_slot]) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -71,16 +72,30 @@ maize_status_t launch(maize_ctx_t *ctx, int attr_slot, Kernel kernel, uint32_t g
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
+    if (ctx->pdl) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster != 0) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = cluster;
+        attr[cfg.numAttrs].val.clusterDim.y = 1;
+        attr[cfg.numAttrs++].val.clusterDim.z = 1;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = ctx->pdl ? 1 : 0;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e != cudaSuccess)
         return fail_cuda(ctx, "kernel launch", e);
     ctx->launches += 1;
     return MAIZE_OK;
+}
+
+template <typename Kernel, typename... Args>
+maize_status_t launch(maize_ctx_t *ctx, int attr_slot, Kernel kernel, uint32_t grid, uint32_t threads, uint32_t smem,
+                      cudaStream_t stream, const Args &...args)
+{
+    return launch_clusters(ctx, attr_slot, kernel, grid, 0, threads, smem, stream, args...);
 }
 
 // CTAs that may run at a time, a multiple of `unit` (the cluster size), at most what `tiles` clusters need.
