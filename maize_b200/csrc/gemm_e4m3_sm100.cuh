@@ -49,55 +49,98 @@ struct F8SmemLayout {
     static constexpr uint32_t kDynamicBytes = kUsedBytes + 1024;
     static_assert(kDynamicBytes <= 232448, "exceeds 227 KiB of shared memory per CTA");
     static_assert(kDynamicBytes > 116224, "two CTAs could share an SM and contend for TMEM");
-    static_assert(kStageWarpBytes <= kTmaStoreBufBytes, "the ragged epilogue's staging is carved out of the TMA one");
 };
 
-// Writes this warp's 32 rows x 128 columns of C, held as 128 fp32 per lane (lane = row).
-__device__ __forceinline__ void f8_store(const GemmParams &p, const CUtensorMap *tma_c, uint8_t *stage_gen,
-                                         uint32_t stage_u32, uint32_t lane, uint32_t row0, uint32_t col0,
-                                         const uint64_t (&acc)[64])
+// Stores 32 rows x 64 columns of C that lie in `stage` as 128-byte rows, 16-byte chunk j of row r at chunk j ^ (r & 7), to
+// rows of any alignment: a lane stores 4 bytes, so a row leaves as one run of 128.  Where a row starts between two words
+// the lanes pass on a half, and the ends of the run are 2-byte stores.  (2-byte stores throughout: 4111 x 3967 x 4112 in 125 us
+// instead of 88; with rows for TMA 75.)
+__device__ __forceinline__ void f8_store_rows(const GemmParams &p, uint32_t stage_u32, uint32_t lane, uint32_t row0, uint32_t col0)
+{
+    const uint32_t rows = min(32u, p.m - row0);
+    const uint32_t left = p.n - col0;  // columns there are
+    const uint32_t chunk = lane >> 2, word = (lane & 3u) * 4u;
+    __nv_bfloat16 *dst = p.c + static_cast<uint64_t>(row0) * p.ldc + col0;
+    if (rows == 32u && left >= 64u) {
+        // every row the same way, but for whether it starts between two words: with an odd pitch every other one does
+        const bool first = (reinterpret_cast<uintptr_t>(dst) & 2u) != 0u, odd_pitch = (p.ldc & 1u) != 0u;
+#pragma unroll 1
+        for (uint32_t r0 = 0; r0 < 32; r0 += 8) {
+            uint32_t v[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+                v[i] = ptx::ld_shared_u32(stage_u32 + (r0 + i) * 128u + ((chunk ^ i) << 4) + word);
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                if (first != (odd_pitch && (i & 1u) != 0u)) {
+                    const uint32_t before = __shfl_up_sync(0xffffffffu, v[i], 1);
+                    if (lane != 0u)
+                        *reinterpret_cast<uint32_t *>(dst + 2u * lane - 1u) = __funnelshift_l(before, v[i], 16);
+                    else
+                        *reinterpret_cast<uint16_t *>(dst) = static_cast<uint16_t>(v[i]);
+                    if (lane == 31u)
+                        *reinterpret_cast<uint16_t *>(dst + 63) = static_cast<uint16_t>(v[i] >> 16);
+                } else {
+                    *reinterpret_cast<uint32_t *>(dst + 2u * lane) = v[i];
+                }
+                dst += p.ldc;
+            }
+        }
+        __syncwarp();
+        return;
+    }
+#pragma unroll 1
+    for (uint32_t r = 0; r < rows; ++r) {
+        // at the edges of C: two columns per lane, each by itself
+        const uint32_t mine = ptx::ld_shared_u32(stage_u32 + r * 128u + ((chunk ^ (r & 7u)) << 4) + word);
+        if (2u * lane < left)
+            *reinterpret_cast<uint16_t *>(dst + 2u * lane) = static_cast<uint16_t>(mine);
+        if (2u * lane + 1u < left)
+            *reinterpret_cast<uint16_t *>(dst + 2u * lane + 1u) = static_cast<uint16_t>(mine >> 16);
+        dst += p.ldc;
+    }
+    __syncwarp();
+}
+
+// Writes this warp's 32 rows x 128 columns of C, held as 128 fp32 per lane (lane = row): through the warp's staging buffer
+// and TMA stores, or f8_store_rows where C's rows are not for TMA.
+__device__ __forceinline__ void f8_store(const GemmParams &p, const CUtensorMap *tma_c, uint32_t stage_u32, uint32_t lane,
+                                         uint32_t row0, uint32_t col0, const uint64_t (&acc)[64])
 {
     if (row0 >= p.m)
         return;
-    if (p.c_tma_ok) {
 #pragma unroll
-        for (uint32_t g = 0; g < 2; ++g) {
-            const uint32_t col = col0 + g * 64u;
-            if (col < p.n) {
-                if (lane == 0)
-                    ptx::bulk_wait_group_read<0>();  // the warp's one staging buffer has been read
-                __syncwarp();
-                const uint32_t row = stage_u32 + lane * 128u;
-                const uint32_t sw = lane & 7u;
+    for (uint32_t g = 0; g < 2; ++g) {
+        const uint32_t col = col0 + g * 64u;
+        if (col < p.n) {
+            if (p.c_tma_ok && lane == 0)
+                ptx::bulk_wait_group_read<0>();  // the warp's one staging buffer has been read
+            __syncwarp();
+            const uint32_t row = stage_u32 + lane * 128u;
+            const uint32_t sw = lane & 7u;
 #pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) {
-                    uint32_t w[4];
+            for (uint32_t j = 0; j < 8; ++j) {
+                uint32_t w[4];
 #pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-                        uint32_t lo, hi;
-                        ptx::unpack_f32x2(acc[g * 32 + 4 * j + i], lo, hi);
-                        w[i] = ptx::pack_bf16x2(lo, hi);
-                    }
-                    ptx::st_shared_v4(row + ((j ^ sw) << 4), w[0], w[1], w[2], w[3]);
+                for (uint32_t i = 0; i < 4; ++i) {
+                    uint32_t lo, hi;
+                    ptx::unpack_f32x2(acc[g * 32 + 4 * j + i], lo, hi);
+                    w[i] = ptx::pack_bf16x2(lo, hi);
                 }
+                ptx::st_shared_v4(row + ((j ^ sw) << 4), w[0], w[1], w[2], w[3]);
+            }
+            if (p.c_tma_ok) {
                 ptx::fence_proxy_async_shared();
                 __syncwarp();
                 if (lane == 0) {
                     ptx::tma_store_2d(tma_c, stage_u32, static_cast<int32_t>(col), static_cast<int32_t>(row0));
                     ptx::bulk_commit_group();
                 }
+            } else {
+                __syncwarp();
+                f8_store_rows(p, stage_u32, lane, row0, col);
             }
         }
-        return;
-    }
-#pragma unroll
-    for (uint32_t g = 0; g < 4; ++g) {
-        uint32_t v[32];
-#pragma unroll
-        for (uint32_t i = 0; i < 16; ++i)
-            ptx::unpack_f32x2(acc[g * 16 + i], v[2 * i], v[2 * i + 1]);
-        store_chunk(p, stage_gen, row0, col0 + g * 32u, lane, v);
-        __syncwarp();
     }
 }
 
@@ -245,7 +288,6 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
         // ---------------------------------------------- promotion and epilogue --
         const uint32_t quarter = warp & 3u;
         const uint32_t half = (warp - kF8ControlWarps) >> 2;
-        uint8_t *stage_gen = smem_gen + L::kStagingOffset + (warp - kF8ControlWarps) * kTmaStoreBufBytes;
         const uint32_t stage_u32 = smem_base + L::kStagingOffset + (warp - kF8ControlWarps) * kTmaStoreBufBytes;
         const uint32_t lane_cols = tmem_base + ((quarter * 32u) << 16) + half * 128u;
         const uint32_t leader_empty0 = ptx::mapa_shared(acc_empty_bar(0), 0);
@@ -303,7 +345,7 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
             }
             if (!ok)
                 break;
-            f8_store(p, &tma_c, stage_gen, stage_u32, lane, row0, col0, acc);
+            f8_store(p, &tma_c, stage_u32, lane, row0, col0, acc);
             __syncwarp();
         }
         if (p.c_tma_ok)
