@@ -40,6 +40,7 @@ struct GroupedParams {
     uint32_t c_pair_ok;      // 1: a column pair (even, odd) of any row of C is 4-byte aligned
     uint32_t c_vec_ok;       // 1: rows of C are 16-byte aligned
     uint32_t c_tma_ok;       // 1: the tensor map of C is valid (weight gradient)
+    uint32_t c_evict_first;  // 1: TMA stores of C carry an evict-first L2 hint
     uint32_t pdl;
     DeviceStatus *status;
     uint64_t timeout_ns;

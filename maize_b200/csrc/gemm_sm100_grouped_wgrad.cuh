@@ -98,7 +98,12 @@ __device__ __forceinline__ void wgrad_drain_tma(const GroupedParams &p, const CU
         ptx::fence_proxy_async_shared();
         __syncwarp();
         if (lane == 0) {
-            ptx::tma_store_3d(tma_c, base, static_cast<int32_t>(col), static_cast<int32_t>(row0), static_cast<int32_t>(z));
+            // DW passes through L2 once: evict first (32 groups of 128 rows, 1024 x 1408: 47 -> 41 us)
+            if (p.c_evict_first)
+                ptx::tma_store_3d_hint(tma_c, base, static_cast<int32_t>(col), static_cast<int32_t>(row0), static_cast<int32_t>(z),
+                                       ptx::policy_evict_first());
+            else
+                ptx::tma_store_3d(tma_c, base, static_cast<int32_t>(col), static_cast<int32_t>(row0), static_cast<int32_t>(z));
             ptx::bulk_commit_group();
         }
         buf ^= 1u;

@@ -201,6 +201,7 @@ maize_status_t maize_grouped_gemm_bf16_wgrad(maize_ctx_t *ctx, const void *a, ui
     p.rows = rows;
     p.n = n;
     p.k = k;
+    p.c_evict_first = ctx->c_evict_first;
     p.pdl = ctx->pdl;
     p.status = ctx->d_status;
     p.timeout_ns = ctx->timeout_ns;

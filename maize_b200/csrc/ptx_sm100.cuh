@@ -193,6 +193,15 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, uint32_t sm
                  : "memory");
 }
 
+__device__ __forceinline__ void tma_store_3d_hint(const CUtensorMap *map, uint32_t smem_src, int32_t x, int32_t y, int32_t z,
+                                                  uint64_t policy)
+{
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group.L2::cache_hint [%0, {%2, %3, %4}], [%1], %5;" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(smem_src), "r"(x), "r"(y), "r"(z), "l"(policy)
+                 : "memory");
+}
+
 __device__ __forceinline__ void bulk_commit_group() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 
 // Until at most N of this thread's bulk groups are still READING their shared-memory source.
