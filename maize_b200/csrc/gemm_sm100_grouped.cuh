@@ -12,7 +12,8 @@
 // of A on the M side a group of 300 rows would multiply 512.
 //
 // What follows from that: the accumulator is C transposed (TMEM lane = column of C, TMEM column = row of C); the epilogue
-// trades neighbouring lanes' halves so that a lane stores two columns of one row (4 bytes, 64-byte runs per row).
+// trades neighbouring lanes' halves so that a lane has two columns of one row.  These go through shared memory and TMA stores
+// where C's rows allow it, else out as 4-byte (2-byte) stores.
 //
 // Rows of A past the end of a group's tile may be loaded (they belong to the next group); they meet only accumulator
 // columns that are never stored, or lie beyond the MMA's N.  W is a stack of matrices in a 3-D tensor map, so rows and
@@ -39,7 +40,7 @@ struct GroupedParams {
     uint32_t n, k;
     uint32_t c_pair_ok;      // 1: a column pair (even, odd) of any row of C is 4-byte aligned
     uint32_t c_vec_ok;       // 1: rows of C are 16-byte aligned
-    uint32_t c_tma_ok;       // 1: the tensor map of C is valid (weight gradient)
+    uint32_t c_tma_ok;       // 1: the tensor map of C is valid
     uint32_t c_evict_first;  // 1: TMA stores of C carry an evict-first L2 hint
     uint32_t pdl;
     DeviceStatus *status;
@@ -140,12 +141,18 @@ __device__ __forceinline__ GroupedTile grouped_tile(uint64_t t, uint32_t n_block
     return r;
 }
 
+// The grouped kernel has eight epilogue warps, two for each quarter of the lanes: they take the 32-row chunks of a tile in
+// turn.  Two warps with neighbouring quarters share a staging buffer of 32 rows x 64 columns.
+constexpr uint32_t kGroupedEpilogueWarps = 8;
+constexpr uint32_t kGroupedThreads = 64 + 32 * kGroupedEpilogueWarps;
+
 template <uint32_t STAGES>
 struct GroupedSmemLayout {
     static constexpr uint32_t kWBytes = kBlockM * kBlockK * 2;                  // this CTA's 128 rows of W, one k-block
     static constexpr uint32_t kABytes = (kGroupedTileRows / 2) * kBlockK * 2;   // this CTA's half of the rows of A
     static constexpr uint32_t kStageBytes = kWBytes + kABytes;
-    static constexpr uint32_t kBarOffset = STAGES * kStageBytes;
+    static constexpr uint32_t kStagingOffset = STAGES * kStageBytes;
+    static constexpr uint32_t kBarOffset = kStagingOffset + kGroupedEpilogueWarps / 2 * kTmaStoreBufBytes;
     static constexpr uint32_t kNumBars = 2 * STAGES + 4;
     static constexpr uint32_t kTmemSlotOffset = kBarOffset + kNumBars * 8;
     static constexpr uint32_t kAbortOffset = kTmemSlotOffset + 4;
@@ -192,12 +199,50 @@ __device__ __forceinline__ void store_transposed_chunk(const GroupedParams &p, u
             dst[static_cast<uint64_t>(j) * p.ldc] = __float2bfloat16_rn(__uint_as_float(acc[j]));
 }
 
+// The same for C that TMA can store: two warps write their 32 columns each as rows of 64 into a shared buffer (16-byte chunk
+// j of row r at j ^ (r & 7)); all 32 rows of a whole chunk leave as one TMA store of 128-byte rows, those of a chunk that the
+// group's end cuts are stored row by row.  `half` = which of the two warps, `barrier` = the pair's barrier.
+__device__ __forceinline__ void store_transposed_chunk_tma(const GroupedParams &p, const CUtensorMap *tma_c, uint32_t stage_u32,
+                                                           uint32_t barrier, uint32_t half, uint32_t row0, uint32_t valid,
+                                                           uint32_t col0, uint32_t lane, const uint32_t (&acc)[32])
+{
+    if (half == 0 && lane == 0)
+        ptx::bulk_wait_group_read<0>();  // the buffer's last store has read it
+    ptx::named_barrier(barrier, 64);
+    const bool odd = (lane & 1u) != 0u;
+    const uint32_t chunk = half * 4u + (lane >> 3), at = ((lane >> 1) & 3u) * 4u;
+#pragma unroll
+    for (uint32_t j = 0; j < 32; j += 2) {
+        const uint32_t mine = ptx::pack_bf16x2(acc[j], acc[j + 1]);
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+        const uint32_t word = odd ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
+        const uint32_t r = j + (odd ? 1u : 0u);
+        ptx::st_shared_u32(stage_u32 + r * 128u + ((chunk ^ (r & 7u)) << 4) + at, word);
+    }
+    ptx::fence_proxy_async_shared();
+    ptx::named_barrier(barrier, 64);
+    if (valid == 32u) {
+        if (half == 0 && lane == 0) {
+            ptx::tma_store_2d(tma_c, stage_u32, static_cast<int32_t>(col0), static_cast<int32_t>(row0));
+            ptx::bulk_commit_group();
+        }
+    } else {
+        const uint32_t col = col0 + lane * 2u;
+        for (uint32_t r = half; r < valid; r += 2) {
+            const uint32_t word = ptx::ld_shared_u32(stage_u32 + r * 128u + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4u);
+            if (col < p.n)  // N is even
+                *reinterpret_cast<uint32_t *>(p.c + static_cast<uint64_t>(row0 + r) * p.ldc + col) = word;
+        }
+    }
+    __syncwarp();
+}
+
 // W_KN: the weights are stored K x N; this CTA's 128 columns are two boxes of {64 columns, 64 k-rows} per k-block, read
 // by the MMA as an MN-major operand.
 template <bool W_KN, uint32_t STAGES>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNumThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
 gemm_bf16_sm100_grouped(const __grid_constant__ RowMaps tma_a, const __grid_constant__ CUtensorMap tma_w,
-                        const GroupedParams p)
+                        const __grid_constant__ CUtensorMap tma_c, const GroupedParams p)
 {
     using L = GroupedSmemLayout<STAGES>;
     constexpr uint32_t kTmemCols = 2 * kGroupedTileRows;  // two accumulator buffers of 256 columns
@@ -235,7 +280,7 @@ gemm_bf16_sm100_grouped(const __grid_constant__ RowMaps tma_a, const __grid_cons
         }
         for (uint32_t b = 0; b < 2; ++b) {
             ptx::mbar_init(acc_full_bar(b), 1);
-            ptx::mbar_init(acc_empty_bar(b), 2 * kNumEpilogueWarps);
+            ptx::mbar_init(acc_empty_bar(b), 2 * kGroupedEpilogueWarps);
         }
         *abort_flag = 0;
         ptx::fence_barrier_init();
@@ -344,25 +389,33 @@ gemm_bf16_sm100_grouped(const __grid_constant__ RowMaps tma_a, const __grid_cons
         __syncwarp();
     } else {
         // ----------------------------------------------------------- epilogue --
-        const uint32_t quarter = warp & 3u;
+        const uint32_t quarter = warp & 3u, turn = (warp - 2u) >> 2;  // this warp takes every other chunk of 32 rows
+        const uint32_t share = turn * 2u + (quarter >> 1);               // buffer and barrier of the two warps side by side
+        const uint32_t stage_u32 = smem_base + L::kStagingOffset + share * kTmaStoreBufBytes;
         uint32_t acc = 0, acc_phase = 0, g = 0;
         bool ok = true;
         for (uint64_t t = pair; ok && t < num_tiles; t += num_pairs) {
             const GroupedTile tile = grouped_tile(t, n_blocks, tab, g);
             ok = wait_bounded<true>(acc_full_bar(acc), acc_phase, ctl, 3);
-            ok = __all_sync(0xffffffffu, ok);
+            // both warps of a buffer go on or both give up: neither may wait at their barrier for one that has left
+            ok = ptx::named_barrier_and(1u + share, 64, ok);
             if (!ok)
                 break;
             ptx::tcgen05_fence_after();
             const uint32_t taddr = tmem_base + acc * kGroupedTileRows + ((quarter * 32u) << 16);
-            const uint32_t warp_col = tile.n_blk * kGroupedTileCols + cta_rank * kBlockM + quarter * 32u;
-            if (warp_col < p.n) {
+            const uint32_t pair_col = tile.n_blk * kGroupedTileCols + cta_rank * kBlockM + (quarter >> 1) * 64u;
+            const uint32_t warp_col = pair_col + (quarter & 1u) * 32u;
+            if (pair_col < p.n) {
 #pragma unroll 1
-                for (uint32_t r = 0; r < tile.rows; r += 32) {
+                for (uint32_t r = turn * 32u; r < tile.rows; r += 64) {
                     uint32_t v[32];
                     ptx::tmem_ld_32x32b_x32(taddr + r, v);
                     ptx::tmem_ld_wait();
-                    store_transposed_chunk(p, tile.row0 + r, min(32u, tile.rows - r), warp_col + lane, lane, v);
+                    const uint32_t valid = min(32u, tile.rows - r);
+                    if (p.c_tma_ok)
+                        store_transposed_chunk_tma(p, &tma_c, stage_u32, 1u + share, quarter & 1u, tile.row0 + r, valid, pair_col, lane, v);
+                    else if (warp_col < p.n)
+                        store_transposed_chunk(p, tile.row0 + r, valid, warp_col + lane, lane, v);
                     __syncwarp();
                 }
             }
@@ -375,6 +428,8 @@ gemm_bf16_sm100_grouped(const __grid_constant__ RowMaps tma_a, const __grid_cons
                 acc_phase ^= 1u;
             }
         }
+        if (p.c_tma_ok)
+            tma_store_drain(lane);
         role_ok = ok;
     }
     if (!role_ok) {

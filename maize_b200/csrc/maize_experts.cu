@@ -107,15 +107,23 @@ maize_status_t grouped_impl(maize_ctx_t *ctx, const void *a, uint64_t lda, const
     if (st != MAIZE_OK)
         return st;
 
+    // rows of C that TMA can store (N has to end on a 16-byte piece, see the weight gradient)
+    CUtensorMap tc;
+    memset(&tc, 0, sizeof tc);
+    if (ctx->tma_store && n % 8 == 0 && ldc % 8 == 0 && aligned(c, 16) && ldc * 2 < (1ull << 40)) {
+        p.c_tma_ok = matrix_map(ctx, &tc, c, rows, n, ldc, 32) == MAIZE_OK;
+        ctx->err.clear();
+    }
+
     const uint64_t n_blocks = (uint64_t(n) + maize::kGroupedTileCols - 1) / maize::kGroupedTileCols;
     // at most: whole row tiles plus one more in every group that has rows
     const uint64_t row_tiles = rows / maize::kGroupedTileRows + (rows < groups ? rows : groups);
     const uint32_t grid = persistent_grid(ctx, row_tiles * n_blocks, 2);
     using L = maize::GroupedSmemLayout<6>;
-    return b_kn ? launch(ctx, maize::kAttrGroupedKn, maize::gemm_bf16_sm100_grouped<true, 6>, grid, maize::kNumThreads,
-                         L::kDynamicBytes, stream, ta, tw, p)
-                : launch(ctx, maize::kAttrGrouped, maize::gemm_bf16_sm100_grouped<false, 6>, grid, maize::kNumThreads,
-                         L::kDynamicBytes, stream, ta, tw, p);
+    return b_kn ? launch(ctx, maize::kAttrGroupedKn, maize::gemm_bf16_sm100_grouped<true, 6>, grid, maize::kGroupedThreads,
+                         L::kDynamicBytes, stream, ta, tw, tc, p)
+                : launch(ctx, maize::kAttrGrouped, maize::gemm_bf16_sm100_grouped<false, 6>, grid, maize::kGroupedThreads,
+                         L::kDynamicBytes, stream, ta, tw, tc, p);
 }
 
 }  // namespace

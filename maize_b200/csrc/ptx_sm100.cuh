@@ -229,6 +229,34 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+__device__ __forceinline__ void st_shared_u32(uint32_t addr, uint32_t v)
+{
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+// Barrier `id` (1 .. 15) among `threads` threads of the CTA, whole warps.
+__device__ __forceinline__ void named_barrier(uint32_t id, uint32_t threads)
+{
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// The same, and whether `value` holds for all of them.
+__device__ __forceinline__ bool named_barrier_and(uint32_t id, uint32_t threads, bool value)
+{
+    uint32_t all;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.and.pred q, %2, %3, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t"
+        "}"
+        : "=r"(all)
+        : "r"(static_cast<uint32_t>(value)), "r"(id), "r"(threads)
+        : "memory");
+    return all != 0;
+}
+
 __device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr)
 {
     uint32_t v;

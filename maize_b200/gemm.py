@@ -80,6 +80,7 @@ class Context:
             raise MaizeError(st, self._lib.maize_status_string(st).decode())
         self._h = handle
         self.device = int(device)
+        self._device = f"cuda:{self.device}"  # torch's name of it
 
     def close(self) -> None:
         if getattr(self, "_h", None):
@@ -269,28 +270,26 @@ class Context:
     def _stream(self, stream) -> int:
         """Handle of the stream a call runs on: the given one, or the current stream of the context's device."""
         if stream is None:
-            import torch
-            return torch.cuda.current_stream(self.device).cuda_stream if _raw_stream is None else _raw_stream(self.device)
+            return _torch.cuda.current_stream(self.device).cuda_stream if _raw_stream is None else _raw_stream(self.device)
         return stream if isinstance(stream, int) else stream.cuda_stream
 
-    def _new(self, like, shape, dtype, stream):
-        """An output tensor on the device of `like`, allocated for the stream the call runs on."""
+    def _new(self, shape, dtype, stream):
+        """An output tensor, allocated for the stream the call runs on."""
         if stream is None:
-            return like.new_empty(shape, dtype=dtype)
-        import torch
+            return _torch.empty(*shape, dtype=dtype, device=self._device)
         if isinstance(stream, int):
-            stream = torch.cuda.ExternalStream(stream, device=self.device)
-        with torch.cuda.stream(stream):
-            return like.new_empty(shape, dtype=dtype)
+            stream = _torch.cuda.ExternalStream(stream, device=self.device)
+        with _torch.cuda.stream(stream):
+            return _torch.empty(*shape, dtype=dtype, device=self._device)
 
     def _offsets(self, offsets, groups: int) -> int:
-        if (offsets.dtype is _types().int32 and offsets.dim() == 1 and offsets.shape[0] == groups + 1
+        if (offsets.dtype is _torch.int32 and offsets.dim() == 1 and offsets.numel() == groups + 1
                 and offsets.get_device() == self.device and offsets.is_contiguous()):
             return offsets.data_ptr()
         raise MaizeError(_ffi.INVALID_ARG, f"offsets: expected {groups + 1} contiguous int32 values on cuda:{self.device}")
 
     def _grouped(self, entry, a, b, offsets, out, stream, kn: bool):
-        bf16 = _types().bfloat16
+        bf16 = (_torch or _types()).bfloat16
         sa, sb = self._own("a", a, 2, bf16), self._own("b", b, 3, bf16)
         rows, k = a.shape
         groups, b_rows, b_cols = b.shape
@@ -299,7 +298,7 @@ class Context:
             raise MaizeError(_ffi.INVALID_ARG, f"a has {k} columns, the matrices of b a K of {kb}")
         at = self._offsets(offsets, groups)
         if out is None:
-            out = self._new(a, (rows, n), bf16, stream)
+            out = self._new((rows, n), bf16, stream)
             ldc = n
         else:
             ldc = self._own("out", out, 2, bf16)[0]
@@ -327,7 +326,7 @@ class Context:
     def grouped_gemm_wgrad(self, a, dc, offsets, out=None, stream=None):
         """``out[g] = dc[rows of g].T @ a[rows of g]``: the gradient of ``grouped_gemm``'s b (groups x N x K) from its
         input ``a`` (rows x K) and the gradient ``dc`` (rows x N) of its result.  A group without rows gets zeros."""
-        bf16 = _types().bfloat16
+        bf16 = (_torch or _types()).bfloat16
         sa, sd = self._own("a", a, 2, bf16), self._own("dc", dc, 2, bf16)
         rows, k = a.shape
         rows_dc, n = dc.shape
@@ -338,7 +337,7 @@ class Context:
             raise MaizeError(_ffi.INVALID_ARG, "offsets: expected groups + 1 int32 values")
         at = self._offsets(offsets, groups)
         if out is None:
-            out = self._new(a, (groups, n, k), bf16, stream)
+            out = self._new((groups, n, k), bf16, stream)
             so = (n * k, k)
         else:
             so = self._own("out", out, 3, bf16)
@@ -356,21 +355,21 @@ class Context:
     def quantize_e4m3(self, x, block_rows: int = 1, out=None, scales=None, stream=None):
         """bf16 rows x cols -> (e4m3 tensor of the same shape, fp32 scales), with a power-of-two scale for each 1 x 128
         (``block_rows`` = 1: activations) or 128 x 128 block (``block_rows`` = 128: weights): ``x ~ q * scale``."""
-        torch = _types()
+        torch = _torch or _types()
         sx = self._own("x", x, 2, torch.bfloat16)
         rows, cols = x.shape
         if block_rows != 1 and block_rows != 128:
             raise MaizeError(_ffi.INVALID_ARG, "block_rows must be 1 or 128")
         down, across = -(-rows // block_rows), -(-cols // 128)
         if out is None:
-            out = self._new(x, (rows, cols), torch.float8_e4m3fn, stream)
+            out = self._new((rows, cols), torch.float8_e4m3fn, stream)
             ldq = cols
         else:
             ldq = self._own("out", out, 2, torch.float8_e4m3fn)[0]
             if out.shape != (rows, cols):
                 raise MaizeError(_ffi.INVALID_ARG, f"out: expected {rows} x {cols}")
         if scales is None:
-            scales = self._new(x, (down, across), torch.float32, stream)
+            scales = self._new((down, across), torch.float32, stream)
             lds = across
         else:
             lds = self._own("scales", scales, 2, torch.float32)[0]
@@ -386,7 +385,7 @@ class Context:
     def gemm_e4m3(self, a, a_scales, b, b_scales, out=None, stream=None):
         """``out = (a * a_scales) @ (b * b_scales).T`` in bf16 for e4m3 a (M x K) with a scale for each 1 x 128 block
         (M x ceil(K/128), fp32) and e4m3 b (N x K) with one for each 128 x 128 block (ceil(N/128) x ceil(K/128))."""
-        torch = _types()
+        torch = _torch or _types()
         f8, f32 = torch.float8_e4m3fn, torch.float32
         sa, sb = self._own("a", a, 2, f8), self._own("b", b, 2, f8)
         ssa, ssb = self._own("a_scales", a_scales, 2, f32), self._own("b_scales", b_scales, 2, f32)
@@ -398,7 +397,7 @@ class Context:
         if a_scales.shape != (m, blocks) or b_scales.shape != (down, blocks):
             raise MaizeError(_ffi.INVALID_ARG, f"scales: expected {m} x {blocks} for a, {down} x {blocks} for b")
         if out is None:
-            out = self._new(a, (m, n), torch.bfloat16, stream)
+            out = self._new((m, n), torch.bfloat16, stream)
             ldc = n
         else:
             ldc = self._own("out", out, 2, torch.bfloat16)[0]
