@@ -1,4 +1,4 @@
-// The e4m3 product for few rows of A (M <= 128): bound by reading B once.
+// The e4m3 product for few rows of A, or few tiles: K is split over the CTAs of a cluster.  For M <= 128 bound by reading B once.
 //
 // Rows of A are the M side of the MMA, up to 256 rows of B its N side: an MMA takes about 128 cycles for the 32 k of its 128
 // M-side rows whatever its N, so the operand that has to stream belongs on the N side (with B on the M side 16 x 16384 x 4096
@@ -23,7 +23,7 @@ namespace maize {
 constexpr uint32_t kF8SkinnyThreads = 64 + 32 * 8;
 
 struct F8SkinnyParams {
-    GemmParams g;  // C and the sizes; tiles_n = tiles
+    GemmParams g;  // C and the sizes; tiles_m blocks of 128 rows of A (1 with copies of them), tiles_n blocks of B
     const float *sa, *sb;
     uint64_t ld_sa, ld_sb;
     uint32_t bn;  // rows of B per tile, a multiple of 32, at most 256
@@ -52,8 +52,56 @@ struct F8SkinnyLayout {
     static constexpr uint32_t kDynamicBytes = kUsedBytes + 1024;
     static_assert(kDynamicBytes <= 232448, "exceeds 227 KiB of shared memory per CTA");
     static_assert(kDynamicBytes > 116224, "two CTAs could share an SM and contend for TMEM");
-    static_assert(kShare < 32 || kShare * 128 >= kStageWarpBytes, "a warp's part of the exchange serves as its staging buffer");
+    static_assert(kShare >= 8 && kShare <= 32, "columns of a warp that one CTA finishes");
 };
+
+// Stores 32 rows x COLS columns of C, lane = row: 16 bytes at a time where C's rows are aligned.  Else through `stage` (32 rows
+// of COLS bf16), so that COLS / 2 lanes store a row in 4-byte words; a row that starts between two words gets its halves
+// from the neighbouring lane and 2-byte stores at its ends.
+template <uint32_t COLS>
+__device__ __forceinline__ void f8_skinny_store(const GemmParams &p, uint32_t stage, uint32_t lane, uint32_t row0, uint32_t col0,
+                                                uint32_t end, const uint32_t (&out)[COLS])
+{
+    uint32_t word[COLS / 2];
+#pragma unroll
+    for (uint32_t i = 0; i < COLS / 2; ++i)
+        word[i] = ptx::pack_bf16x2(out[2 * i], out[2 * i + 1]);
+    if (p.c_vec_ok && col0 + COLS <= end) {
+        if (row0 + lane < p.m) {
+            uint4 *dst = reinterpret_cast<uint4 *>(p.c + static_cast<uint64_t>(row0 + lane) * p.ldc + col0);
+#pragma unroll
+            for (uint32_t i = 0; i < COLS / 8; ++i)
+                dst[i] = make_uint4(word[4 * i], word[4 * i + 1], word[4 * i + 2], word[4 * i + 3]);
+        }
+        return;
+    }
+    constexpr uint32_t kLanes = COLS / 2, kRows = 32 / kLanes;  // lanes per row, rows at a time
+#pragma unroll
+    for (uint32_t i = 0; i < COLS / 8; ++i)
+        ptx::st_shared_v4(stage + lane * (COLS * 2) + i * 16u, word[4 * i], word[4 * i + 1], word[4 * i + 2], word[4 * i + 3]);
+    __syncwarp();
+    const uint32_t l = lane % kLanes, left = end - col0;
+#pragma unroll 4
+    for (uint32_t r = lane / kLanes; r < 32; r += kRows) {
+        const uint32_t mine = ptx::ld_shared_u32(stage + r * (COLS * 2) + l * 4u);
+        const uint32_t before = __shfl_up_sync(0xffffffffu, mine, 1, kLanes);
+        if (row0 + r >= p.m)
+            continue;
+        __nv_bfloat16 *dst = p.c + static_cast<uint64_t>(row0 + r) * p.ldc + col0;
+        const bool between = (reinterpret_cast<uintptr_t>(dst) & 2u) != 0u;
+        const int32_t c = static_cast<int32_t>(2u * l) - (between ? 1 : 0);  // this lane's two columns from here
+        const uint32_t v = between ? __funnelshift_l(before, mine, 16) : mine;
+        if (c < 0)
+            *reinterpret_cast<uint16_t *>(dst) = static_cast<uint16_t>(mine);
+        else if (static_cast<uint32_t>(c) + 1 < left)
+            *reinterpret_cast<uint32_t *>(dst + c) = v;
+        else if (static_cast<uint32_t>(c) < left)
+            *reinterpret_cast<uint16_t *>(dst + c) = static_cast<uint16_t>(v);
+        if (between && l == kLanes - 1 && COLS - 1 < left)
+            *reinterpret_cast<uint16_t *>(dst + COLS - 1) = static_cast<uint16_t>(mine >> 16);
+    }
+    __syncwarp();
+}
 
 template <uint32_t REPL, uint32_t S, uint32_t STAGES>
 __global__ void __launch_bounds__(kF8SkinnyThreads, 1)
@@ -88,6 +136,7 @@ gemm_e4m3_sm100_skinny(const __grid_constant__ CUtensorMap tma_a, const __grid_c
     const uint32_t per_cta = (all_kb + S - 1) / S;
     const uint32_t kb0 = min(rank * per_cta, all_kb);
     const uint32_t num_kb = min(per_cta, all_kb - kb0);  // may be 0 in the last CTAs
+    const uint32_t tiles = p.tiles_m * p.tiles_n;  // the blocks of A run fastest: they share a block of B
     const WaitCtl ctl{abort_flag, p.status, p.timeout_ns};
 
     if (threadIdx.x == 0) {
@@ -127,8 +176,8 @@ gemm_e4m3_sm100_skinny(const __grid_constant__ CUtensorMap tma_a, const __grid_c
         if (lane == 0) {
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            const uint32_t bytes = (f.bn + REPL * p.m) * kF8BlockK;
-            for (uint32_t t = cluster; ok && t < p.tiles_n; t += num_clusters) {
+            const uint32_t bytes = (f.bn + REPL * min(p.m, kBlockM)) * kF8BlockK;
+            for (uint32_t t = cluster; ok && t < tiles; t += num_clusters) {
                 for (uint32_t kb = 0; kb < num_kb; ++kb) {
                     ok = wait_bounded(empty_bar(stage), phase ^ 1u, ctl, 1);
                     if (!ok)
@@ -136,10 +185,11 @@ gemm_e4m3_sm100_skinny(const __grid_constant__ CUtensorMap tma_a, const __grid_c
                     const uint32_t sa = smem_base + stage * L::kStageBytes;
                     const int32_t kx = static_cast<int32_t>((kb0 + kb) * kF8BlockK);
                     ptx::mbar_arrive_expect_tx(full_bar(stage), bytes);
-                    ptx::tma_load_2d(sa + L::kABytes, &tma_b, full_bar(stage), kx, static_cast<int32_t>(t * f.bn));
+                    ptx::tma_load_2d(sa + L::kABytes, &tma_b, full_bar(stage), kx, static_cast<int32_t>(t / p.tiles_m * f.bn));
 #pragma unroll
                     for (uint32_t r = 0; r < REPL; ++r)
-                        ptx::tma_load_2d(sa + r * L::kRows * kF8BlockK, &tma_a, full_bar(stage), kx, 0);
+                        ptx::tma_load_2d(sa + r * L::kRows * kF8BlockK, &tma_a, full_bar(stage), kx,
+                                         static_cast<int32_t>(t % p.tiles_m * kBlockM));
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1u;
@@ -156,7 +206,7 @@ gemm_e4m3_sm100_skinny(const __grid_constant__ CUtensorMap tma_a, const __grid_c
             uint32_t acc = 0, acc_phase = 0;
             bool ok = true;
             const uint32_t idesc = ptx::make_instr_desc_e4m3(kBlockM, f.bn);
-            for (uint32_t t = cluster; ok && t < p.tiles_n; t += num_clusters) {
+            for (uint32_t t = cluster; ok && t < tiles; t += num_clusters) {
                 for (uint32_t kb = 0; kb < num_kb; ++kb) {
                     ok = wait_bounded(full_bar(stage), phase, ctl, 2) &&
                          wait_bounded(acc_empty_bar(acc), acc_phase ^ 1u, ctl, 2);
@@ -188,16 +238,16 @@ gemm_e4m3_sm100_skinny(const __grid_constant__ CUtensorMap tma_a, const __grid_c
         // ---------------------------------------------- promotion and epilogue --
         const uint32_t quarter = warp & 3u, w = warp - 2u;
         // this warp's rows of A and columns of the tile
-        const uint32_t row0 = REPL == 4 ? 0u : (REPL == 2 ? (quarter & 1u) * 32u : quarter * 32u);
+        const uint32_t warp_row = REPL == 4 ? 0u : (REPL == 2 ? (quarter & 1u) * 32u : quarter * 32u);
         const uint32_t col0 = (REPL == 4 ? quarter * 64u : (REPL == 2 ? (quarter >> 1) * 128u : 0u)) + (w >> 2) * L::kWarpCols;
         const uint32_t lane_addr = tmem_base + ((quarter * 32u) << 16) + col0;
-        const float *sa = f.sa + static_cast<uint64_t>(min(row0 + lane, p.m - 1)) * f.ld_sa + kb0;
         const uint32_t last_block = (p.n - 1) / 128u, last_kb = num_kb > 0 ? num_kb - 1 : 0u;
         const uint32_t exchange = smem_base + L::kExchangeOffset;
         uint32_t acc = 0, acc_phase = 0, parity = 0;
         bool ok = true;
-        for (uint32_t t = cluster; ok && t < p.tiles_n; t += num_clusters, parity ^= 1u) {
-            const uint32_t n0 = t * f.bn;
+        for (uint32_t t = cluster; ok && t < tiles; t += num_clusters, parity ^= 1u) {
+            const uint32_t n0 = t / p.tiles_m * f.bn, row0 = t % p.tiles_m * kBlockM + warp_row;
+            const float *sa = f.sa + static_cast<uint64_t>(min(row0 + lane, p.m - 1)) * f.ld_sa + kb0;
             // the (at most two) scale blocks of this warp's columns; bit c of `second`: chunk c lies in the second
             const uint32_t block0 = (n0 + col0) / 128u;
             uint32_t second = 0;
@@ -314,37 +364,10 @@ gemm_e4m3_sm100_skinny(const __grid_constant__ CUtensorMap tma_a, const __grid_c
                 out[4 * i + 2] = __float_as_uint(total.z), out[4 * i + 3] = __float_as_uint(total.w);
             }
             __syncwarp();
-            // ---- store this CTA's share: kShare columns of 32 rows
+            // ---- store this CTA's share: kShare columns of 32 rows (what came for this warp has been read: its place serves)
             const uint32_t end = min(p.n, n0 + f.bn), out_col = n0 + col0 + rank * L::kShare;
-            if constexpr (L::kShare >= 32) {
-                GemmParams q = p;
-                q.n = end;
-                uint8_t *staging = smem_gen + L::kExchangeOffset + w * (L::kShare * 128u);  // what came has been read
-#pragma unroll
-                for (uint32_t c = 0; c < L::kShare; c += 32) {
-                    uint32_t v[32];
-#pragma unroll
-                    for (uint32_t i = 0; i < 32; ++i)
-                        v[i] = out[c + i];
-                    store_chunk(q, staging, row0, out_col + c, lane, v);
-                    __syncwarp();
-                }
-            } else if (row0 + lane < p.m) {
-                __nv_bfloat16 *dst = p.c + static_cast<uint64_t>(row0 + lane) * p.ldc + out_col;
-#pragma unroll
-                for (uint32_t i = 0; i < L::kShare; i += 8) {
-                    if (p.c_vec_ok && out_col + i + 8 <= end) {
-                        *reinterpret_cast<uint4 *>(dst + i) =
-                            make_uint4(ptx::pack_bf16x2(out[i], out[i + 1]), ptx::pack_bf16x2(out[i + 2], out[i + 3]),
-                                       ptx::pack_bf16x2(out[i + 4], out[i + 5]), ptx::pack_bf16x2(out[i + 6], out[i + 7]));
-                    } else {
-#pragma unroll
-                        for (uint32_t j = 0; j < 8; ++j)
-                            if (out_col + i + j < end)
-                                dst[i + j] = __float2bfloat16_rn(__uint_as_float(out[i + j]));
-                    }
-                }
-            }
+            if (row0 < p.m && out_col < end)
+                f8_skinny_store<L::kShare>(p, exchange + w * (L::kShare * 128u), lane, row0, out_col, end, out);
             __syncwarp();
             if (lane < S && lane != rank)
                 ptx::mbar_arrive_cluster_addr(ptx::mapa_shared(sums_taken_bar, lane));

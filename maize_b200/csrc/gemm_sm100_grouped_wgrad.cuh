@@ -13,21 +13,26 @@
 // MN-major tiles a row is 128 consecutive bytes per box whatever the swizzle does inside it, so the clearing is a plain
 // fill of at most 15 rows x 4 boxes x 128 bytes.
 //
-// Roles per CTA (224 threads): TMA producer, MMA issuer (leader only), four epilogue warps, the fix warp.
+// Roles per CTA: TMA producer, MMA issuer (leader only), eight epilogue warps, the fix warp.
 // Bound: tensor pipe where groups have a few hundred rows, the HBM writes of DW below.
 #pragma once
 #include "gemm_sm100_grouped.cuh"
 
 namespace maize {
 
-constexpr uint32_t kWgradThreads = 224;
+// Eight epilogue warps, two for each quarter of the lanes, that take the tile's groups of 64 columns in turn.
+constexpr uint32_t kWgradEpilogueWarps = 8;
+constexpr uint32_t kWgradFixWarp = 2 + kWgradEpilogueWarps;
+constexpr uint32_t kWgradThreads = 32 * (kWgradFixWarp + 1);
+// One staging buffer of 32 rows x 64 columns per warp (a second one, at the cost of a ring stage, gained nothing).
+constexpr uint32_t kWgradStageWarpBytes = kTmaStoreBufBytes;
 
 template <uint32_t STAGES>
 struct WgradSmemLayout {
     static constexpr uint32_t kOperandBytes = kBlockM * kBlockK * 2;  // two boxes of 64 columns x 64 rows
     static constexpr uint32_t kStageBytes = 2 * kOperandBytes;        // [DC0, DC1, A0, A1]
     static constexpr uint32_t kStagingOffset = STAGES * kStageBytes;
-    static constexpr uint32_t kBarOffset = kStagingOffset + kTmaStageBytesTotal;
+    static constexpr uint32_t kBarOffset = kStagingOffset + kWgradEpilogueWarps * kWgradStageWarpBytes;
     static constexpr uint32_t kNumBars = 4 * STAGES + 4;
     static constexpr uint32_t kTmemSlotOffset = kBarOffset + kNumBars * 8;
     static constexpr uint32_t kAbortOffset = kTmemSlotOffset + 4;
@@ -61,12 +66,12 @@ __device__ __forceinline__ WgradTile wgrad_tile(uint32_t t, uint32_t m_blocks, u
 // boxes into matrix `z` of the stack; the map clips at N and K.
 __device__ __forceinline__ void wgrad_drain_tma(const GroupedParams &p, const CUtensorMap *tma_c, uint32_t stage_u32,
                                                 uint32_t taddr, bool zeros, uint32_t lane, uint32_t row0, uint32_t col0,
-                                                uint32_t z, uint32_t &buf)
+                                                uint32_t z, uint32_t turn)
 {
     if (row0 >= p.n)
         return;
 #pragma unroll 1
-    for (uint32_t g = 0; g < kGroupedTileCols / 64; ++g) {
+    for (uint32_t g = turn; g < kGroupedTileCols / 64; g += 2) {
         const uint32_t col = col0 + g * 64u;
         if (col >= p.k)
             break;
@@ -81,10 +86,9 @@ __device__ __forceinline__ void wgrad_drain_tma(const GroupedParams &p, const CU
             ptx::tmem_ld_wait();
         }
         if (lane == 0)
-            ptx::bulk_wait_group_read<1>();
+            ptx::bulk_wait_group_read<0>();  // the buffer's last store has read it
         __syncwarp();
-        const uint32_t base = stage_u32 + buf * kTmaStoreBufBytes;
-        const uint32_t row = base + lane * 128u;
+        const uint32_t row = stage_u32 + lane * 128u;
         const uint32_t sw = lane & 7u;
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
@@ -100,20 +104,20 @@ __device__ __forceinline__ void wgrad_drain_tma(const GroupedParams &p, const CU
         if (lane == 0) {
             // DW passes through L2 once: evict first (32 groups of 128 rows, 1024 x 1408: 47 -> 41 us)
             if (p.c_evict_first)
-                ptx::tma_store_3d_hint(tma_c, base, static_cast<int32_t>(col), static_cast<int32_t>(row0), static_cast<int32_t>(z),
+                ptx::tma_store_3d_hint(tma_c, stage_u32, static_cast<int32_t>(col), static_cast<int32_t>(row0), static_cast<int32_t>(z),
                                        ptx::policy_evict_first());
             else
-                ptx::tma_store_3d(tma_c, base, static_cast<int32_t>(col), static_cast<int32_t>(row0), static_cast<int32_t>(z));
+                ptx::tma_store_3d(tma_c, stage_u32, static_cast<int32_t>(col), static_cast<int32_t>(row0), static_cast<int32_t>(z));
             ptx::bulk_commit_group();
         }
-        buf ^= 1u;
     }
 }
 
 // The same with plain stores, for a DW whose rows are not 16-byte aligned: lane = row, 2-byte stores that are
 // consecutive across the warp after a transposition through the warp's staging buffer.
 __device__ __forceinline__ void wgrad_drain_plain(const GroupedParams &p, uint8_t *stage_warp, uint32_t taddr, bool zeros,
-                                                  uint32_t lane, uint32_t row0, uint32_t col0, uint32_t z)
+                                                  uint32_t lane, uint32_t row0, uint32_t col0, uint32_t z,
+                                                  uint32_t turn)
 {
     GemmParams q{};
     q.c = p.c + static_cast<uint64_t>(z) * p.c_stride;
@@ -122,7 +126,7 @@ __device__ __forceinline__ void wgrad_drain_plain(const GroupedParams &p, uint8_
     q.n = p.k;
     q.c_vec_ok = 0;
 #pragma unroll 1
-    for (uint32_t c = 0; c < kGroupedTileCols / 32; ++c) {
+    for (uint32_t c = turn; c < kGroupedTileCols / 32; c += 2) {
         uint32_t v[32];
         if (zeros) {
 #pragma unroll
@@ -186,7 +190,7 @@ gemm_bf16_sm100_grouped_wgrad(const __grid_constant__ CUtensorMap tma_dc, const 
         }
         for (uint32_t b = 0; b < 2; ++b) {
             ptx::mbar_init(acc_full_bar(b), 1);
-            ptx::mbar_init(acc_empty_bar(b), 2 * kNumEpilogueWarps);
+            ptx::mbar_init(acc_empty_bar(b), 2 * kWgradEpilogueWarps);
         }
         *abort_flag = 0;
         ptx::fence_barrier_init();
@@ -298,7 +302,7 @@ gemm_bf16_sm100_grouped_wgrad(const __grid_constant__ CUtensorMap tma_dc, const 
             role_ok = ok;
         }
         __syncwarp();
-    } else if (warp == 6) {
+    } else if (warp == kWgradFixWarp) {
         // ----------------------------------------------------------- fix warp --
         uint32_t stage = 0;
         uint32_t tail_phase = 0;  // bit s: parity of the next use of tail_bar(s) and peer_bar(s)
@@ -346,10 +350,9 @@ gemm_bf16_sm100_grouped_wgrad(const __grid_constant__ CUtensorMap tma_dc, const 
         role_ok = ok;
     } else {
         // ----------------------------------------------------------- epilogue --
-        const uint32_t quarter = warp & 3u;
-        uint8_t *stage_warp = smem_gen + L::kStagingOffset + (warp - 2u) * kTmaStageWarpBytes;
-        const uint32_t stage_u32 = smem_base + L::kStagingOffset + (warp - 2u) * kTmaStageWarpBytes;
-        uint32_t store_buf = 0;
+        const uint32_t quarter = warp & 3u, turn = (warp - 2u) >> 2;
+        uint8_t *stage_warp = smem_gen + L::kStagingOffset + (warp - 2u) * kWgradStageWarpBytes;
+        const uint32_t stage_u32 = smem_base + L::kStagingOffset + (warp - 2u) * kWgradStageWarpBytes;
         uint32_t acc = 0, acc_phase = 0;
         bool ok = true;
         for (uint32_t t = pair; ok && t < num_tiles; t += num_pairs) {
@@ -366,9 +369,9 @@ gemm_bf16_sm100_grouped_wgrad(const __grid_constant__ CUtensorMap tma_dc, const 
             const uint32_t row0 = tile.m_blk * 2 * kBlockM + cta_rank * kBlockM + quarter * 32u;
             const uint32_t col0 = tile.n_blk * kGroupedTileCols;
             if (p.c_tma_ok)
-                wgrad_drain_tma(p, &tma_dw, stage_u32, taddr, zeros, lane, row0, col0, tile.group, store_buf);
+                wgrad_drain_tma(p, &tma_dw, stage_u32, taddr, zeros, lane, row0, col0, tile.group, turn);
             else
-                wgrad_drain_plain(p, stage_warp, taddr, zeros, lane, row0, col0, tile.group);
+                wgrad_drain_plain(p, stage_warp, taddr, zeros, lane, row0, col0, tile.group, turn);
             if (!zeros) {
                 ptx::tcgen05_fence_before();
                 __syncwarp();

@@ -29,44 +29,52 @@ maize_status_t launch_skinny(maize_ctx_t *ctx, int slot, uint32_t clusters, cons
                              const maize::F8SkinnyParams &f, cudaStream_t stream)
 {
     using L = maize::F8SkinnyLayout<REPL, S, STAGES>;
-    const uint32_t grid = (f.g.tiles_n < clusters ? f.g.tiles_n : clusters) * S;
+    const uint64_t tiles = uint64_t(f.g.tiles_m) * f.g.tiles_n;
+    const uint32_t grid = (tiles < clusters ? static_cast<uint32_t>(tiles) : clusters) * S;
     return maize::launch_clusters(ctx, slot, maize::gemm_e4m3_sm100_skinny<REPL, S, STAGES>, grid, S, maize::kF8SkinnyThreads,
                                   L::kDynamicBytes, stream, ta, tb, f);
 }
 
-// How the tiles of a skinny product are cut: `parts` CTAs share a tile's K, `bn` rows of B per tile.
+// How the tiles of a product with K split over clusters are cut.
 struct SkinnyPlan {
-    uint32_t parts, clusters, bn;
-    double cost;  // microseconds, for comparison only
+    uint32_t copies;    // of the rows of A in an MMA's 128 lanes
+    uint32_t parts;     // CTAs that share a tile's K
+    uint32_t clusters;  // at a time
+    uint32_t tiles_m;   // blocks of 128 rows of A
+    uint32_t bn;        // rows of B per tile
+    double cost;        // microseconds beyond what every call takes, for comparison only
 };
 
-// One round of clusters covers clusters * widest rows of B; the tiles are as wide as fills whole rounds.  A k-block costs a
-// CTA 0.34 us (four MMAs of 128 rows and their hand-over) or its bytes at 80 GB/s per SM, measured; joining four parts about
-// 0.8 us more than joining two.  16 x 512 x 8192: 9.8 us in four parts, 14.7 in two; 5 x 9001 x 2048: 12.8 and 7.8.
-SkinnyPlan skinny_plan(uint32_t ctas, uint32_t parts, uint32_t widest, uint32_t rows_loaded, uint32_t n, uint32_t kblocks)
+// The tiles are as wide as fills whole rounds of clusters.  A k-block costs a CTA 0.34 us (the MMA thread's issue and the
+// hand-over of its accumulator) or its bytes at 80 GB/s per SM (47 with 128 different rows of A), a tile's end 2 us,
+// measured; joining four parts about 0.8 us more than joining two.  16 x 512 x 8192: 9.8 us in four parts, 14.7 in two; 5 x 9001 x 2048: 12.8, 7.8.
+SkinnyPlan skinny_plan(uint32_t ctas, uint32_t parts, uint32_t m, uint32_t n, uint32_t kblocks)
 {
     SkinnyPlan q;
+    q.copies = m <= 32 ? 4 : (m <= 64 ? 2 : 1);
     q.parts = parts;
+    q.tiles_m = (m + 127) / 128;
     // clusters of four fit only within a GPC: of the 37 that 148 SMs would make, 32 are counted on
     q.clusters = parts == 2 ? ctas / 2 : ctas * 32 / 148;
     if (q.clusters == 0)
         q.clusters = 1;
-    const uint64_t rounds = (uint64_t(n) + uint64_t(q.clusters) * widest - 1) / (uint64_t(q.clusters) * widest);
-    q.bn = static_cast<uint32_t>((uint64_t(n) + q.clusters * rounds - 1) / (q.clusters * rounds) + 31) / 32 * 32;
-    const double bytes = (q.bn + rows_loaded) * 128.0, block = bytes / 80e3 > 0.34 ? bytes / 80e3 : 0.34;
-    q.cost = double(rounds) * ((kblocks + parts - 1) / parts) * block + (parts == 2 ? 0.0 : 0.8);
+    const uint64_t widest = q.copies == 1 ? 128 : 256;
+    const uint64_t rounds = (uint64_t(q.tiles_m) * ((n + widest - 1) / widest) + q.clusters - 1) / q.clusters;
+    uint64_t per_m = rounds * q.clusters / q.tiles_m;  // tiles along N that fill the rounds
+    if (per_m == 0)
+        per_m = 1;
+    uint64_t bn = ((n + per_m - 1) / per_m + 31) / 32 * 32;
+    q.bn = static_cast<uint32_t>(bn < widest ? bn : widest);
+    const double bytes = (q.bn + q.copies * (m < 128 ? m : 128u)) * 128.0;
+    const double rate = q.copies == 1 ? 47e3 : 80e3, block = bytes / rate > 0.34 ? bytes / rate : 0.34;
+    q.cost = double(rounds) * (((kblocks + parts - 1) / parts) * block + (parts == 2 ? 2.0 : 2.8));
     return q;
 }
 
-maize_status_t skinny(maize_ctx_t *ctx, const void *a, uint64_t lda, const float *sa, uint64_t ld_sa, const void *b, uint64_t ldb,
-                      const float *sb, uint64_t ld_sb, void *c, uint64_t ldc, uint32_t m, uint32_t n, uint32_t k, cudaStream_t stream)
+maize_status_t skinny(maize_ctx_t *ctx, const SkinnyPlan &plan, const void *a, uint64_t lda, const float *sa, uint64_t ld_sa,
+                      const void *b, uint64_t ldb, const float *sb, uint64_t ld_sb, void *c, uint64_t ldc, uint32_t m, uint32_t n,
+                      uint32_t k, cudaStream_t stream)
 {
-    const uint32_t copies = m <= 32 ? 4 : (m <= 64 ? 2 : 1), widest = copies == 1 ? 128 : 256;
-    const uint32_t kblocks = (k + 127) / 128, ctas = maize::persistent_grid(ctx, 0xffffffffull, 1);
-    SkinnyPlan plan = skinny_plan(ctas, 2, widest, copies * m, n, kblocks);
-    const SkinnyPlan four = skinny_plan(ctas, 4, widest, copies * m, n, kblocks);
-    if (four.cost < plan.cost)
-        plan = four;
     const uint32_t bn = plan.bn;
     maize::F8SkinnyParams f = {};
     f.g.c = static_cast<__nv_bfloat16 *>(c);
@@ -74,6 +82,7 @@ maize_status_t skinny(maize_ctx_t *ctx, const void *a, uint64_t lda, const float
     f.g.m = m;
     f.g.n = n;
     f.g.k = k;
+    f.g.tiles_m = plan.tiles_m;
     f.g.tiles_n = (n + bn - 1) / bn;
     f.g.c_vec_ok = (ldc % 8 == 0 && aligned(c, 16)) ? 1u : 0u;
     f.g.pdl = ctx->pdl;
@@ -86,14 +95,14 @@ maize_status_t skinny(maize_ctx_t *ctx, const void *a, uint64_t lda, const float
     f.bn = bn;
     CUtensorMap ta, tb;
     maize_status_t st;
-    if ((st = byte_map(ctx, &ta, a, m, k, lda, m)) != MAIZE_OK || (st = byte_map(ctx, &tb, b, n, k, ldb, bn)) != MAIZE_OK)
+    if ((st = byte_map(ctx, &ta, a, m, k, lda, m < 128 ? m : 128)) != MAIZE_OK || (st = byte_map(ctx, &tb, b, n, k, ldb, bn)) != MAIZE_OK)
         return st;
     const int slot = maize::kAttrE4m3Skinny;
     const bool two = plan.parts == 2;
-    if (copies == 1)
+    if (plan.copies == 1)
         return two ? launch_skinny<1, 2, 6>(ctx, slot, plan.clusters, ta, tb, f, stream)
                    : launch_skinny<1, 4, 5>(ctx, slot + 1, plan.clusters, ta, tb, f, stream);
-    if (copies == 2)
+    if (plan.copies == 2)
         return two ? launch_skinny<2, 2, 4>(ctx, slot + 2, plan.clusters, ta, tb, f, stream)
                    : launch_skinny<2, 4, 3>(ctx, slot + 3, plan.clusters, ta, tb, f, stream);
     return two ? launch_skinny<4, 2, 4>(ctx, slot + 4, plan.clusters, ta, tb, f, stream)
@@ -196,8 +205,17 @@ maize_status_t maize_gemm_e4m3(maize_ctx_t *ctx, const void *a, uint64_t lda, co
         return fail(ctx, MAIZE_ERR_UNSUPPORTED, "A and B must be 16-byte aligned");
     if (lda >= (1ull << 40) || ldb >= (1ull << 40))
         return fail(ctx, MAIZE_ERR_UNSUPPORTED, "row pitch beyond the TMA limit of 2^40 bytes");
-    if (m <= 128)
-        return skinny(ctx, a, lda, static_cast<const float *>(a_scales), ld_a_scales, b, ldb, static_cast<const float *>(b_scales),
+    // Few rows of A, or few tiles: K over a cluster.  The other kernel takes 0.55 us for a k-block of a 256 x 256 tile and about
+    // 1.5 us more for a tile's end.
+    const uint32_t ctas = maize::persistent_grid(ctx, 0xffffffffull, 1), kb = static_cast<uint32_t>(kblocks);
+    SkinnyPlan plan = skinny_plan(ctas, 2, m, n, kb);
+    const SkinnyPlan four = skinny_plan(ctas, 4, m, n, kb);
+    if (four.cost < plan.cost)
+        plan = four;
+    const uint64_t pair_tiles = ((uint64_t(m) + 255) / 256) * ((uint64_t(n) + 255) / 256), pairs = ctas / 2 ? ctas / 2 : 1;
+    const double pair_cost = double((pair_tiles + pairs - 1) / pairs) * (kb * 0.55 + 1.5);
+    if (m <= 128 || plan.cost < pair_cost)
+        return skinny(ctx, plan, a, lda, static_cast<const float *>(a_scales), ld_a_scales, b, ldb, static_cast<const float *>(b_scales),
                       ld_b_scales, c, ldc, m, n, k, stream);
     CUtensorMap ta, tb, tc;
     maize_status_t st;

@@ -148,7 +148,11 @@ def close(out, ref, size, k, what=""):
 
 SHAPES = [(1, 1, 16), (1, 128, 128), (16, 256, 128), (128, 128, 256), (256, 256, 128), (257, 130, 144), (3, 1000, 272),
           (130, 7, 1024), (300, 520, 2064), (64, 384, 128 * 13), (1030, 776, 400), (2500, 2304, 256), (33, 4096, 512),
-          (5, 9000, 256), (16, 300, 4096)]
+          (5, 9000, 256), (16, 300, 4096),
+          # K over two or four CTAs: one, few and many rows of A, tiles that touch two scale blocks, K not cut evenly
+          (1, 4096, 4096), (16, 512, 8192), (17, 500, 2064), (32, 9001, 1040), (33, 700, 8192), (64, 1001, 4096), (65, 1000, 1024),
+          (128, 520, 8192), (100, 1001, 4112), (129, 1000, 4000), (300, 1001, 4000), (500, 77, 8192), (1000, 64, 2048),
+          (16, 16384, 256), (127, 20000, 128)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)

@@ -1,0 +1,130 @@
+"""CPU tests of the host side of the grouped and 8-bit calls: what the binding hands to the C entry points, what it refuses
+before it hands anything over, and what the C entry points refuse without a context.  No GPU: the library is replaced by a
+recorder, and the context's "device" is the one torch reports for CPU tensors."""
+import sys
+
+import pytest
+import torch
+
+import maize_b200
+from maize_b200 import _ffi
+
+BF16, F8 = torch.bfloat16, torch.float8_e4m3fn
+
+
+class Recorder:
+    """Takes any entry point's place and keeps the arguments of the last call."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def entry(*args):
+            self.calls.append((name, args))
+            return _ffi.OK
+        return entry
+
+
+@pytest.fixture
+def ctx():
+    sys.modules["maize_b200.gemm"]._types()
+    c = maize_b200.Context.__new__(maize_b200.Context)
+    c._lib, c._h, c.device = Recorder(), None, -1
+    c._new = lambda shape, dtype, stream: torch.empty(shape, dtype=dtype)
+    return c
+
+
+def t(*shape, dtype=BF16):
+    return torch.zeros(shape, dtype=dtype)
+
+
+def offs(*values):
+    return torch.tensor(values, dtype=torch.int32)
+
+
+def test_grouped_arguments(ctx):
+    a, b, o = t(10, 32)[:, :16], t(3, 24, 40)[:, :, :16], offs(0, 4, 4, 9)
+    out = ctx.grouped_gemm(a, b, o, stream=7)
+    name, args = ctx._lib.calls[-1]
+    assert name == "maize_grouped_gemm_bf16" and out.shape == (10, 24) and out.dtype == BF16
+    assert args == (None, a.data_ptr(), 32, b.data_ptr(), 40, 24 * 40, out.data_ptr(), 24, o.data_ptr(), 3, 10, 24, 16, 7)
+    b = t(3, 16, 24)
+    out = ctx.grouped_gemm_kn(a, b, o, out=t(10, 30)[:, :24], stream=7)
+    name, args = ctx._lib.calls[-1]
+    assert name == "maize_grouped_gemm_bf16_kn"
+    assert args == (None, a.data_ptr(), 32, b.data_ptr(), 24, 16 * 24, out.data_ptr(), 30, o.data_ptr(), 3, 10, 24, 16, 7)
+    dc = t(10, 24)
+    out = ctx.grouped_gemm_wgrad(a, dc, o, stream=7)
+    name, args = ctx._lib.calls[-1]
+    assert name == "maize_grouped_gemm_bf16_wgrad" and out.shape == (3, 24, 16)
+    assert args == (None, a.data_ptr(), 32, dc.data_ptr(), 24, out.data_ptr(), 16, 24 * 16, o.data_ptr(), 3, 10, 24, 16, 7)
+
+
+def test_strides_of_single_rows_do_not_matter(ctx):
+    """torch may report any stride for a dimension of one."""
+    a = torch.as_strided(t(64), (1, 13), (3, 1))
+    b = torch.as_strided(t(128), (1, 13, 8), (1, 8, 1))
+    ctx.grouped_gemm_kn(a, b, offs(0, 1), stream=7)
+    args = ctx._lib.calls[-1][1]
+    assert args[2] == 16 and args[4] == 8  # pitches that the loads can take
+    a, s = torch.as_strided(t(64, dtype=F8), (1, 32), (1, 1)), torch.as_strided(t(8, dtype=torch.float32), (1, 1), (5, 1))
+    ctx.gemm_e4m3(a, s, a, s, stream=7)
+    args = ctx._lib.calls[-1][1]
+    assert args[2] == 32 and args[4] == 1 and args[6] == 32 and args[8] == 1
+
+
+def test_e4m3_arguments(ctx):
+    x = t(5, 300)
+    q, s = ctx.quantize_e4m3(x, stream=7)
+    assert q.shape == (5, 300) and q.dtype == F8 and s.shape == (5, 3) and s.dtype == torch.float32
+    assert ctx._lib.calls[-1] == ("maize_quantize_e4m3", (None, x.data_ptr(), 300, 5, 300, 1, q.data_ptr(), 300, s.data_ptr(), 3, 7))
+    q, s = ctx.quantize_e4m3(t(300, 129), 128, stream=7)
+    assert s.shape == (3, 2)
+    a, b, sa, sb = t(5, 272, dtype=F8), t(200, 272, dtype=F8), t(5, 3, dtype=torch.float32), t(2, 3, dtype=torch.float32)
+    c = ctx.gemm_e4m3(a, sa, b, sb, stream=7)
+    assert ctx._lib.calls[-1] == ("maize_gemm_e4m3", (None, a.data_ptr(), 272, sa.data_ptr(), 3, b.data_ptr(), 272, sb.data_ptr(), 3,
+                                                      c.data_ptr(), 200, 5, 200, 272, 7))
+
+
+def test_refused_before_the_library_is_called(ctx):
+    a, b, o, f32 = t(10, 16), t(2, 24, 16), offs(0, 4, 10), torch.float32
+    qa, sa, qb, sb = t(10, 256, dtype=F8), t(10, 2, dtype=f32), t(200, 256, dtype=F8), t(2, 2, dtype=f32)
+    bad = [
+        lambda: ctx.grouped_gemm(a, t(2, 24, 8), o), lambda: ctx.grouped_gemm(a, t(3, 24, 16), o),
+        lambda: ctx.grouped_gemm(a, b, o.long()), lambda: ctx.grouped_gemm(a.float(), b, o),
+        lambda: ctx.grouped_gemm(a, t(24, 16), o), lambda: ctx.grouped_gemm(t(16, 10).T, b, o),
+        lambda: ctx.grouped_gemm(a, b, o, out=t(10, 23)), lambda: ctx.grouped_gemm(a, b, o, out=t(10, 24, dtype=f32)),
+        lambda: ctx.grouped_gemm(a, b, torch.stack([o, o], 1)[:, 0]), lambda: ctx.grouped_gemm(a, b, o[None]),
+        lambda: ctx.grouped_gemm_kn(a, b, o),
+        lambda: ctx.grouped_gemm_wgrad(a, t(9, 24), o), lambda: ctx.grouped_gemm_wgrad(a, t(10, 24), o[:0]),
+        lambda: ctx.grouped_gemm_wgrad(a, t(10, 24), o, out=t(2, 16, 24)), lambda: ctx.grouped_gemm_wgrad(a, t(10, 24), o[None]),
+        lambda: ctx.quantize_e4m3(a, 64), lambda: ctx.quantize_e4m3(a.float()), lambda: ctx.quantize_e4m3(t(16, 10).T),
+        lambda: ctx.quantize_e4m3(a, out=t(10, 16)), lambda: ctx.quantize_e4m3(a, scales=t(10, 2, dtype=f32)),
+        lambda: ctx.gemm_e4m3(qa, sa, qb[:, :128], sb), lambda: ctx.gemm_e4m3(qa, sa[:9], qb, sb),
+        lambda: ctx.gemm_e4m3(qa, sa, qb, sb[:1]), lambda: ctx.gemm_e4m3(qa.view(torch.uint8), sa, qb, sb),
+        lambda: ctx.gemm_e4m3(qa, sa.double(), qb, sb), lambda: ctx.gemm_e4m3(qa, sa, qb, sb, out=t(10, 199)),
+    ]
+    for call in bad:
+        with pytest.raises(maize_b200.MaizeError) as e:
+            call()
+        assert e.value.status == _ffi.INVALID_ARG
+    assert ctx._lib.calls == []
+
+
+def test_module_functions_refuse_cpu_tensors():
+    a = t(4, 16)
+    for call in (lambda: maize_b200.grouped_gemm(a, t(1, 8, 16), offs(0, 4)), lambda: maize_b200.quantize_e4m3(a),
+                 lambda: maize_b200.grouped_gemm_wgrad(a, a, offs(0, 4)),
+                 lambda: maize_b200.gemm_e4m3(a.to(F8), t(4, 1), a.to(F8), t(1, 1))):
+        with pytest.raises(maize_b200.MaizeError) as e:
+            call()
+        assert e.value.status == _ffi.INVALID_ARG
+
+
+def test_null_context_is_rejected():
+    lib = _ffi.load()
+    assert lib.maize_grouped_gemm_bf16(None, None, 8, None, 8, 64, None, 8, None, 1, 1, 8, 8, None) == _ffi.INVALID_ARG
+    assert lib.maize_grouped_gemm_bf16_kn(None, None, 8, None, 8, 64, None, 8, None, 1, 1, 8, 8, None) == _ffi.INVALID_ARG
+    assert lib.maize_grouped_gemm_bf16_wgrad(None, None, 8, None, 8, None, 8, 64, None, 1, 1, 8, 8, None) == _ffi.INVALID_ARG
+    assert lib.maize_quantize_e4m3(None, None, 8, 1, 8, 1, None, 8, None, 1, None) == _ffi.INVALID_ARG
+    assert lib.maize_gemm_e4m3(None, None, 16, None, 1, None, 16, None, 1, None, 8, 1, 8, 16, None) == _ffi.INVALID_ARG
