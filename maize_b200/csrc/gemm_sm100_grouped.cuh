@@ -58,7 +58,6 @@ struct GroupTable {
 };
 constexpr uint32_t kGroupTableBytes = 2 * 4 * (kGroupedMaxGroups + 4);
 
-__device__ __forceinline__ uint32_t row_tiles(uint32_t rows) { return (rows + kGroupedTileRows - 1) / kGroupedTileRows; }
 
 // Whole CTA.  Reads the offsets (into shared memory if `to` is given) and checks them: offsets that do not ascend, or leave
 // [0, rows], are reported as MAIZE_ERR_DEVICE_ABORT and the answer is false.
@@ -84,6 +83,7 @@ __device__ __forceinline__ bool load_offsets(const GroupedParams &p, uint32_t *t
 
 // Whole CTA.  Reads the offsets into shared memory and counts the row tiles before each group; false if they
 // are not right (there are no tiles then).
+template <uint32_t TILE_ROWS = kGroupedTileRows>
 __device__ __forceinline__ bool build_group_table(const GroupedParams &p, const GroupTable &t)
 {
     if (!load_offsets(p, t.offset))
@@ -92,7 +92,7 @@ __device__ __forceinline__ bool build_group_table(const GroupedParams &p, const 
         uint32_t total = 0;
         for (uint32_t base = 0; base < p.groups; base += 32) {
             const uint32_t g = base + threadIdx.x;
-            const uint32_t mine = g < p.groups ? row_tiles(t.offset[g + 1] - t.offset[g]) : 0u;
+            const uint32_t mine = g < p.groups ? (t.offset[g + 1] - t.offset[g] + TILE_ROWS - 1) / TILE_ROWS : 0u;
             uint32_t sum = mine;
 #pragma unroll
             for (uint32_t d = 1; d < 32; d <<= 1) {
@@ -122,6 +122,7 @@ struct GroupedTile {
 
 // Tile `t` of the launch; `g` is the role's cursor over the groups (tiles come in ascending order).  Within a group the
 // row tiles of one block of weights follow each other, so that the weights are read from HBM once.
+template <uint32_t UNIT = kGroupedRowUnit>
 __device__ __forceinline__ GroupedTile grouped_tile(uint64_t t, uint32_t n_blocks, const GroupTable &tab, uint32_t &g)
 {
     while (t >= static_cast<uint64_t>(tab.first[g + 1]) * n_blocks)
@@ -132,7 +133,7 @@ __device__ __forceinline__ GroupedTile grouped_tile(uint64_t t, uint32_t n_block
     const uint32_t local = static_cast<uint32_t>(t - static_cast<uint64_t>(tab.first[g]) * n_blocks);
     const uint32_t tb = local % nt;
     // near-equal tiles: ceil(rows / nt) rounded up to the unit; 256 * (nt - 1) < rows leaves rows for the last one
-    const uint32_t per = ((rows + nt - 1) / nt + kGroupedRowUnit - 1) / kGroupedRowUnit * kGroupedRowUnit;
+    const uint32_t per = ((rows + nt - 1) / nt + UNIT - 1) / UNIT * UNIT;
     GroupedTile r;
     r.group = g;
     r.n_blk = local / nt;

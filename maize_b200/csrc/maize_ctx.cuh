@@ -60,6 +60,7 @@ struct maize_ctx {
     uint32_t tma_store = 1;       // tiled kernels: C through shared memory and TMA stores when its rows are 16-byte aligned
     uint32_t serpentine = 1;      // odd groups of row-blocks sweep the column-blocks backwards
     uint32_t tma_promotion = 3;   // CUtensorMapL2promotion of the operand maps: 0 none, 1 64 B, 2 128 B, 3 256 B
+    uint32_t k_parts = 0;         // CTAs that share a tile's K in the grouped and e4m3 products; 0 = by size
     uint32_t tail_split = 1;      // split the last partial round of pair tiles along K when pairs would idle
     uint32_t chain_stagger = 1;   // two lanes on a source that is all there: offset them by half a chunk
     uint32_t chain_streams = 2;   // 2: maize_chain_forward alternates chunks between the caller's stream and a helper

@@ -210,11 +210,11 @@ maize_status_t maize_gemm_e4m3(maize_ctx_t *ctx, const void *a, uint64_t lda, co
     const uint32_t ctas = maize::persistent_grid(ctx, 0xffffffffull, 1), kb = static_cast<uint32_t>(kblocks);
     SkinnyPlan plan = skinny_plan(ctas, 2, m, n, kb);
     const SkinnyPlan four = skinny_plan(ctas, 4, m, n, kb);
-    if (four.cost < plan.cost)
+    if (ctx->k_parts == 0 ? four.cost < plan.cost : ctx->k_parts >= 4)
         plan = four;
     const uint64_t pair_tiles = ((uint64_t(m) + 255) / 256) * ((uint64_t(n) + 255) / 256), pairs = ctas / 2 ? ctas / 2 : 1;
     const double pair_cost = double((pair_tiles + pairs - 1) / pairs) * (kb * 0.55 + 1.5);
-    if (m <= 128 || plan.cost < pair_cost)
+    if (ctx->k_parts == 0 ? (m <= 128 || plan.cost < pair_cost) : ctx->k_parts != 1)
         return skinny(ctx, plan, a, lda, static_cast<const float *>(a_scales), ld_a_scales, b, ldb, static_cast<const float *>(b_scales),
                       ld_b_scales, c, ldc, m, n, k, stream);
     CUtensorMap ta, tb, tc;

@@ -7,6 +7,7 @@
 
 #include "maize_host.cuh"
 #include "gemm_sm100_grouped.cuh"
+#include "gemm_sm100_grouped_split.cuh"
 #include "gemm_sm100_grouped_wgrad.cuh"
 
 namespace {
@@ -39,6 +40,50 @@ maize_status_t check_groups(maize_ctx_t *ctx, const void *offsets, uint32_t grou
 bool stack_ok(uint32_t count, uint64_t stride, uint64_t rows, uint64_t cols, uint64_t ld)
 {
     return count <= 1 || rows == 0 || stride >= (rows - 1) * ld + cols;
+}
+
+// Clusters of `parts` CTAs at a time: those of four and eight fit only within a GPC.
+uint32_t clusters_of(const maize_ctx_t *ctx, uint32_t parts)
+{
+    const uint32_t ctas = persistent_grid(ctx, 0xffffffffull, 1);
+    const uint32_t c = parts == 2 ? ctas / 2 : (parts == 4 ? ctas * 32 / 148 : ctas * 16 / 148);
+    return c ? c : 1;
+}
+
+// CTAs that share a tile's K, or 1 for the kernel that gives a pair whole tiles.  Both are reckoned with the most tiles that
+// the rows can make; a k-block costs about 0.3 us either way, a tile's end 1 us, and 2 to 3 us where the parts meet.
+// Eight rows for five experts, 144 x 6936: 8 us in eight parts, 35 whole; 39 rows for one, 4096 x 4096: 10.6 in four parts, 20
+// in eight (two rounds), 22 whole; 32 rows for 16 experts, 4096 x 2048: 48 in two parts, 65 in four, 46 to 50 whole.
+uint32_t split_parts(const maize_ctx_t *ctx, uint32_t rows, uint32_t groups, uint32_t n, uint32_t k)
+{
+    if (ctx->k_parts != 0)
+        return ctx->k_parts;
+    const uint64_t with_rows = rows < groups ? rows : groups, kb = (uint64_t(k) + 63) / 64;
+    auto rounds = [](uint64_t tiles, uint64_t at_a_time) { return double((tiles + at_a_time - 1) / at_a_time); };
+    const uint64_t pair_tiles = (rows / maize::kGroupedTileRows + with_rows) * ((uint64_t(n) + 255) / 256);
+    double best = rounds(pair_tiles, clusters_of(ctx, 2)) * (kb * 0.3 + 1.0);
+    const uint64_t tiles = (rows / maize::kSplitTileRows + with_rows) * ((uint64_t(n) + 127) / 128);
+    uint32_t parts = 1;
+    for (uint32_t s = 2; s <= 8; s *= 2) {
+        const double cost = rounds(tiles, clusters_of(ctx, s)) * ((kb + s - 1) / s * 0.3 + (s == 2 ? 2.0 : (s == 4 ? 2.5 : 3.0)));
+        if (cost < best) {
+            best = cost;
+            parts = s;
+        }
+    }
+    return parts;
+}
+
+template <bool W_KN, uint32_t S, uint32_t STAGES>
+maize_status_t launch_split(maize_ctx_t *ctx, const maize::RowMaps &ta, const CUtensorMap &tw, const GroupedParams &p,
+                            cudaStream_t stream)
+{
+    const uint64_t tiles = (p.rows / maize::kSplitTileRows + uint64_t(p.rows < p.groups ? p.rows : p.groups)) *
+                           ((uint64_t(p.n) + maize::kSplitTileCols - 1) / maize::kSplitTileCols);
+    const uint32_t most = clusters_of(ctx, S), clusters = tiles < most ? static_cast<uint32_t>(tiles) : most;
+    const int slot = maize::kAttrGroupedSplit + (W_KN ? 3 : 0) + (S == 2 ? 0 : (S == 4 ? 1 : 2));
+    return maize::launch_clusters(ctx, slot, maize::gemm_bf16_sm100_grouped_split<W_KN, S, STAGES>, clusters * S, S,
+                                  maize::kNumThreads, maize::GroupedSplitLayout<S, STAGES>::kDynamicBytes, stream, ta, tw, p);
 }
 
 maize_status_t grouped_impl(maize_ctx_t *ctx, const void *a, uint64_t lda, const void *b, uint64_t ldb, uint64_t b_stride,
@@ -95,9 +140,11 @@ maize_status_t grouped_impl(maize_ctx_t *ctx, const void *a, uint64_t lda, const
     if (lda * 2 >= (1ull << 40) || ldb * 2 >= (1ull << 40) || b_stride * 2 >= (1ull << 40))
         return fail(ctx, MAIZE_ERR_UNSUPPORTED, "pitch beyond the TMA limit of 2^40 bytes");
 
-    // a CTA brings in half a tile's rows: no box is used that is longer than half of all rows, rounded up
+    const uint32_t parts = split_parts(ctx, rows, groups, n, k);
+    // the boxes that tiles of these rows can need: a CTA of a pair brings in half a tile's rows, one of a split tile all
+    const uint32_t longest = parts > 1 ? rows : (rows + 31) / 32 * 16;
     maize::RowMaps ta = {};
-    for (uint32_t i = 0; i < 4 && (i == 0 || (8u << i) < (rows + 31) / 32 * 16); ++i)
+    for (uint32_t i = 0; i < (parts > 1 ? 3u : 4u) && (i == 0 || (8u << i) < longest); ++i)
         if ((st = matrix_map(ctx, &ta.box[i], a, rows, k, lda, 16u << i)) != MAIZE_OK)
             return st;
     CUtensorMap tw;
@@ -106,6 +153,12 @@ maize_status_t grouped_impl(maize_ctx_t *ctx, const void *a, uint64_t lda, const
               : stack_map(ctx, &tw, b, groups, n, k, ldb, b_stride, maize::kBlockM, promotion);
     if (st != MAIZE_OK)
         return st;
+    if (parts == 8)
+        return b_kn ? launch_split<true, 8, 7>(ctx, ta, tw, p, stream) : launch_split<false, 8, 7>(ctx, ta, tw, p, stream);
+    if (parts == 4)
+        return b_kn ? launch_split<true, 4, 7>(ctx, ta, tw, p, stream) : launch_split<false, 4, 7>(ctx, ta, tw, p, stream);
+    if (parts == 2)
+        return b_kn ? launch_split<true, 2, 7>(ctx, ta, tw, p, stream) : launch_split<false, 2, 7>(ctx, ta, tw, p, stream);
 
     // rows of C that TMA can store (N has to end on a 16-byte piece, see the weight gradient)
     CUtensorMap tc;

@@ -740,7 +740,7 @@ maize_status_t maize_ctx_create(int device, maize_ctx_t **out)
     ctx->repack_bytes = kDefaultRepackBytes;
     // MAIZE_<KEY>=<integer> in the environment presets a tunable of every context (same keys as maize_ctx_set)
     static const char *const kEnvKeys[] = {"pdl", "tma_store", "wide_tile", "wide_max_gflop", "c_evict_first", "serpentine", "tail_split", "group_rows", "tma_promotion",
-                                           "chain_streams", "chain_stagger", "b_static", "timeout_ns", "max_ctas"};
+                                           "chain_streams", "chain_stagger", "b_static", "timeout_ns", "max_ctas", "k_parts"};
     for (const char *key : kEnvKeys) {
         std::string name = "MAIZE_";
         for (const char *c = key; *c; ++c)
@@ -1091,6 +1091,10 @@ maize_status_t maize_ctx_set(maize_ctx_t *ctx, const char *key, int64_t value)
         if (value < 1 || value > static_cast<int64_t>(kMaxChainLanes))
             return fail(ctx, MAIZE_ERR_INVALID_ARG, "chain_streams: 1 to 4");
         ctx->chain_streams = static_cast<uint32_t>(value);
+    } else if (!strcmp(key, "k_parts")) {
+        if (value != 0 && value != 1 && value != 2 && value != 4 && value != 8)
+            return fail(ctx, MAIZE_ERR_INVALID_ARG, "k_parts must be 0 (by size), 1, 2, 4 or 8");
+        ctx->k_parts = static_cast<uint32_t>(value);
     } else if (!strcmp(key, "push_threads")) {
         if (value < 32 || value > 512 || value % 32 != 0)
             return fail(ctx, MAIZE_ERR_INVALID_ARG, "push_threads: a multiple of 32 in [32, 512]");
@@ -1140,6 +1144,8 @@ maize_status_t maize_ctx_get(const maize_ctx_t *ctx, const char *key, int64_t *v
         *value = ctx->chain_streams;
     else if (!strcmp(key, "chain_stagger"))
         *value = ctx->chain_stagger;
+    else if (!strcmp(key, "k_parts"))
+        *value = ctx->k_parts;
     else if (!strcmp(key, "tail_split"))
         *value = ctx->tail_split;
     else if (!strcmp(key, "serpentine"))

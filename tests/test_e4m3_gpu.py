@@ -155,8 +155,20 @@ SHAPES = [(1, 1, 16), (1, 128, 128), (16, 256, 128), (128, 128, 256), (256, 256,
           (16, 16384, 256), (127, 20000, 128)]
 
 
+@pytest.fixture
+def parts(ctx, request):
+    """The number of CTAs that share a tile's K, forced for a test."""
+    ctx.set("k_parts", request.param)
+    yield request.param
+    ctx.set("k_parts", 0)
+
+
+EVERY_KERNEL = pytest.mark.parametrize("parts", [0, 1, 2, 4], indirect=True)
+
+
+@EVERY_KERNEL
 @pytest.mark.parametrize("m,n,k", SHAPES)
-def test_product_sizes(ctx, m, n, k):
+def test_product_sizes(ctx, m, n, k, parts):
     a, sa, b, sb = operands(m + n + k, m, n, k)
     out = ctx.gemm_e4m3(a, sa, b, sb)
     ctx.poll()
@@ -164,9 +176,10 @@ def test_product_sizes(ctx, m, n, k):
     close(out, ref, size, k, f"{m} x {n} x {k}")
 
 
+@EVERY_KERNEL
 @pytest.mark.parametrize("m", [5, 40, 200])
 @pytest.mark.parametrize("n,pad", [(264, 8), (264, 6), (257, 7), (257, 3), (100, 4)])
-def test_product_strided(ctx, m, n, pad):
+def test_product_strided(ctx, m, n, pad, parts):
     """Padded operands, scales and result; nothing around C is touched."""
     import torch
     k = 272
@@ -185,8 +198,9 @@ def test_product_strided(ctx, m, n, pad):
     assert (buf == 7).all()
 
 
-@pytest.mark.parametrize("m", [7, 300])
-def test_nan_stays_in_its_row_and_column(ctx, m):
+@EVERY_KERNEL
+@pytest.mark.parametrize("m", [7, 50, 300])
+def test_nan_stays_in_its_row_and_column(ctx, m, parts):
     import torch
     n, k = 300, 272
     a, sa, b, sb = operands(6, m, n, k)
@@ -201,8 +215,9 @@ def test_nan_stays_in_its_row_and_column(ctx, m):
     assert torch.equal(bad, want)
 
 
+@EVERY_KERNEL
 @pytest.mark.parametrize("m", [2, 300])
-def test_extreme_scales(ctx, m):
+def test_extreme_scales(ctx, m, parts):
     """Scales far from one, and zeros, in single blocks."""
     import torch
     n, k = 200, 512

@@ -78,31 +78,48 @@ SIZES = [
 ]
 
 
+@pytest.fixture
+def parts(ctx, request):
+    """The number of CTAs that share a tile's K, forced for a test."""
+    ctx.set("k_parts", request.param)
+    yield request.param
+    ctx.set("k_parts", 0)
+
+
+EVERY_KERNEL = pytest.mark.parametrize("parts", [0, 1, 2, 4, 8], indirect=True)
+
+
+@EVERY_KERNEL
 @pytest.mark.parametrize("kn", [False, True])
 @pytest.mark.parametrize("sizes", SIZES, ids=lambda s: "-".join(map(str, s[:7])))
-def test_group_sizes(ctx, sizes, kn):
+def test_group_sizes(ctx, sizes, kn, parts):
     check_grouped(ctx, sizes, 520, 264, kn)
 
 
+@EVERY_KERNEL
 @pytest.mark.parametrize("kn", [False, True])
 @pytest.mark.parametrize("n,k", [(8, 8), (256, 64), (256, 384), (40, 8), (264, 520), (2048, 72), (512, 2056), (136, 64 * 21)])
-def test_matrix_sizes(ctx, n, k, kn):
+def test_matrix_sizes(ctx, n, k, kn, parts):
     check_grouped(ctx, [5, 300, 0, 33], n, k, kn, seed=2)
 
 
+@EVERY_KERNEL
 @pytest.mark.parametrize("n", [1, 7, 31, 33, 257, 1031])
-def test_odd_result_rows(ctx, n):
+def test_odd_result_rows(ctx, n, parts):
     """C needs no alignment: odd N, where B is N x K."""
     check_grouped(ctx, [5, 70, 0, 33], n, 136, False, seed=3)
 
 
+@EVERY_KERNEL
 @pytest.mark.parametrize("k", [1, 3, 63, 65, 127])
-def test_any_k_where_b_is_k_by_n(ctx, k):
+def test_any_k_where_b_is_k_by_n(ctx, k, parts):
     """K x N matrices: K is free as long as the rows' pitch is a multiple of 8."""
     import torch
     g = gen(4)
     sizes, n = [9, 0, 40], 72
-    a = bf16(g, (49, 128))[:, :k]
+    a = bf16(g, (49, 128))
+    a[:, k:] = float("nan")  # what lies behind a row's end takes no part
+    a = a[:, :k]
     w = bf16(g, (3, k, n), 0.1)
     o = offsets_of(sizes)
     out = ctx.grouped_gemm_kn(a, w, o)
@@ -111,14 +128,16 @@ def test_any_k_where_b_is_k_by_n(ctx, k):
     close(out, ref, size, k)
 
 
+@EVERY_KERNEL
 @pytest.mark.parametrize("kn", [False, True])
-def test_rows_outside_the_groups_stay(ctx, kn):
+def test_rows_outside_the_groups_stay(ctx, kn, parts):
     check_grouped(ctx, [30, 0, 41], 256, 128, kn, seed=5, first=3, behind=500)
     check_grouped(ctx, [0, 0], 256, 128, kn, seed=5, first=2, behind=9)
 
 
+@EVERY_KERNEL
 @pytest.mark.parametrize("kn", [False, True])
-def test_other_groups_values_do_not_leak(ctx, kn):
+def test_other_groups_values_do_not_leak(ctx, kn, parts):
     """One group's rows or weights are NaN or infinite: the other groups' results do not change."""
     import torch
     g = gen(6)
@@ -136,8 +155,9 @@ def test_other_groups_values_do_not_leak(ctx, kn):
     assert not torch.isfinite(out[70:120].float()).any()
 
 
+@EVERY_KERNEL
 @pytest.mark.parametrize("kn", [False, True])
-def test_strided_operands(ctx, kn):
+def test_strided_operands(ctx, kn, parts):
     """Padded rows of A, C and the weights, and matrices with a gap between them; nothing around C is touched."""
     import torch
     g = gen(7)
@@ -161,6 +181,20 @@ def test_strided_operands(ctx, kn):
 @pytest.mark.parametrize("kn", [False, True])
 def test_large_ragged(ctx, kn):
     check_grouped(ctx, [1000, 17, 0, 2100, 300, 5, 689], 2056, 1032, kn, seed=8)
+
+
+@EVERY_KERNEL
+def test_many_tiles_per_cta(ctx, parts):
+    """More tiles than clusters: accumulator buffers, the exchange and their phases go round."""
+    check_grouped(ctx, [200, 3, 0, 129, 64] * 4, 1032, 328, False, seed=9)
+    check_grouped(ctx, [70] * 40, 776, 72, True, seed=10)
+
+
+@pytest.mark.parametrize("sizes", [[8], [2, 2, 2, 1, 1], [26, 26, 26], [0, 0, 1, 0]])
+def test_few_rows_long_k(ctx, sizes):
+    """The sizes that K is split for by itself."""
+    check_grouped(ctx, sizes, 144, 6936, False, seed=11)
+    check_grouped(ctx, sizes, 144, 6936, True, seed=12)
 
 
 def test_empty_sum_clears_the_groups_rows(ctx):
