@@ -11,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -18,6 +19,9 @@ CSRC = PKG / "csrc"
 OUT = PKG / "_lib" / "libmaize_gemm.so"
 SOURCES = [CSRC / "maize_gemm.cu", CSRC / "maize_mgpu.cu", CSRC / "maize_experts.cu",
            CSRC / "maize_e4m3.cu"]
+# Python callables for the host-bound entry points, linked to the library beside it
+CALLS_SOURCE = CSRC / "calls.c"
+CALLS_OUT = OUT.with_name("maize_calls" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 DEPENDS = sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + [PKG.parent / "include" / "maize_gemm.h"]
 
 NVCC_FLAGS = [
@@ -39,7 +43,7 @@ def is_stale() -> bool:
     if not OUT.exists():
         return True
     t = OUT.stat().st_mtime
-    return any(d.stat().st_mtime > t for d in DEPENDS if d.exists())
+    return any(d.stat().st_mtime > t for d in (*DEPENDS, CALLS_SOURCE) if d.exists())
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -53,7 +57,24 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         sys.stderr.write(proc.stdout + proc.stderr)
     if proc.returncode != 0:
         raise RuntimeError("nvcc failed building libmaize_gemm.so")
+    build_calls()
     return OUT
+
+
+def build_calls() -> None:
+    """Builds ``csrc/calls.c``.  Where Python's headers or a C compiler are missing the binding calls through ctypes."""
+    include = sysconfig.get_paths()["include"]
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None or not Path(include, "Python.h").exists():
+        sys.stderr.write("maize_b200: no C compiler or Python.h, calls go through ctypes\n")
+        CALLS_OUT.unlink(missing_ok=True)
+        return
+    cmd = [cc, "-O2", "-Wall", "-shared", "-fPIC", f"-I{include}", "-o", str(CALLS_OUT), str(CALLS_SOURCE), f"-L{OUT.parent}",
+           f"-l:{OUT.name}", "-Wl,-rpath,$ORIGIN"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        sys.stderr.write(proc.stdout + proc.stderr)
+        raise RuntimeError("the C compiler failed building calls.c")
 
 
 if __name__ == "__main__":

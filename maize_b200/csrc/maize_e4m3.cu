@@ -76,6 +76,8 @@ maize_status_t skinny(maize_ctx_t *ctx, const SkinnyPlan &plan, const void *a, u
                       uint32_t k, cudaStream_t stream)
 {
     const uint32_t bn = plan.bn;
+    if (uint64_t(plan.tiles_m) * ((uint64_t(n) + bn - 1) / bn) > 0x7fffffffull)
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "too many output tiles");
     maize::F8SkinnyParams f = {};
     f.g.c = static_cast<__nv_bfloat16 *>(c);
     f.g.ldc = ldc;

@@ -672,7 +672,7 @@ maize_status_t gemm_impl(maize_ctx_t *ctx, const void *a, uint64_t lda, const vo
 
 extern "C" {
 
-int maize_version(void) { return 100; }
+int maize_version(void) { return 200; }
 
 const char *maize_status_string(maize_status_t s)
 {

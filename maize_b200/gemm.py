@@ -56,15 +56,18 @@ def _stream_handle(stream) -> Optional[int]:
 
 _torch = None
 _raw_stream = None
+_devices = ()
 
 
 def _types():
-    """The torch module (imported with the first call that has tensors to look at), and the shortest way to the current
-    stream's handle where this torch has it."""
-    global _torch, _raw_stream
+    """The torch module, imported with the first call that has tensors to look at; with it, torch's name of every device and
+    the shortest way to a device's current stream that this torch has."""
+    global _torch, _raw_stream, _devices
     if _torch is None:
         import torch
-        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda device: torch.cuda.current_stream(device).cuda_stream)
+        _devices = tuple(torch.device("cuda", i) for i in range(torch.cuda.device_count()))
         _torch = torch
     return _torch
 
@@ -79,13 +82,14 @@ class Context:
         if st != _ffi.OK:
             raise MaizeError(st, self._lib.maize_status_string(st).decode())
         self._h = handle
+        self._ctx = handle.value  # the same for the calls that do not go through ctypes
+        self._calls = _ffi.load_calls()
         self.device = int(device)
-        self._device = f"cuda:{self.device}"  # torch's name of it
 
     def close(self) -> None:
         if getattr(self, "_h", None):
             self._lib.maize_ctx_destroy(self._h)
-            self._h = None
+            self._h = self._ctx = None
 
     def __del__(self):
         try:
@@ -256,59 +260,60 @@ class Context:
         return out
 
     # ------------------------------------------- products grouped by expert --
-    # Small calls are bound by the host, so these checks take each property of a tensor once.
-    def _own(self, name: str, t, dims: int, dtype):
-        """The checks every operand of the calls below shares: kind, device, unit stride along the rows.  Returns the
-        strides."""
-        if t.dtype is dtype and t.dim() == dims and t.get_device() == self.device:
-            strides = t.stride()
-            if strides[-1] == 1 or t.shape[-1] <= 1:
-                return strides
-        raise MaizeError(_ffi.INVALID_ARG, f"{name}: expected a {dims}-D {dtype} tensor with unit column stride on "
-                                           f"cuda:{self.device}")
+    # Small calls are bound by the host: what every call asks of its tensors is asked once and in line, and _own is only
+    # there for those that fail it (or have a dimension of one with an odd stride).
+    def _own(self, name: str, t, dims: int, dtype) -> None:
+        """What every operand of the calls below is checked for: kind, device, unit stride along the rows."""
+        if (t.dtype is not dtype or t.dim() != dims or t.get_device() != self.device
+                or (t.shape[-1] > 1 and t.stride(-1) != 1)):
+            raise MaizeError(_ffi.INVALID_ARG, f"{name}: expected a {dims}-D {dtype} tensor with unit column stride on "
+                                               f"cuda:{self.device}")
+
+    def _result(self, out, shape, dtype, stream):
+        """The tensor a call writes: ``out`` if it is given and fits, else a new one, allocated for the
+        stream the call runs on."""
+        if out is not None:
+            self._own("out", out, len(shape), dtype)
+            if out.shape != shape:
+                raise MaizeError(_ffi.INVALID_ARG, f"out: expected {' x '.join(map(str, shape))}")
+            return out
+        if stream is None:
+            return _torch.empty(*shape, dtype=dtype, device=_devices[self.device])
+        if isinstance(stream, int):
+            stream = _torch.cuda.ExternalStream(stream, device=self.device)
+        with _torch.cuda.stream(stream):
+            return _torch.empty(*shape, dtype=dtype, device=_devices[self.device])
 
     def _stream(self, stream) -> int:
         """Handle of the stream a call runs on: the given one, or the current stream of the context's device."""
         if stream is None:
-            return _torch.cuda.current_stream(self.device).cuda_stream if _raw_stream is None else _raw_stream(self.device)
+            return _raw_stream(self.device)
         return stream if isinstance(stream, int) else stream.cuda_stream
 
-    def _new(self, shape, dtype, stream):
-        """An output tensor, allocated for the stream the call runs on."""
-        if stream is None:
-            return _torch.empty(*shape, dtype=dtype, device=self._device)
-        if isinstance(stream, int):
-            stream = _torch.cuda.ExternalStream(stream, device=self.device)
-        with _torch.cuda.stream(stream):
-            return _torch.empty(*shape, dtype=dtype, device=self._device)
-
-    def _offsets(self, offsets, groups: int) -> int:
-        if (offsets.dtype is _torch.int32 and offsets.dim() == 1 and offsets.numel() == groups + 1
-                and offsets.get_device() == self.device and offsets.is_contiguous()):
-            return offsets.data_ptr()
-        raise MaizeError(_ffi.INVALID_ARG, f"offsets: expected {groups + 1} contiguous int32 values on cuda:{self.device}")
+    def _offsets(self, offsets, groups: int) -> None:
+        if (offsets.dtype is not _torch.int32 or offsets.dim() != 1 or offsets.numel() != groups + 1
+                or offsets.get_device() != self.device or not offsets.is_contiguous()):
+            raise MaizeError(_ffi.INVALID_ARG, f"offsets: expected {groups + 1} contiguous int32 values on cuda:{self.device}")
 
     def _grouped(self, entry, a, b, offsets, out, stream, kn: bool):
-        bf16 = (_torch or _types()).bfloat16
-        sa, sb = self._own("a", a, 2, bf16), self._own("b", b, 3, bf16)
+        bf16, device = (_torch or _types()).bfloat16, self.device
+        sa, sb = a.stride(), b.stride()
+        if not (a.dtype is bf16 and b.dtype is bf16 and len(sa) == 2 and len(sb) == 3 and sa[1] == 1 and sb[2] == 1
+                and a.get_device() == device and b.get_device() == device):
+            self._own("a", a, 2, bf16)
+            self._own("b", b, 3, bf16)
         rows, k = a.shape
         groups, b_rows, b_cols = b.shape
         n, kb = (b_cols, b_rows) if kn else (b_rows, b_cols)
         if k != kb:
             raise MaizeError(_ffi.INVALID_ARG, f"a has {k} columns, the matrices of b a K of {kb}")
-        at = self._offsets(offsets, groups)
-        if out is None:
-            out = self._new((rows, n), bf16, stream)
-            ldc = n
-        else:
-            ldc = self._own("out", out, 2, bf16)[0]
-            if out.shape != (rows, n):
-                raise MaizeError(_ffi.INVALID_ARG, f"out: expected {rows} x {n}")
+        self._offsets(offsets, groups)
+        out = self._result(out, (rows, n), bf16, stream)
         # the stride of a dimension of one is not used and may be anything
-        st = entry(self._h, a.data_ptr(), sa[0] if rows > 1 else -(-k // 8) * 8, b.data_ptr(),
-                   sb[1] if b_rows > 1 else -(-b_cols // 8) * 8, sb[0], out.data_ptr(), ldc if rows > 1 else n, at,
-                   groups, rows, n, k, self._stream(stream))
-        if st != _ffi.OK:
+        st = entry(self._ctx, a.data_ptr(), sa[0] if rows > 1 else -(-k // 8) * 8, b.data_ptr(),
+                   sb[1] if b_rows > 1 else -(-b_cols // 8) * 8, sb[0], out.data_ptr(), out.stride(0) if rows > 1 else n,
+                   offsets.data_ptr(), groups, rows, n, k, self._stream(stream))
+        if st:
             self._check(st)
         return out
 
@@ -316,38 +321,37 @@ class Context:
         """``out[r] = a[r] @ b[g].T`` for the rows ``offsets[g] <= r < offsets[g + 1]`` of every group g: a is rows x K,
         b is groups x N x K (one weight matrix per expert), offsets int32 on the device, ascending, groups + 1 of them.
         Rows outside all groups are left as they were.  Groups may be empty; their sizes are never read on the host."""
-        return self._grouped(self._lib.maize_grouped_gemm_bf16, a, b, offsets, out, stream, False)
+        return self._grouped(self._calls.maize_grouped_gemm_bf16, a, b, offsets, out, stream, False)
 
     def grouped_gemm_kn(self, a, b, offsets, out=None, stream=None):
         """``out[r] = a[r] @ b[g]`` with b given groups x K x N.  With ``a`` the gradient of ``grouped_gemm``'s result and
         the same b this is the gradient of its input."""
-        return self._grouped(self._lib.maize_grouped_gemm_bf16_kn, a, b, offsets, out, stream, True)
+        return self._grouped(self._calls.maize_grouped_gemm_bf16_kn, a, b, offsets, out, stream, True)
 
     def grouped_gemm_wgrad(self, a, dc, offsets, out=None, stream=None):
         """``out[g] = dc[rows of g].T @ a[rows of g]``: the gradient of ``grouped_gemm``'s b (groups x N x K) from its
         input ``a`` (rows x K) and the gradient ``dc`` (rows x N) of its result.  A group without rows gets zeros."""
-        bf16 = (_torch or _types()).bfloat16
-        sa, sd = self._own("a", a, 2, bf16), self._own("dc", dc, 2, bf16)
+        bf16, device = (_torch or _types()).bfloat16, self.device
+        sa, sd = a.stride(), dc.stride()
+        if not (a.dtype is bf16 and dc.dtype is bf16 and len(sa) == 2 and len(sd) == 2 and sa[1] == 1 and sd[1] == 1
+                and a.get_device() == device and dc.get_device() == device):
+            self._own("a", a, 2, bf16)
+            self._own("dc", dc, 2, bf16)
         rows, k = a.shape
         rows_dc, n = dc.shape
         if rows_dc != rows:
             raise MaizeError(_ffi.INVALID_ARG, f"a has {rows} rows, dc {rows_dc}")
-        groups = offsets.shape[0] - 1 if offsets.dim() == 1 else -1
+        groups = offsets.numel() - 1
         if groups < 0:
             raise MaizeError(_ffi.INVALID_ARG, "offsets: expected groups + 1 int32 values")
-        at = self._offsets(offsets, groups)
-        if out is None:
-            out = self._new((groups, n, k), bf16, stream)
-            so = (n * k, k)
-        else:
-            so = self._own("out", out, 3, bf16)
-            if out.shape != (groups, n, k):
-                raise MaizeError(_ffi.INVALID_ARG, f"out: expected {groups} x {n} x {k}")
-        st = self._lib.maize_grouped_gemm_bf16_wgrad(
-            self._h, a.data_ptr(), sa[0] if rows > 1 else -(-k // 8) * 8, dc.data_ptr(),
-            sd[0] if rows > 1 else -(-n // 8) * 8, out.data_ptr(), so[1] if n > 1 else k, so[0], at, groups, rows, n, k,
-            self._stream(stream))
-        if st != _ffi.OK:
+        self._offsets(offsets, groups)
+        out = self._result(out, (groups, n, k), bf16, stream)
+        so = out.stride()
+        st = self._calls.maize_grouped_gemm_bf16_wgrad(
+            self._ctx, a.data_ptr(), sa[0] if rows > 1 else -(-k // 8) * 8, dc.data_ptr(),
+            sd[0] if rows > 1 else -(-n // 8) * 8, out.data_ptr(), so[1] if n > 1 else k, so[0], offsets.data_ptr(), groups, rows,
+            n, k, self._stream(stream))
+        if st:
             self._check(st)
         return out
 
@@ -356,29 +360,19 @@ class Context:
         """bf16 rows x cols -> (e4m3 tensor of the same shape, fp32 scales), with a power-of-two scale for each 1 x 128
         (``block_rows`` = 1: activations) or 128 x 128 block (``block_rows`` = 128: weights): ``x ~ q * scale``."""
         torch = _torch or _types()
-        sx = self._own("x", x, 2, torch.bfloat16)
+        sx = x.stride()
+        if not (x.dtype is torch.bfloat16 and len(sx) == 2 and sx[1] == 1 and x.get_device() == self.device):
+            self._own("x", x, 2, torch.bfloat16)
         rows, cols = x.shape
         if block_rows != 1 and block_rows != 128:
             raise MaizeError(_ffi.INVALID_ARG, "block_rows must be 1 or 128")
         down, across = -(-rows // block_rows), -(-cols // 128)
-        if out is None:
-            out = self._new((rows, cols), torch.float8_e4m3fn, stream)
-            ldq = cols
-        else:
-            ldq = self._own("out", out, 2, torch.float8_e4m3fn)[0]
-            if out.shape != (rows, cols):
-                raise MaizeError(_ffi.INVALID_ARG, f"out: expected {rows} x {cols}")
-        if scales is None:
-            scales = self._new((down, across), torch.float32, stream)
-            lds = across
-        else:
-            lds = self._own("scales", scales, 2, torch.float32)[0]
-            if scales.shape != (down, across):
-                raise MaizeError(_ffi.INVALID_ARG, f"scales: expected {down} x {across}")
-        st = self._lib.maize_quantize_e4m3(self._h, x.data_ptr(), sx[0] if rows > 1 else cols, rows, cols, block_rows,
-                                           out.data_ptr(), ldq if rows > 1 else cols, scales.data_ptr(),
-                                           lds if down > 1 else across, self._stream(stream))
-        if st != _ffi.OK:
+        out = self._result(out, (rows, cols), torch.float8_e4m3fn, stream)
+        scales = self._result(scales, (down, across), torch.float32, stream)
+        st = self._calls.maize_quantize_e4m3(self._ctx, x.data_ptr(), sx[0] if rows > 1 else cols, rows, cols, block_rows,
+                                             out.data_ptr(), out.stride(0) if rows > 1 else cols, scales.data_ptr(),
+                                             scales.stride(0) if down > 1 else across, self._stream(stream))
+        if st:
             self._check(st)
         return out, scales
 
@@ -386,9 +380,14 @@ class Context:
         """``out = (a * a_scales) @ (b * b_scales).T`` in bf16 for e4m3 a (M x K) with a scale for each 1 x 128 block
         (M x ceil(K/128), fp32) and e4m3 b (N x K) with one for each 128 x 128 block (ceil(N/128) x ceil(K/128))."""
         torch = _torch or _types()
-        f8, f32 = torch.float8_e4m3fn, torch.float32
-        sa, sb = self._own("a", a, 2, f8), self._own("b", b, 2, f8)
-        ssa, ssb = self._own("a_scales", a_scales, 2, f32), self._own("b_scales", b_scales, 2, f32)
+        f8, f32, device = torch.float8_e4m3fn, torch.float32, self.device
+        sa, sb, ssa, ssb = a.stride(), b.stride(), a_scales.stride(), b_scales.stride()
+        if not (a.dtype is f8 and b.dtype is f8 and a_scales.dtype is f32 and b_scales.dtype is f32
+                and len(sa) == 2 and len(sb) == 2 and len(ssa) == 2 and len(ssb) == 2
+                and sa[1] == 1 and sb[1] == 1 and ssa[1] == 1 and ssb[1] == 1 and a.get_device() == device
+                and b.get_device() == device and a_scales.get_device() == device and b_scales.get_device() == device):
+            for name, t, dtype in (("a", a, f8), ("b", b, f8), ("a_scales", a_scales, f32), ("b_scales", b_scales, f32)):
+                self._own(name, t, 2, dtype)
         m, k = a.shape
         n, kb = b.shape
         if k != kb:
@@ -396,18 +395,12 @@ class Context:
         blocks, down = -(-k // 128), -(-n // 128)
         if a_scales.shape != (m, blocks) or b_scales.shape != (down, blocks):
             raise MaizeError(_ffi.INVALID_ARG, f"scales: expected {m} x {blocks} for a, {down} x {blocks} for b")
-        if out is None:
-            out = self._new((m, n), torch.bfloat16, stream)
-            ldc = n
-        else:
-            ldc = self._own("out", out, 2, torch.bfloat16)[0]
-            if out.shape != (m, n):
-                raise MaizeError(_ffi.INVALID_ARG, f"out: expected {m} x {n}")
-        st = self._lib.maize_gemm_e4m3(self._h, a.data_ptr(), sa[0] if m > 1 else k, a_scales.data_ptr(),
-                                       ssa[0] if m > 1 else blocks, b.data_ptr(), sb[0] if n > 1 else k,
-                                       b_scales.data_ptr(), ssb[0] if down > 1 else blocks, out.data_ptr(),
-                                       ldc if m > 1 else n, m, n, k, self._stream(stream))
-        if st != _ffi.OK:
+        out = self._result(out, (m, n), torch.bfloat16, stream)
+        st = self._calls.maize_gemm_e4m3(self._ctx, a.data_ptr(), sa[0] if m > 1 else k, a_scales.data_ptr(),
+                                         ssa[0] if m > 1 else blocks, b.data_ptr(), sb[0] if n > 1 else k, b_scales.data_ptr(),
+                                         ssb[0] if down > 1 else blocks, out.data_ptr(), out.stride(0) if m > 1 else n, m, n, k,
+                                         self._stream(stream))
+        if st:
             self._check(st)
         return out
 

@@ -29,8 +29,11 @@ class Recorder:
 def ctx():
     sys.modules["maize_b200.gemm"]._types()
     c = maize_b200.Context.__new__(maize_b200.Context)
-    c._lib, c._h, c.device = Recorder(), None, -1
-    c._new = lambda shape, dtype, stream: torch.empty(shape, dtype=dtype)
+    c._lib = c._calls = Recorder()
+    c._h, c._ctx, c.device = None, None, -1
+    given = maize_b200.Context._result
+    c._result = lambda out, shape, dtype, stream: (torch.empty(shape, dtype=dtype) if out is None
+                                                   else given(c, out, shape, dtype, stream))
     return c
 
 
@@ -128,3 +131,18 @@ def test_null_context_is_rejected():
     assert lib.maize_grouped_gemm_bf16_wgrad(None, None, 8, None, 8, None, 8, 64, None, 1, 1, 8, 8, None) == _ffi.INVALID_ARG
     assert lib.maize_quantize_e4m3(None, None, 8, 1, 8, 1, None, 8, None, 1, None) == _ffi.INVALID_ARG
     assert lib.maize_gemm_e4m3(None, None, 16, None, 1, None, 16, None, 1, None, 8, 1, 8, 16, None) == _ffi.INVALID_ARG
+
+
+def test_compiled_calls_agree_with_ctypes():
+    """The compiled callables have the entry points' names and give their status codes."""
+    lib, calls = _ffi.load(), _ffi.load_calls()
+    if calls is lib:
+        pytest.skip("built without a C compiler or Python's headers")
+    for name in ("maize_grouped_gemm_bf16", "maize_grouped_gemm_bf16_kn", "maize_grouped_gemm_bf16_wgrad", "maize_quantize_e4m3",
+                 "maize_gemm_e4m3"):
+        count = len(_ffi.SYMBOLS[name][1])
+        assert getattr(calls, name)(*[None] * count) == getattr(lib, name)(*[None] + [0] * (count - 1)) == _ffi.INVALID_ARG
+        with pytest.raises(TypeError):
+            getattr(calls, name)(*[0] * (count - 1))
+        with pytest.raises(TypeError):
+            getattr(calls, name)(*["0"] * count)
