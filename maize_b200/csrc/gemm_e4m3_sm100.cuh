@@ -54,7 +54,7 @@ struct F8SmemLayout {
 // Stores 32 rows x 64 columns of C that lie in `stage` as 128-byte rows, 16-byte chunk j of row r at chunk j ^ (r & 7), to
 // rows of any alignment: a lane stores 4 bytes, so a row leaves as one run of 128.  Where a row starts between two words
 // the lanes pass on a half, and the ends of the run are 2-byte stores.  (2-byte stores throughout: 4111 x 3967 x 4112 in 125 us
-// instead of 88; with rows for TMA 75.)
+// instead of 81; with rows for TMA 75.)
 __device__ __forceinline__ void f8_store_rows(const GemmParams &p, uint32_t stage_u32, uint32_t lane, uint32_t row0, uint32_t col0)
 {
     const uint32_t rows = min(32u, p.m - row0);
@@ -64,26 +64,32 @@ __device__ __forceinline__ void f8_store_rows(const GemmParams &p, uint32_t stag
     if (rows == 32u && left >= 64u) {
         // every row the same way, but for whether it starts between two words: with an odd pitch every other one does
         const bool first = (reinterpret_cast<uintptr_t>(dst) & 2u) != 0u, odd_pitch = (p.ldc & 1u) != 0u;
+        __nv_bfloat16 *to = dst + 2u * lane;
 #pragma unroll 1
-        for (uint32_t r0 = 0; r0 < 32; r0 += 8) {
-            uint32_t v[8];
+        for (uint32_t r0 = 0; r0 < 32; r0 += 16) {
+            uint32_t v[16];
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i)
-                v[i] = ptx::ld_shared_u32(stage_u32 + (r0 + i) * 128u + ((chunk ^ i) << 4) + word);
+            for (uint32_t i = 0; i < 16; ++i)
+                v[i] = ptx::ld_shared_u32(stage_u32 + (r0 + i) * 128u + ((chunk ^ (i & 7u)) << 4) + word);
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
+            for (uint32_t i = 0; i < 16; ++i) {
                 if (first != (odd_pitch && (i & 1u) != 0u)) {
                     const uint32_t before = __shfl_up_sync(0xffffffffu, v[i], 1);
                     if (lane != 0u)
-                        *reinterpret_cast<uint32_t *>(dst + 2u * lane - 1u) = __funnelshift_l(before, v[i], 16);
-                    else
-                        *reinterpret_cast<uint16_t *>(dst) = static_cast<uint16_t>(v[i]);
-                    if (lane == 31u)
-                        *reinterpret_cast<uint16_t *>(dst + 63) = static_cast<uint16_t>(v[i] >> 16);
+                        *reinterpret_cast<uint32_t *>(to - 1) = __funnelshift_l(before, v[i], 16);
                 } else {
-                    *reinterpret_cast<uint32_t *>(dst + 2u * lane) = v[i];
+                    *reinterpret_cast<uint32_t *>(to) = v[i];
                 }
-                dst += p.ldc;
+                to += p.ldc;
+            }
+        }
+        // the first and the last column of the rows that start between words: a lane for each of 32 such ends
+        if (first || odd_pitch) {
+            for (uint32_t pass = 0; pass < (odd_pitch ? 1u : 2u); ++pass) {
+                const uint32_t r = odd_pitch ? (lane >> 1) * 2u + (first ? 0u : 1u) : pass * 16u + (lane >> 1);
+                const uint32_t c = (lane & 1u) * 63u;
+                dst[static_cast<uint64_t>(r) * p.ldc + c] =
+                    ptx::ld_shared_bf16(stage_u32 + r * 128u + (((c >> 3) ^ (r & 7u)) << 4) + (c & 7u) * 2u);
             }
         }
         __syncwarp();
