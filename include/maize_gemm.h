@@ -175,8 +175,8 @@ MAIZE_API maize_status_t maize_ctx_poll(maize_ctx_t *ctx, void *cuda_stream);
  * C use a 256 x 512 tile per CTA pair, which moves a quarter less data from L2 per flop; "wide_max_gflop", default 1000000, is the largest
  * 2MNK / 1e9 that takes it: multi-millisecond GEMMs run back to back for seconds are 1-3 % faster on the 256 x 256
  * tile), "tma_promotion" (L2 promotion of the operand tensor maps: 0 none, 1 64 B, 2 128 B, 3 256 B
- * = default), "k_parts" (default 0 = by size: CTAs of a cluster that share a tile's K in the grouped products, 1, 2, 4 or 8,
- * and in the e4m3 product, 1, 2 or 4; the weight gradient is not cut), "chain_streams"
+ * = default), "k_parts" (default 0 = by size: CTAs of a cluster that share a tile's sum, over K in the grouped products and
+ * over a group's rows in their weight gradient, 1, 2, 4 or 8, and in the e4m3 product, 1, 2 or 4), "chain_streams"
  * (1 to 4, default 2: streams that maize_chain_forward deals its chunks over), "chain_stagger"
  * (default 1: when the source is all there, as on the root, the streams start a fraction of a chunk apart,
  * so that they never publish at the same time and the link never idles), "repack_bytes" (size of an

@@ -55,54 +55,6 @@ struct F8SkinnyLayout {
     static_assert(kShare >= 8 && kShare <= 32, "columns of a warp that one CTA finishes");
 };
 
-// Stores 32 rows x COLS columns of C, lane = row: 16 bytes at a time where C's rows are aligned.  Else through `stage` (32 rows
-// of COLS bf16), so that COLS / 2 lanes store a row in 4-byte words; a row that starts between two words gets its halves
-// from the neighbouring lane and 2-byte stores at its ends.
-template <uint32_t COLS>
-__device__ __forceinline__ void f8_skinny_store(const GemmParams &p, uint32_t stage, uint32_t lane, uint32_t row0, uint32_t col0,
-                                                uint32_t end, const uint32_t (&out)[COLS])
-{
-    uint32_t word[COLS / 2];
-#pragma unroll
-    for (uint32_t i = 0; i < COLS / 2; ++i)
-        word[i] = ptx::pack_bf16x2(out[2 * i], out[2 * i + 1]);
-    if (p.c_vec_ok && col0 + COLS <= end) {
-        if (row0 + lane < p.m) {
-            uint4 *dst = reinterpret_cast<uint4 *>(p.c + static_cast<uint64_t>(row0 + lane) * p.ldc + col0);
-#pragma unroll
-            for (uint32_t i = 0; i < COLS / 8; ++i)
-                dst[i] = make_uint4(word[4 * i], word[4 * i + 1], word[4 * i + 2], word[4 * i + 3]);
-        }
-        return;
-    }
-    constexpr uint32_t kLanes = COLS / 2, kRows = 32 / kLanes;  // lanes per row, rows at a time
-#pragma unroll
-    for (uint32_t i = 0; i < COLS / 8; ++i)
-        ptx::st_shared_v4(stage + lane * (COLS * 2) + i * 16u, word[4 * i], word[4 * i + 1], word[4 * i + 2], word[4 * i + 3]);
-    __syncwarp();
-    const uint32_t l = lane % kLanes, left = end - col0;
-#pragma unroll 4
-    for (uint32_t r = lane / kLanes; r < 32; r += kRows) {
-        const uint32_t mine = ptx::ld_shared_u32(stage + r * (COLS * 2) + l * 4u);
-        const uint32_t before = __shfl_up_sync(0xffffffffu, mine, 1, kLanes);
-        if (row0 + r >= p.m)
-            continue;
-        __nv_bfloat16 *dst = p.c + static_cast<uint64_t>(row0 + r) * p.ldc + col0;
-        const bool between = (reinterpret_cast<uintptr_t>(dst) & 2u) != 0u;
-        const int32_t c = static_cast<int32_t>(2u * l) - (between ? 1 : 0);  // this lane's two columns from here
-        const uint32_t v = between ? __funnelshift_l(before, mine, 16) : mine;
-        if (c < 0)
-            *reinterpret_cast<uint16_t *>(dst) = static_cast<uint16_t>(mine);
-        else if (static_cast<uint32_t>(c) + 1 < left)
-            *reinterpret_cast<uint32_t *>(dst + c) = v;
-        else if (static_cast<uint32_t>(c) < left)
-            *reinterpret_cast<uint16_t *>(dst + c) = static_cast<uint16_t>(v);
-        if (between && l == kLanes - 1 && COLS - 1 < left)
-            *reinterpret_cast<uint16_t *>(dst + COLS - 1) = static_cast<uint16_t>(mine >> 16);
-    }
-    __syncwarp();
-}
-
 template <uint32_t REPL, uint32_t S, uint32_t STAGES>
 __global__ void __launch_bounds__(kF8SkinnyThreads, 1)
 gemm_e4m3_sm100_skinny(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
@@ -367,7 +319,7 @@ gemm_e4m3_sm100_skinny(const __grid_constant__ CUtensorMap tma_a, const __grid_c
             // ---- store this CTA's share: kShare columns of 32 rows (what came for this warp has been read: its place serves)
             const uint32_t end = min(p.n, n0 + f.bn), out_col = n0 + col0 + rank * L::kShare;
             if (row0 < p.m && out_col < end)
-                f8_skinny_store<L::kShare>(p, exchange + w * (L::kShare * 128u), lane, row0, out_col, end, out);
+                store_share<L::kShare>(p, exchange + w * (L::kShare * 128u), lane, row0, out_col, end, out);
             __syncwarp();
             if (lane < S && lane != rank)
                 ptx::mbar_arrive_cluster_addr(ptx::mapa_shared(sums_taken_bar, lane));

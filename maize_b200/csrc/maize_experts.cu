@@ -9,6 +9,7 @@
 #include "gemm_sm100_grouped.cuh"
 #include "gemm_sm100_grouped_split.cuh"
 #include "gemm_sm100_grouped_wgrad.cuh"
+#include "gemm_sm100_grouped_wgrad_split.cuh"
 
 namespace {
 
@@ -84,6 +85,40 @@ maize_status_t launch_split(maize_ctx_t *ctx, const maize::RowMaps &ta, const CU
     const int slot = maize::kAttrGroupedSplit + (W_KN ? 3 : 0) + (S == 2 ? 0 : (S == 4 ? 1 : 2));
     return maize::launch_clusters(ctx, slot, maize::gemm_bf16_sm100_grouped_split<W_KN, S, STAGES>, clusters * S, S,
                                   maize::kNumThreads, maize::GroupedSplitLayout<S, STAGES>::kDynamicBytes, stream, ta, tw, p);
+}
+
+// The same choice for the weight gradient, whose sum runs over a group's rows: reckoned with the mean group.  11186 rows of one
+// group, 136 x 544: 15 us in eight parts, 21 in four, 61 whole; 16384 rows, 4096 x 4096: 417 whole, 751 in two.
+uint32_t wgrad_parts(const maize_ctx_t *ctx, uint32_t rows, uint32_t groups, uint32_t n, uint32_t k)
+{
+    if (ctx->k_parts != 0)
+        return ctx->k_parts;
+    const uint64_t kb = (uint64_t(rows) / groups + 63) / 64;
+    auto blocks = [](uint64_t size, uint64_t tile) { return (size + tile - 1) / tile; };
+    double best = double(blocks(groups * blocks(n, 256) * blocks(k, 256), clusters_of(ctx, 2))) * (kb * 0.33 + 2.5);
+    const uint64_t tiles = groups * blocks(n, maize::kWgradSplitTile) * blocks(k, maize::kWgradSplitTile);
+    uint32_t parts = 1;
+    for (uint32_t s = 2; s <= 8; s *= 2) {
+        const double cost = double(blocks(tiles, clusters_of(ctx, s))) * (blocks(kb, s) * 0.33 + (s == 2 ? 3.0 : (s == 4 ? 3.5 : 4.0)));
+        if (cost < best) {
+            best = cost;
+            parts = s;
+        }
+    }
+    return parts;
+}
+
+template <uint32_t S, uint32_t STAGES>
+maize_status_t launch_wgrad_split(maize_ctx_t *ctx, const CUtensorMap &tdc, const CUtensorMap &ta, const GroupedParams &p,
+                                  cudaStream_t stream)
+{
+    const uint64_t tiles = uint64_t(p.groups) * ((uint64_t(p.n) + 127) / 128) * ((uint64_t(p.k) + 127) / 128);
+    if (tiles > 0x7fffffffull)
+        return fail(ctx, MAIZE_ERR_UNSUPPORTED, "too many output tiles");
+    const uint32_t most = clusters_of(ctx, S), clusters = tiles < most ? static_cast<uint32_t>(tiles) : most;
+    const int slot = maize::kAttrWgradSplit + (S == 2 ? 0 : (S == 4 ? 1 : 2));
+    return maize::launch_clusters(ctx, slot, maize::gemm_bf16_sm100_grouped_wgrad_split<S, STAGES>, clusters * S, S,
+                                  maize::kWgradSplitThreads, maize::WgradSplitLayout<S, STAGES>::kDynamicBytes, stream, tdc, ta, p);
 }
 
 maize_status_t grouped_impl(maize_ctx_t *ctx, const void *a, uint64_t lda, const void *b, uint64_t ldb, uint64_t b_stride,
@@ -266,6 +301,13 @@ maize_status_t maize_grouped_gemm_bf16_wgrad(maize_ctx_t *ctx, const void *a, ui
     p.pdl = ctx->pdl;
     p.status = ctx->d_status;
     p.timeout_ns = ctx->timeout_ns;
+    p.c_vec_ok = (lddb % 8 == 0 && db_stride % 8 == 0 && aligned(db, 16)) ? 1u : 0u;
+    switch (wgrad_parts(ctx, rows, groups, n, k)) {
+    case 2: return launch_wgrad_split<2, 4>(ctx, tdc, ta, p, stream);
+    case 4: return launch_wgrad_split<4, 4>(ctx, tdc, ta, p, stream);
+    case 8: return launch_wgrad_split<8, 4>(ctx, tdc, ta, p, stream);
+    default: break;
+    }
     // Rows of DB that TMA can store: a store writes whole 16-byte pieces, so K has to end on one (a K of 57 had zeros
     // written into the seven columns behind it).  A stack the driver refuses goes by plain stores too.
     if (ctx->tma_store && k % 8 == 0 && lddb % 8 == 0 && db_stride % 8 == 0 && aligned(db, 16) && lddb * 2 < (1ull << 40) &&

@@ -9,7 +9,8 @@ namespace maize {
 constexpr uint32_t kMaxDim = 0x7fffff00u;  // sizes are TMA coordinates (int32); room for a tile past the end
 
 // ctx->attr_experts slots: kernels whose shared-memory limit has been raised on the context's device
-enum { kAttrGrouped = 0, kAttrGroupedKn = 1, kAttrWgrad = 2, kAttrE4m3 = 3, kAttrE4m3Skinny = 4 /* .. 9 */, kAttrGroupedSplit = 10 /* .. 15 */ };
+enum { kAttrGrouped = 0, kAttrGroupedKn = 1, kAttrWgrad = 2, kAttrE4m3 = 3, kAttrE4m3Skinny = 4 /* .. 9 */, kAttrGroupedSplit = 10 /* .. 15 */,
+       kAttrWgradSplit = 16 /* .. 18 */ };
 
 inline bool aligned(const void *p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 

@@ -253,18 +253,21 @@ def check_wgrad(ctx, sizes, n, k, seed=11, first=0, behind=0):
         at += s
 
 
+@EVERY_KERNEL
 @pytest.mark.parametrize("sizes", SIZES + [[64, 128, 192], [16, 32, 48], [63, 65, 127, 1], [320, 0, 321, 15]],
                          ids=lambda s: "-".join(map(str, s[:7])))
-def test_wgrad_group_sizes(ctx, sizes):
+def test_wgrad_group_sizes(ctx, sizes, parts):
     check_wgrad(ctx, sizes, 264, 520, behind=70)
 
 
+@EVERY_KERNEL
 @pytest.mark.parametrize("n,k", [(8, 8), (256, 256), (256, 64), (64, 256), (40, 264), (1032, 72), (776, 2056)])
-def test_wgrad_matrix_sizes(ctx, n, k):
+def test_wgrad_matrix_sizes(ctx, n, k, parts):
     check_wgrad(ctx, [5, 300, 0, 33], n, k, seed=12, first=3)
 
 
-def test_wgrad_neighbours_do_not_leak(ctx):
+@EVERY_KERNEL
+def test_wgrad_neighbours_do_not_leak(ctx, parts):
     """Rows of the next group are infinite or NaN in both operands: a block that crosses the border drops them."""
     import torch
     g = gen(13)
@@ -278,8 +281,9 @@ def test_wgrad_neighbours_do_not_leak(ctx):
     assert torch.equal(out[0], clean[0]) and torch.equal(out[2], clean[2])
 
 
+@EVERY_KERNEL
 @pytest.mark.parametrize("n,k", [(264, 200), (33, 57)])
-def test_wgrad_strided(ctx, n, k):
+def test_wgrad_strided(ctx, n, k, parts):
     """Padded operand rows; results with 16-byte rows (TMA stores), odd rows (plain stores) and gaps between matrices."""
     import torch
     g = gen(14)
@@ -300,6 +304,17 @@ def test_wgrad_strided(ctx, n, k):
             at += s
         out.fill_(7.0)
         assert (buf == 7).all()
+
+
+def test_wgrad_of_one_long_group(ctx):
+    """The sizes that the rows are split for by themselves."""
+    check_wgrad(ctx, [5003], 136, 544, seed=15)
+    check_wgrad(ctx, [2100, 0, 900], 200, 104, seed=16, first=7, behind=9)
+
+
+@EVERY_KERNEL
+def test_wgrad_many_tiles_per_cta(ctx, parts):
+    check_wgrad(ctx, [200, 3, 0, 129, 64] * 4, 520, 776, seed=17)
 
 
 def test_wgrad_without_rows_is_zero(ctx):
@@ -412,8 +427,9 @@ def test_other_stream_and_graphs(ctx):
     assert all(torch.equal(a, b) for a, b in zip(outs[0], again))
 
 
+@EVERY_KERNEL
 @pytest.mark.parametrize("bad", [[0, 5, 4, 10], [0, 5, 8, 11], [-1, 2, 3, 4]])
-def test_wrong_offsets_are_reported(ctx, bad):
+def test_wrong_offsets_are_reported(ctx, bad, parts):
     """Offsets that descend or leave the rows: the kernels' own check reports them, nothing is written."""
     import torch
     import maize_b200
