@@ -4,7 +4,9 @@
 //     C[r, :] = A[r, :] * W[g]^T   (W[g] stored N x K)      or      C[r, :] = A[r, :] * W[g]   (W[g] stored K x N).
 //
 // The offsets live on the device, so the host knows neither the sizes of the groups nor the number of tiles: every CTA
-// builds the table of tiles itself (group_table below) and the persistent pairs deal the tiles out round robin.
+// builds the table of tiles itself (build_group_table below) and the persistent pairs deal the tiles out round robin.  (Groups
+// with large tiles first, as the weight gradient has them, cost 1 us more at the start and gained nothing: 16 groups of
+// 2000 uneven rows, 2048 x 2048, 39 us instead of 37.  What bounds uneven groups is reading W, not the longest pair.)
 //
 // The WEIGHTS are the M side of the MMA (256 rows of W per CTA pair, 128 per CTA) and the rows of A the N side: an MMA's
 // M is fixed but its N is a field of the run-time instruction descriptor, so the ragged end of a group costs its rows
@@ -54,10 +56,17 @@ struct RowMaps {
 
 struct GroupTable {
     uint32_t *offset;  // shared memory: groups + 1 row numbers
-    uint32_t *first;   // shared memory: groups + 1 numbers of row tiles before the group
-};
-constexpr uint32_t kGroupTableBytes = 2 * 4 * (kGroupedMaxGroups + 4);
+    uint32_t *first;   // shared memory: numbers of row tiles before each group of `order`, then the number of all
+    uint16_t *order;   // shared memory: the groups with rows; for the weight gradient all groups, those with most rows first
 
+    __device__ __forceinline__ explicit GroupTable(uint8_t *at)
+        : offset(reinterpret_cast<uint32_t *>(at)), first(offset + kGroupedMaxGroups + 4),
+          order(reinterpret_cast<uint16_t *>(first + kGroupedMaxGroups + 4))
+    {
+    }
+};
+constexpr uint32_t kGroupTableBytes = 2 * 4 * (kGroupedMaxGroups + 4) + 2 * kGroupedMaxGroups;
+static_assert(kGroupedMaxGroups <= 65536, "groups are listed in 16 bits");
 
 // Whole CTA.  Reads the offsets (into shared memory if `to` is given) and checks them: offsets that do not ascend, or leave
 // [0, rows], are reported as MAIZE_ERR_DEVICE_ABORT and the answer is false.
@@ -81,18 +90,28 @@ __device__ __forceinline__ bool load_offsets(const GroupedParams &p, uint32_t *t
     return true;
 }
 
-// Whole CTA.  Reads the offsets into shared memory and counts the row tiles before each group; false if they
-// are not right (there are no tiles then).
-template <uint32_t TILE_ROWS = kGroupedTileRows>
-__device__ __forceinline__ bool build_group_table(const GroupedParams &p, const GroupTable &t)
+// Rows of each of the `nt` near-equal tiles of a group: ceil(rows / nt) rounded up to the unit; TILE_ROWS * (nt - 1) < rows
+// leaves rows for the last one.
+template <uint32_t UNIT>
+__device__ __forceinline__ uint32_t rows_per_tile(uint32_t rows, uint32_t nt)
+{
+    return ((rows + nt - 1) / nt + UNIT - 1) / UNIT * UNIT;
+}
+
+// Whole CTA.  Reads the offsets into shared memory, lists the groups that have rows (with 1000 groups and 300 rows, a walk
+// over the empty ones took half of the call: 44 us instead of 13) and counts the row tiles before each.  `tiles` = their
+// number; false if the offsets are not right.
+template <uint32_t TILE_ROWS>
+__device__ __forceinline__ bool build_group_table(const GroupedParams &p, const GroupTable &t, uint32_t &tiles)
 {
     if (!load_offsets(p, t.offset))
         return false;
     if (threadIdx.x < 32) {
-        uint32_t total = 0;
+        uint32_t total = 0, listed = 0;
         for (uint32_t base = 0; base < p.groups; base += 32) {
             const uint32_t g = base + threadIdx.x;
             const uint32_t mine = g < p.groups ? (t.offset[g + 1] - t.offset[g] + TILE_ROWS - 1) / TILE_ROWS : 0u;
+            const uint32_t with_rows = __ballot_sync(0xffffffffu, mine != 0);
             uint32_t sum = mine;
 #pragma unroll
             for (uint32_t d = 1; d < 32; d <<= 1) {
@@ -100,14 +119,21 @@ __device__ __forceinline__ bool build_group_table(const GroupedParams &p, const 
                 if (threadIdx.x >= d)
                     sum += up;
             }
-            if (g < p.groups)
-                t.first[g] = total + sum - mine;
+            if (mine != 0) {
+                const uint32_t at = listed + __popc(with_rows & ((1u << threadIdx.x) - 1u));
+                t.first[at] = total + sum - mine;
+                t.order[at] = static_cast<uint16_t>(g);
+            }
+            listed += __popc(with_rows);
             total += __shfl_sync(0xffffffffu, sum, 31);
         }
-        if (threadIdx.x == 0)
-            t.first[p.groups] = total;
+        if (threadIdx.x == 0) {
+            t.first[listed] = total;
+            t.offset[kGroupedMaxGroups + 1] = total;
+        }
     }
     __syncthreads();
+    tiles = t.offset[kGroupedMaxGroups + 1];
     return true;
 }
 
@@ -120,20 +146,20 @@ struct GroupedTile {
     }
 };
 
-// Tile `t` of the launch; `g` is the role's cursor over the groups (tiles come in ascending order).  Within a group the
+// Tile `t` of the launch; `at` is the role's cursor over the listed groups (tiles come in ascending order).  Within a group the
 // row tiles of one block of weights follow each other, so that the weights are read from HBM once.
-template <uint32_t UNIT = kGroupedRowUnit>
-__device__ __forceinline__ GroupedTile grouped_tile(uint64_t t, uint32_t n_blocks, const GroupTable &tab, uint32_t &g)
+template <uint32_t UNIT>
+__device__ __forceinline__ GroupedTile grouped_tile(uint64_t t, uint32_t n_blocks, const GroupTable &tab, uint32_t &at)
 {
-    while (t >= static_cast<uint64_t>(tab.first[g + 1]) * n_blocks)
-        ++g;
+    while (t >= static_cast<uint64_t>(tab.first[at + 1]) * n_blocks)
+        ++at;
+    const uint32_t g = tab.order[at];
     const uint32_t begin = tab.offset[g];
     const uint32_t rows = tab.offset[g + 1] - begin;
-    const uint32_t nt = tab.first[g + 1] - tab.first[g];
-    const uint32_t local = static_cast<uint32_t>(t - static_cast<uint64_t>(tab.first[g]) * n_blocks);
+    const uint32_t nt = tab.first[at + 1] - tab.first[at];
+    const uint32_t local = static_cast<uint32_t>(t - static_cast<uint64_t>(tab.first[at]) * n_blocks);
     const uint32_t tb = local % nt;
-    // near-equal tiles: ceil(rows / nt) rounded up to the unit; 256 * (nt - 1) < rows leaves rows for the last one
-    const uint32_t per = ((rows + nt - 1) / nt + UNIT - 1) / UNIT * UNIT;
+    const uint32_t per = rows_per_tile<UNIT>(rows, nt);
     GroupedTile r;
     r.group = g;
     r.n_blk = local / nt;
@@ -260,9 +286,7 @@ gemm_bf16_sm100_grouped(const __grid_constant__ RowMaps tma_a, const __grid_cons
     auto acc_empty_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + 2 + b); };
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + L::kTmemSlotOffset);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem_gen + L::kAbortOffset);
-    GroupTable tab;
-    tab.offset = reinterpret_cast<uint32_t *>(smem_gen + L::kTableOffset);
-    tab.first = tab.offset + kGroupedMaxGroups + 4;
+    const GroupTable tab(smem_gen + L::kTableOffset);
 
     const uint32_t warp = threadIdx.x >> 5;
     const uint32_t lane = threadIdx.x & 31u;
@@ -301,8 +325,9 @@ gemm_bf16_sm100_grouped(const __grid_constant__ RowMaps tma_a, const __grid_cons
         ptx::grid_dependency_wait();
     }
     // both CTAs of a pair read the same offsets and come to the same tiles
-    const bool table_ok = build_group_table(p, tab);
-    const uint64_t num_tiles = table_ok ? static_cast<uint64_t>(tab.first[p.groups]) * n_blocks : 0ull;
+    uint32_t row_tiles = 0;
+    build_group_table<kGroupedTileRows>(p, tab, row_tiles);
+    const uint64_t num_tiles = static_cast<uint64_t>(row_tiles) * n_blocks;
 
     bool role_ok = true;
     if (warp == 0) {
@@ -311,7 +336,7 @@ gemm_bf16_sm100_grouped(const __grid_constant__ RowMaps tma_a, const __grid_cons
             uint32_t stage = 0, phase = 0, g = 0;
             bool ok = true;
             for (uint64_t t = pair; ok && t < num_tiles; t += num_pairs) {
-                const GroupedTile tile = grouped_tile(t, n_blocks, tab, g);
+                const GroupedTile tile = grouped_tile<kGroupedRowUnit>(t, n_blocks, tab, g);
                 const uint32_t half = tile.mma_n() / 2;  // rows of A this CTA brings in
                 const uint32_t box = half <= 16 ? 0u : (half <= 32 ? 1u : (half <= 64 ? 2u : 3u));
                 const uint32_t a_bytes = (16u << box) * (kBlockK * 2);
@@ -352,7 +377,7 @@ gemm_bf16_sm100_grouped(const __grid_constant__ RowMaps tma_a, const __grid_cons
             uint32_t acc = 0, acc_phase = 0;
             bool ok = true;
             for (uint64_t t = pair; ok && t < num_tiles; t += num_pairs) {
-                const GroupedTile tile = grouped_tile(t, n_blocks, tab, g);
+                const GroupedTile tile = grouped_tile<kGroupedRowUnit>(t, n_blocks, tab, g);
                 const uint32_t idesc = ptx::make_instr_desc_bf16(2 * kBlockM, tile.mma_n(), false, W_KN);
                 ok = wait_bounded<true>(acc_empty_bar(acc), acc_phase ^ 1u, ctl, 2);
                 if (!ok)
@@ -396,7 +421,7 @@ gemm_bf16_sm100_grouped(const __grid_constant__ RowMaps tma_a, const __grid_cons
         uint32_t acc = 0, acc_phase = 0, g = 0;
         bool ok = true;
         for (uint64_t t = pair; ok && t < num_tiles; t += num_pairs) {
-            const GroupedTile tile = grouped_tile(t, n_blocks, tab, g);
+            const GroupedTile tile = grouped_tile<kGroupedRowUnit>(t, n_blocks, tab, g);
             ok = wait_bounded<true>(acc_full_bar(acc), acc_phase, ctl, 3);
             // both warps of a buffer go on or both give up: neither may wait at their barrier for one that has left
             ok = ptx::named_barrier_and(1u + share, 64, ok);

@@ -58,9 +58,7 @@ gemm_bf16_sm100_grouped_split(const __grid_constant__ RowMaps tma_a, const __gri
     const uint32_t sums_taken_bar = bar_base + 8u * (2 * STAGES + 5);  // the others have read what this CTA sent
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + L::kTmemSlotOffset);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem_gen + L::kAbortOffset);
-    GroupTable tab;
-    tab.offset = reinterpret_cast<uint32_t *>(smem_gen + L::kTableOffset);
-    tab.first = tab.offset + kGroupedMaxGroups + 4;
+    const GroupTable tab(smem_gen + L::kTableOffset);
 
     const uint32_t warp = threadIdx.x >> 5;
     const uint32_t lane = threadIdx.x & 31u;
@@ -104,8 +102,9 @@ gemm_bf16_sm100_grouped_split(const __grid_constant__ RowMaps tma_a, const __gri
         ptx::grid_dependency_wait();
     }
     // all CTAs of a cluster read the same offsets and come to the same tiles
-    const bool table_ok = build_group_table<kSplitTileRows>(p, tab);
-    const uint64_t num_tiles = table_ok ? static_cast<uint64_t>(tab.first[p.groups]) * n_blocks : 0ull;
+    uint32_t row_tiles = 0;
+    build_group_table<kSplitTileRows>(p, tab, row_tiles);
+    const uint64_t num_tiles = static_cast<uint64_t>(row_tiles) * n_blocks;
 
     bool role_ok = true;
     if (warp == 0) {

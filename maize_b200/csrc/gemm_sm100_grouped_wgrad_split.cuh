@@ -46,8 +46,8 @@ __device__ __forceinline__ WgradSplitTile wgrad_split_tile(uint32_t t, uint32_t 
 {
     const uint32_t per_group = m_blocks * n_blocks;
     WgradSplitTile r;
-    r.group = t / per_group;
-    const uint32_t local = t - r.group * per_group;
+    const uint32_t at = t / per_group, local = t - at * per_group;
+    r.group = tab.order[at];
     r.m0 = local / n_blocks * kWgradSplitTile;
     r.n0 = local % n_blocks * kWgradSplitTile;
     const uint32_t begin = tab.offset[r.group], all = tab.offset[r.group + 1] - begin;
@@ -83,9 +83,7 @@ gemm_bf16_sm100_grouped_wgrad_split(const __grid_constant__ CUtensorMap tma_dc, 
     const uint32_t sums_taken_bar = bar_base + 8u * (3 * STAGES + 5);  // the others have read what this CTA sent
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + L::kTmemSlotOffset);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem_gen + L::kAbortOffset);
-    GroupTable tab;
-    tab.offset = reinterpret_cast<uint32_t *>(smem_gen + L::kTableOffset);
-    tab.first = tab.offset + kGroupedMaxGroups + 4;
+    const GroupTable tab(smem_gen + L::kTableOffset);
 
     const uint32_t warp = threadIdx.x >> 5;
     const uint32_t lane = threadIdx.x & 31u;
@@ -127,8 +125,8 @@ gemm_bf16_sm100_grouped_wgrad_split(const __grid_constant__ CUtensorMap tma_dc, 
             ptx::grid_dependency_launch_dependents();
         ptx::grid_dependency_wait();
     }
-    const bool table_ok = build_group_table(p, tab);
-    const uint32_t num_tiles = table_ok ? p.groups * m_blocks * n_blocks : 0u;
+    const uint32_t all_tiles = p.groups * m_blocks * n_blocks;
+    const uint32_t num_tiles = build_wgrad_table(p, tab, all_tiles <= num_clusters) ? all_tiles : 0u;
 
     bool role_ok = true;
     if (warp == 0) {
@@ -136,8 +134,8 @@ gemm_bf16_sm100_grouped_wgrad_split(const __grid_constant__ CUtensorMap tma_dc, 
         if (lane == 0) {
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            for (uint32_t t = cluster; ok && t < num_tiles; t += num_clusters) {
-                const WgradSplitTile tile = wgrad_split_tile<S>(t, m_blocks, n_blocks, rank, tab);
+            for (uint64_t round = 0, t; ok && (t = dealt_tile(round, cluster, num_clusters)) < num_tiles; ++round) {
+                const WgradSplitTile tile = wgrad_split_tile<S>(static_cast<uint32_t>(t), m_blocks, n_blocks, rank, tab);
                 for (uint32_t b = 0; b < tile.blocks; ++b) {
                     ok = wait_bounded(empty_bar(stage), phase ^ 1u, ctl, 1);
                     if (!ok)
@@ -169,8 +167,8 @@ gemm_bf16_sm100_grouped_wgrad_split(const __grid_constant__ CUtensorMap tma_dc, 
             uint32_t stage = 0, phase = 0;
             uint32_t acc = 0, acc_phase = 0;
             bool ok = true;
-            for (uint32_t t = cluster; ok && t < num_tiles; t += num_clusters) {
-                const WgradSplitTile tile = wgrad_split_tile<S>(t, m_blocks, n_blocks, rank, tab);
+            for (uint64_t round = 0, t; ok && (t = dealt_tile(round, cluster, num_clusters)) < num_tiles; ++round) {
+                const WgradSplitTile tile = wgrad_split_tile<S>(static_cast<uint32_t>(t), m_blocks, n_blocks, rank, tab);
                 if (tile.blocks == 0)
                     continue;  // nothing of this tile here: no accumulator changes hands
                 ok = wait_bounded(acc_empty_bar(acc), acc_phase ^ 1u, ctl, 2);
@@ -213,8 +211,8 @@ gemm_bf16_sm100_grouped_wgrad_split(const __grid_constant__ CUtensorMap tma_dc, 
         uint32_t stage = 0;
         uint32_t tail_phase = 0;  // bit s: parity of the next use of tail_bar(s)
         bool ok = true;
-        for (uint32_t t = cluster; ok && t < num_tiles; t += num_clusters) {
-            const WgradSplitTile tile = wgrad_split_tile<S>(t, m_blocks, n_blocks, rank, tab);
+        for (uint64_t round = 0, t; ok && (t = dealt_tile(round, cluster, num_clusters)) < num_tiles; ++round) {
+            const WgradSplitTile tile = wgrad_split_tile<S>(static_cast<uint32_t>(t), m_blocks, n_blocks, rank, tab);
             if (tile.blocks == 0)
                 continue;
             const uint32_t last = (stage + tile.blocks - 1) % STAGES;
@@ -248,8 +246,8 @@ gemm_bf16_sm100_grouped_wgrad_split(const __grid_constant__ CUtensorMap tma_dc, 
         const uint8_t *from = smem_gen + L::kExchangeOffset + w * L::kWarpBytes + lane * 16u;
         uint32_t acc = 0, acc_phase = 0, parity = 0;
         bool ok = true;
-        for (uint32_t t = cluster; ok && t < num_tiles; t += num_clusters, parity ^= 1u) {
-            const WgradSplitTile tile = wgrad_split_tile<S>(t, m_blocks, n_blocks, rank, tab);
+        for (uint64_t round = 0, t; ok && (t = dealt_tile(round, cluster, num_clusters)) < num_tiles; ++round, parity ^= 1u) {
+            const WgradSplitTile tile = wgrad_split_tile<S>(static_cast<uint32_t>(t), m_blocks, n_blocks, rank, tab);
             uint32_t v[kWgradSplitTile];  // one row of DW's tile
             if (tile.blocks > 0) {
                 ok = wait_bounded(acc_full_bar(acc), acc_phase, ctl, 3);

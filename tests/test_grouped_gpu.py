@@ -488,6 +488,19 @@ def test_most_groups(ctx):
     check_wgrad(ctx, sizes, 40, 24, seed=32)
 
 
+@EVERY_KERNEL
+@pytest.mark.parametrize("sizes", [
+    [(37 * i) % 200 for i in range(90)],                       # all different, some empty, several rounds of tiles
+    [0, 0, 300, 0, 1, 0, 0, 129, 0] * 10,                      # the same sizes again and again: ties in the order
+    [0] * 500 + [70] + [0] * 400 + [500, 1] + [0] * 121,       # 1024 groups, three with rows
+    [64 * (1 << i) + d for i in range(6) for d in (-1, 0, 1)], # around the borders between the classes
+], ids=["different", "ties", "sparse", "borders"])
+def test_order_of_uneven_groups(ctx, parts, sizes):
+    """The groups are listed, and for the weight gradient sorted, by their rows: every one is still computed once."""
+    check_grouped(ctx, sizes, 264, 72, False, seed=51)
+    check_wgrad(ctx, sizes, 264, 72, seed=52)
+
+
 def test_module_functions_use_the_tensors_device():
     import torch
     import maize_b200
