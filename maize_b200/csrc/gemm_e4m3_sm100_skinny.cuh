@@ -1,10 +1,11 @@
 // The e4m3 product for few rows of A, or few tiles: K is split over the CTAs of a cluster.  For M <= 128 bound by reading B once.
 //
-// Rows of A are the M side of the MMA, up to 256 rows of B its N side: an MMA takes about 128 cycles for the 32 k of its 128
-// M-side rows whatever its N, so the operand that has to stream belongs on the N side (with B on the M side 16 x 16384 x 4096
-// took 16.6 us, bound by the MMAs; 11.3 this way, 6.0 TB/s).  For M <= 32 (64) the rows of A are loaded four times (twice)
+// Rows of A are the M side of the MMA, up to 256 rows of B its N side: a k-block costs a CTA about 0.34 us in MMA issue and
+// hand-overs whatever the tile's width, so the operand that streams belongs on the side that may be 256 wide.  16 x 16384 x
+// 4096: 16.6 us with B on the M side, 128 rows at a time, 11.9 this way (both with B in L2; 15.2, 4.5 TB/s, when it comes from
+// HBM).  For M <= 32 (64) the rows of A are loaded four times (twice)
 // into the 128 lanes, so that every promotion warp has lanes with all rows and only some of the columns: REPL copies.  Only
-// the m rows there are are loaded (a box that reaches past the end of A takes longer: 17 against 11 us for one row of A);
+// the m rows there are are loaded (a box that reaches past the end of A takes longer: one row took 16.6 us, 16 rows 13.8);
 // what lies in the other lanes is never stored.  For 64 < M the tile is 128 wide, so that four accumulator buffers fit and
 // the MMA does not wait for hand-overs.
 //
