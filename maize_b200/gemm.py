@@ -269,6 +269,11 @@ class Context:
             raise MaizeError(_ffi.INVALID_ARG, f"{name}: expected a {dims}-D {dtype} tensor with unit column stride on "
                                                f"cuda:{self.device}")
 
+    @staticmethod
+    def _too_large(*sizes):
+        """The entry points take 32-bit sizes; what passes 31 bits would arrive there cut off."""
+        return MaizeError(_ffi.UNSUPPORTED, f"sizes {' x '.join(map(str, sizes))}: one is beyond the kernels' range")
+
     def _result(self, out, shape, dtype, stream):
         """The tensor a call writes: ``out`` if it is given and fits, else a new one, allocated for the
         stream the call runs on."""
@@ -307,6 +312,8 @@ class Context:
         n, kb = (b_cols, b_rows) if kn else (b_rows, b_cols)
         if k != kb:
             raise MaizeError(_ffi.INVALID_ARG, f"a has {k} columns, the matrices of b a K of {kb}")
+        if (rows | n | k | groups) >> 31:
+            raise self._too_large(rows, n, k, groups)
         self._offsets(offsets, groups)
         out = self._result(out, (rows, n), bf16, stream)
         # the stride of a dimension of one is not used and may be anything
@@ -341,6 +348,8 @@ class Context:
         rows_dc, n = dc.shape
         if rows_dc != rows:
             raise MaizeError(_ffi.INVALID_ARG, f"a has {rows} rows, dc {rows_dc}")
+        if (rows | n | k) >> 31:
+            raise self._too_large(rows, n, k)
         groups = offsets.numel() - 1
         if groups < 0:
             raise MaizeError(_ffi.INVALID_ARG, "offsets: expected groups + 1 int32 values")
@@ -366,6 +375,8 @@ class Context:
         rows, cols = x.shape
         if block_rows != 1 and block_rows != 128:
             raise MaizeError(_ffi.INVALID_ARG, "block_rows must be 1 or 128")
+        if (rows | cols) >> 31:
+            raise self._too_large(rows, cols)
         down, across = -(-rows // block_rows), -(-cols // 128)
         out = self._result(out, (rows, cols), torch.float8_e4m3fn, stream)
         scales = self._result(scales, (down, across), torch.float32, stream)
@@ -392,6 +403,8 @@ class Context:
         n, kb = b.shape
         if k != kb:
             raise MaizeError(_ffi.INVALID_ARG, "a.shape[1] != b.shape[1] (b is stored N x K)")
+        if (m | n | k) >> 31:
+            raise self._too_large(m, n, k)
         blocks, down = -(-k // 128), -(-n // 128)
         if a_scales.shape != (m, blocks) or b_scales.shape != (down, blocks):
             raise MaizeError(_ffi.INVALID_ARG, f"scales: expected {m} x {blocks} for a, {down} x {blocks} for b")

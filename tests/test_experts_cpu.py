@@ -114,6 +114,32 @@ def test_refused_before_the_library_is_called(ctx):
     assert ctx._lib.calls == []
 
 
+def test_sizes_beyond_the_entry_points_range_are_refused(ctx):
+    """The C entry points take 32-bit sizes: 2^32 + 10 rows may not arrive there as ten."""
+    many = (1 << 32) + 10
+    f32 = torch.float32
+
+    def tall(cols, dtype=BF16):
+        return t(1, cols, dtype=dtype).expand(many, cols)
+
+    o = offs(0, 10)
+    calls = [
+        lambda: ctx.grouped_gemm(tall(16), t(1, 24, 16), o, out=tall(24), stream=7),
+        lambda: ctx.grouped_gemm(t(10, 16), t(1, 1, 16).expand(1, many, 16), o, out=t(10, 1).expand(10, many), stream=7),
+        lambda: ctx.grouped_gemm_kn(tall(16), t(1, 16, 24), o, out=tall(24), stream=7),
+        lambda: ctx.grouped_gemm_wgrad(tall(16), tall(24), o, out=t(1, 24, 16), stream=7),
+        lambda: ctx.quantize_e4m3(tall(16), out=tall(16, F8), scales=tall(1, f32), stream=7),
+        lambda: ctx.gemm_e4m3(tall(16, F8), tall(1, f32), t(24, 16, dtype=F8), t(1, 1, dtype=f32), out=tall(24), stream=7),
+        lambda: ctx.gemm_e4m3(t(10, 16, dtype=F8), t(10, 1, dtype=f32), tall(16, F8),
+                              t(1, 1, dtype=f32).expand(-(-many // 128), 1), out=t(10, 1).expand(10, many), stream=7),
+    ]
+    for call in calls:
+        with pytest.raises(maize_b200.MaizeError) as e:
+            call()
+        assert e.value.status == _ffi.UNSUPPORTED
+    assert ctx._lib.calls == []
+
+
 def test_module_functions_refuse_cpu_tensors():
     a = t(4, 16)
     for call in (lambda: maize_b200.grouped_gemm(a, t(1, 8, 16), offs(0, 4)), lambda: maize_b200.quantize_e4m3(a),
