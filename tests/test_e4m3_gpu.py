@@ -334,6 +334,47 @@ def test_refusals(ctx):
     assert ctx.launch_count == before
 
 
+@EVERY_KERNEL
+def test_product_past_32_bits(ctx, parts):
+    """The last rows of operands and of a result that lie more than 2^32 bytes behind the start."""
+    import torch
+    f8 = torch.float8_e4m3fn
+    for m, n, k in ((300_000, 8193, 144), (270_001, 40, 16_384), (40, 270_001, 16_384)):  # C, A, B beyond 4 GiB
+        a, sa, b, sb = operands(71, 40 if m > 40 else m, 40 if n > 8193 else n, k, False)
+        if m > 40:
+            big = torch.zeros((m, k), dtype=torch.uint8, device="cuda").view(f8)
+            big[-40:] = a
+            big_s = torch.ones((m, sa.shape[1]), device="cuda")
+            big_s[-40:] = sa
+            out = ctx.gemm_e4m3(big, big_s, b, sb)[-40:]
+        elif n > 8193:
+            # rows of B in two scale blocks: the last 40 start inside the block before the last
+            big = torch.zeros((n, k), dtype=torch.uint8, device="cuda").view(f8)
+            big[-40:] = b
+            big_s = torch.ones((-(-n // 128), sb.shape[1]), device="cuda")
+            out = ctx.gemm_e4m3(a, sa, big, big_s)[:, -40:]
+            sb = torch.ones_like(sb)
+        ctx.poll()
+        ref, size = plain_product(a, sa, b, sb)
+        close(out, ref, size, k, f"{m} {n} {k}")
+        del big, big_s, out
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("cols", [16_384, 16_391])
+def test_quantize_past_32_bits(ctx, cols, block_rows):
+    import torch
+    rows = 270_000
+    x = torch.zeros((rows, cols), dtype=torch.bfloat16, device="cuda")
+    tail = rows % 128  # whole blocks of 128 rows before it
+    x[-tail:] = spread(gen(72), tail, cols)
+    q, s = ctx.quantize_e4m3(x, block_rows)
+    ctx.poll()
+    want, scale = plain_quantize(x[-tail:], block_rows)
+    assert same(s[-scale.shape[0]:].double(), scale) and same(q[-tail:].double(), want)
+    assert (s[:-scale.shape[0]] == 1).all() and not q[:256].view(torch.uint8).any()
+
+
 def test_module_functions(ctx):
     import torch
     import maize_b200

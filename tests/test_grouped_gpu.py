@@ -501,6 +501,48 @@ def test_order_of_uneven_groups(ctx, parts, sizes):
     check_wgrad(ctx, sizes, 264, 72, seed=52)
 
 
+@EVERY_KERNEL
+def test_elements_past_32_bits(ctx, parts):
+    """Rows of A and C, matrices of B and of DB that lie more than 2^32 bytes behind the start: a group at the very end."""
+    import torch
+    g = gen(61)
+    rows, k, n = 300_000, 8192, 8192  # A and C of 4.9e9 bytes each
+    a = torch.zeros((rows, k), dtype=torch.bfloat16, device="cuda")
+    a[-100:] = bf16(g, (100, k))
+    w = bf16(g, (2, n, k), 0.1)
+    o = torch.tensor([rows - 100, rows - 70, rows], dtype=torch.int32, device="cuda")
+    out = torch.full((rows, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    near = torch.tensor([0, 30, 100], dtype=torch.int32, device="cuda")
+    for kn in (False, True):
+        (ctx.grouped_gemm_kn if kn else ctx.grouped_gemm)(a, w, o, out=out)
+        ctx.poll()
+        ref, size = plain_grouped(a[-100:], w, near, kn)
+        close(out[-100:], ref, size, k)
+        assert (out[:64] == 7).all() and (out[-164:-100] == 7).all()
+    dw = ctx.grouped_gemm_wgrad(a, out, o)  # rows in front of the groups hold sevens
+    ctx.poll()
+    for i, (b, e) in enumerate(((0, 30), (30, 100))):
+        x, y = a[-100:][b:e].double(), out[-100:][b:e].double()
+        close(dw[i, :256], y[:, :256].T @ x, y[:, :256].abs().T @ x.abs(), e - b)
+        close(dw[i, -256:], y[:, -256:].T @ x, y[:, -256:].abs().T @ x.abs(), e - b)
+    del a, out, w, dw
+    # stacks of matrices: 33 of 8192 x 8192, rows for the first and the last
+    a, w, dy = bf16(g, (20, k)), torch.zeros((33, n, k), dtype=torch.bfloat16, device="cuda"), bf16(g, (20, n))
+    w[0], w[-1] = bf16(g, (n, k), 0.1), bf16(g, (n, k), 0.1)
+    o = torch.tensor([0] + [7] * 32 + [20], dtype=torch.int32, device="cuda")
+    for kn in (False, True):
+        out = (ctx.grouped_gemm_kn if kn else ctx.grouped_gemm)(a, w, o)
+        ctx.poll()
+        ref, size = plain_grouped(a, w[[0, -1]], torch.tensor([0, 7, 20]), kn)
+        close(out, ref, size, k)
+    dw = ctx.grouped_gemm_wgrad(a, dy, o, out=w.fill_(7.0))
+    ctx.poll()
+    assert not dw[1:-1].any()
+    for i, (b, e) in ((0, (0, 7)), (32, (7, 20))):
+        x, y = a[b:e].double(), dy[b:e].double()
+        close(dw[i, -256:], y[:, -256:].T @ x, y[:, -256:].abs().T @ x.abs(), e - b)
+
+
 def test_module_functions_use_the_tensors_device():
     import torch
     import maize_b200
