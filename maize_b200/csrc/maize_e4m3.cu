@@ -46,8 +46,9 @@ struct SkinnyPlan {
 };
 
 // The tiles are as wide as fills whole rounds of clusters.  A k-block costs a CTA 0.34 us (the MMA thread's issue and the
-// hand-over of its accumulator) or its bytes at 80 GB/s per SM (47 with 128 different rows of A), a tile's end 2 us,
-// measured; joining four parts about 0.8 us more than joining two.  16 x 512 x 8192: 9.8 us in four parts, 14.7 in two; 5 x 9001 x 2048: 12.8, 7.8.
+// hand-over of its accumulator) or its bytes at 80 GB/s per SM (47 with 128 different rows of A), a tile's end 2 to 3.5 us by the
+// rows there are (rounds of 50000 x 512: 3 us each for 16 rows, 5.1 for 33, 4.6 for 65), measured; joining four parts about 0.8
+// us more than joining two.  16 x 512 x 8192: 9.8 us in four parts, 14.7 in two; 5 x 9001 x 2048: 12.8, 7.8.
 SkinnyPlan skinny_plan(uint32_t ctas, uint32_t parts, uint32_t m, uint32_t n, uint32_t kblocks)
 {
     SkinnyPlan q;
@@ -67,7 +68,8 @@ SkinnyPlan skinny_plan(uint32_t ctas, uint32_t parts, uint32_t m, uint32_t n, ui
     q.bn = static_cast<uint32_t>(bn < widest ? bn : widest);
     const double bytes = (q.bn + q.copies * (m < 128 ? m : 128u)) * 128.0;
     const double rate = q.copies == 1 ? 47e3 : 80e3, block = bytes / rate > 0.34 ? bytes / rate : 0.34;
-    q.cost = double(rounds) * (((kblocks + parts - 1) / parts) * block + (parts == 2 ? 2.0 : 2.8));
+    const double end = (q.copies == 4 ? 2.0 : (q.copies == 2 ? 3.5 : 3.2)) + (parts == 2 ? 0.0 : 0.8);
+    q.cost = double(rounds) * (((kblocks + parts - 1) / parts) * block + end);
     return q;
 }
 
@@ -208,7 +210,7 @@ maize_status_t maize_gemm_e4m3(maize_ctx_t *ctx, const void *a, uint64_t lda, co
     if (lda >= (1ull << 40) || ldb >= (1ull << 40))
         return fail(ctx, MAIZE_ERR_UNSUPPORTED, "row pitch beyond the TMA limit of 2^40 bytes");
     // Few rows of A, or few tiles: K over a cluster.  The other kernel takes 0.55 us for a k-block of a 256 x 256 tile and about
-    // 1.5 us more for a tile's end.
+    // 1.5 us more for a tile's end.  128 x 8192 x 2048: 10.7 us over clusters, 12.4 in pairs; 128 x 16384 x 4096: 27.8, 20.9.
     const uint32_t ctas = maize::persistent_grid(ctx, 0xffffffffull, 1), kb = static_cast<uint32_t>(kblocks);
     SkinnyPlan plan = skinny_plan(ctas, 2, m, n, kb);
     const SkinnyPlan four = skinny_plan(ctas, 4, m, n, kb);
@@ -216,7 +218,7 @@ maize_status_t maize_gemm_e4m3(maize_ctx_t *ctx, const void *a, uint64_t lda, co
         plan = four;
     const uint64_t pair_tiles = ((uint64_t(m) + 255) / 256) * ((uint64_t(n) + 255) / 256), pairs = ctas / 2 ? ctas / 2 : 1;
     const double pair_cost = double((pair_tiles + pairs - 1) / pairs) * (kb * 0.55 + 1.5);
-    if (ctx->k_parts == 0 ? (m <= 128 || plan.cost < pair_cost) : ctx->k_parts != 1)
+    if (ctx->k_parts == 0 ? plan.cost < pair_cost : ctx->k_parts != 1)
         return skinny(ctx, plan, a, lda, static_cast<const float *>(a_scales), ld_a_scales, b, ldb, static_cast<const float *>(b_scales),
                       ld_b_scales, c, ldc, m, n, k, stream);
     CUtensorMap ta, tb, tc;
