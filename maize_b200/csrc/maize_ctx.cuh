@@ -88,6 +88,7 @@ struct maize_ctx {
     bool attr_set[maize::kMaxVariants] = {};
     bool attr_set_kn[maize::kMaxVariants] = {};  // the same for the K x N (MN-major B) instantiations
     bool attr_experts[24] = {};                  // the same for the kernels of maize_experts.cu and maize_e4m3.cu
+    uint32_t clusters_at_once[2] = {0, 0};  // clusters of four, of eight CTAs that the device runs at a time; 0: not asked yet
     float *d_partials = nullptr;        // stream-K scratch of the skinny kernels
     unsigned int *d_counters = nullptr;  // arrival counters, zero between launches
     unsigned int *d_push_counter = nullptr;  // [0]: CTA arrivals of the multicast push; [16 + p]: of the scatter per rank

@@ -49,16 +49,14 @@ struct SkinnyPlan {
 // hand-over of its accumulator) or its bytes at 80 GB/s per SM (47 with 128 different rows of A), a tile's end 2 to 3.5 us by the
 // rows there are (rounds of 50000 x 512: 3 us each for 16 rows, 5.1 for 33, 4.6 for 65), measured; joining four parts about 0.8
 // us more than joining two.  16 x 512 x 8192: 9.8 us in four parts, 14.7 in two; 5 x 9001 x 2048: 12.8, 7.8.
-SkinnyPlan skinny_plan(uint32_t ctas, uint32_t parts, uint32_t m, uint32_t n, uint32_t kblocks)
+SkinnyPlan skinny_plan(maize_ctx_t *ctx, uint32_t parts, uint32_t m, uint32_t n, uint32_t kblocks)
 {
     SkinnyPlan q;
     q.copies = m <= 32 ? 4 : (m <= 64 ? 2 : 1);
     q.parts = parts;
     q.tiles_m = (m + 127) / 128;
-    // clusters of four fit only within a GPC: of the 37 that 148 SMs would make, 32 are counted on
-    q.clusters = parts == 2 ? ctas / 2 : ctas * 32 / 148;
-    if (q.clusters == 0)
-        q.clusters = 1;
+    q.clusters = maize::clusters_at_once(ctx, parts, maize::gemm_e4m3_sm100_skinny<1, 4, 5>, maize::kF8SkinnyThreads,
+                                         maize::F8SkinnyLayout<1, 4, 5>::kDynamicBytes);
     const uint64_t widest = q.copies == 1 ? 128 : 256;
     const uint64_t rounds = (uint64_t(q.tiles_m) * ((n + widest - 1) / widest) + q.clusters - 1) / q.clusters;
     uint64_t per_m = rounds * q.clusters / q.tiles_m;  // tiles along N that fill the rounds
@@ -212,8 +210,8 @@ maize_status_t maize_gemm_e4m3(maize_ctx_t *ctx, const void *a, uint64_t lda, co
     // Few rows of A, or few tiles: K over a cluster.  The other kernel takes 0.55 us for a k-block of a 256 x 256 tile and about
     // 1.5 us more for a tile's end.  128 x 8192 x 2048: 10.7 us over clusters, 12.4 in pairs; 128 x 16384 x 4096: 27.8, 20.9.
     const uint32_t ctas = maize::persistent_grid(ctx, 0xffffffffull, 1), kb = static_cast<uint32_t>(kblocks);
-    SkinnyPlan plan = skinny_plan(ctas, 2, m, n, kb);
-    const SkinnyPlan four = skinny_plan(ctas, 4, m, n, kb);
+    SkinnyPlan plan = skinny_plan(ctx, 2, m, n, kb);
+    const SkinnyPlan four = skinny_plan(ctx, 4, m, n, kb);
     if (ctx->k_parts == 0 ? four.cost < plan.cost : ctx->k_parts >= 4)
         plan = four;
     const uint64_t pair_tiles = ((uint64_t(m) + 255) / 256) * ((uint64_t(n) + 255) / 256), pairs = ctas / 2 ? ctas / 2 : 1;

@@ -43,30 +43,45 @@ bool stack_ok(uint32_t count, uint64_t stride, uint64_t rows, uint64_t cols, uin
     return count <= 1 || rows == 0 || stride >= (rows - 1) * ld + cols;
 }
 
-// Clusters of `parts` CTAs at a time: those of four and eight fit only within a GPC.
-uint32_t clusters_of(const maize_ctx_t *ctx, uint32_t parts)
+uint32_t clusters_of(maize_ctx_t *ctx, uint32_t parts)
 {
-    const uint32_t ctas = persistent_grid(ctx, 0xffffffffull, 1);
-    const uint32_t c = parts == 2 ? ctas / 2 : (parts == 4 ? ctas * 32 / 148 : ctas * 16 / 148);
-    return c ? c : 1;
+    if (parts == 8)
+        return maize::clusters_at_once(ctx, 8, maize::gemm_bf16_sm100_grouped_split<false, 8, 7>, maize::kNumThreads,
+                                       maize::GroupedSplitLayout<8, 7>::kDynamicBytes);
+    return maize::clusters_at_once(ctx, parts, maize::gemm_bf16_sm100_grouped_split<false, 4, 7>, maize::kNumThreads,
+                                   maize::GroupedSplitLayout<4, 7>::kDynamicBytes);
+}
+
+// What sharing a tile's sum among `parts` CTAs costs, in microseconds beyond what every call takes, for comparison only.
+struct SplitCost {
+    double end;    // of the last tile
+    double least;  // of any other tile: behind a short sum the one before is not yet stored
+};
+
+double split_cost(const SplitCost &c, uint64_t tiles, uint64_t at_a_time, double sum)
+{
+    const uint64_t rounds = (tiles + at_a_time - 1) / at_a_time;
+    return c.end + sum + double(rounds - 1) * (sum > c.least ? sum : c.least);
 }
 
 // CTAs that share a tile's K, or 1 for the kernel that gives a pair whole tiles.  Both are reckoned with the most tiles that
-// the rows can make; a k-block costs about 0.3 us either way, a tile's end 1 us, and 2 to 3 us where the parts meet.
+// the rows can make, 0.27 us for a k-block, and what was measured of the tiles' ends; neither is faster than the weights come.
 // Eight rows for five experts, 144 x 6936: 8 us in eight parts, 35 whole; 39 rows for one, 4096 x 4096: 10.6 in four parts, 20
 // in eight (two rounds), 22 whole; 32 rows for 16 experts, 4096 x 2048: 48 in two parts, 65 in four, 46 to 50 whole.
-uint32_t split_parts(const maize_ctx_t *ctx, uint32_t rows, uint32_t groups, uint32_t n, uint32_t k)
+uint32_t split_parts(maize_ctx_t *ctx, uint32_t rows, uint32_t groups, uint32_t n, uint32_t k)
 {
     if (ctx->k_parts != 0)
         return ctx->k_parts;
     const uint64_t with_rows = rows < groups ? rows : groups, kb = (uint64_t(k) + 63) / 64;
-    auto rounds = [](uint64_t tiles, uint64_t at_a_time) { return double((tiles + at_a_time - 1) / at_a_time); };
+    const double weights = double(with_rows) * n * k * 2 / 6.2e6;
+    const SplitCost costs[4] = {{1.0, 2.1}, {1.6, 2.6}, {1.4, 2.1}, {1.3, 3.6}};
     const uint64_t pair_tiles = (rows / maize::kGroupedTileRows + with_rows) * ((uint64_t(n) + 255) / 256);
-    double best = rounds(pair_tiles, clusters_of(ctx, 2)) * (kb * 0.3 + 1.0);
+    double best = split_cost(costs[0], pair_tiles, clusters_of(ctx, 2), double(kb) * 0.27);
     const uint64_t tiles = (rows / maize::kSplitTileRows + with_rows) * ((uint64_t(n) + 127) / 128);
     uint32_t parts = 1;
-    for (uint32_t s = 2; s <= 8; s *= 2) {
-        const double cost = rounds(tiles, clusters_of(ctx, s)) * ((kb + s - 1) / s * 0.3 + (s == 2 ? 2.0 : (s == 4 ? 2.5 : 3.0)));
+    for (uint32_t i = 1; i <= 3 && best > weights; ++i) {
+        const uint32_t s = 1u << i;
+        const double cost = split_cost(costs[i], tiles, clusters_of(ctx, s), double((kb + s - 1) / s) * 0.27);
         if (cost < best) {
             best = cost;
             parts = s;
@@ -87,19 +102,26 @@ maize_status_t launch_split(maize_ctx_t *ctx, const maize::RowMaps &ta, const CU
                                   maize::kNumThreads, maize::GroupedSplitLayout<S, STAGES>::kDynamicBytes, stream, ta, tw, p);
 }
 
-// The same choice for the weight gradient, whose sum runs over a group's rows: reckoned with the mean group.  11186 rows of one
-// group, 136 x 544: 15 us in eight parts, 21 in four, 61 whole; 16384 rows, 4096 x 4096: 417 whole, 751 in two.
-uint32_t wgrad_parts(const maize_ctx_t *ctx, uint32_t rows, uint32_t groups, uint32_t n, uint32_t k)
+// The same choice for the weight gradient, whose sum runs over a group's rows: reckoned with the mean group, half as long again
+// where every tile has a pair or cluster to itself and the longest group decides.  11186 rows of one group, 136 x 544: 15 us in
+// eight parts, 21 in four, 61 whole; 16384 rows, 4096 x 4096: 417 whole, 751 in two; 290 rows, 112 x 32: 6 whole, 10.9 in two.
+uint32_t wgrad_parts(maize_ctx_t *ctx, uint32_t rows, uint32_t groups, uint32_t n, uint32_t k)
 {
     if (ctx->k_parts != 0)
         return ctx->k_parts;
-    const uint64_t kb = (uint64_t(rows) / groups + 63) / 64;
+    const uint64_t mean = (uint64_t(rows) / groups + 63) / 64;
     auto blocks = [](uint64_t size, uint64_t tile) { return (size + tile - 1) / tile; };
-    double best = double(blocks(groups * blocks(n, 256) * blocks(k, 256), clusters_of(ctx, 2))) * (kb * 0.33 + 2.5);
+    auto sum = [&](uint64_t tiles, uint64_t at_a_time, uint64_t parts) {
+        return double(blocks(groups > 1 && tiles <= at_a_time ? mean + mean / 2 : mean, parts)) * 0.35;
+    };
+    const SplitCost costs[4] = {{1.0, 2.7}, {5.0, 4.5}, {4.5, 3.5}, {3.9, 4.0}};
+    const uint64_t pair_tiles = groups * blocks(n, 256) * blocks(k, 256), pairs = clusters_of(ctx, 2);
+    double best = split_cost(costs[0], pair_tiles, pairs, sum(pair_tiles, pairs, 1));
     const uint64_t tiles = groups * blocks(n, maize::kWgradSplitTile) * blocks(k, maize::kWgradSplitTile);
     uint32_t parts = 1;
-    for (uint32_t s = 2; s <= 8; s *= 2) {
-        const double cost = double(blocks(tiles, clusters_of(ctx, s))) * (blocks(kb, s) * 0.33 + (s == 2 ? 3.0 : (s == 4 ? 3.5 : 4.0)));
+    for (uint32_t i = 1; i <= 3; ++i) {
+        const uint32_t s = 1u << i, at_a_time = clusters_of(ctx, s);
+        const double cost = split_cost(costs[i], tiles, at_a_time, sum(tiles, at_a_time, s));
         if (cost < best) {
             best = cost;
             parts = s;
