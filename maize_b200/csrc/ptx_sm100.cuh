@@ -202,6 +202,14 @@ __device__ __forceinline__ void tma_store_3d_hint(const CUtensorMap *map, uint32
                  : "memory");
 }
 
+// Brings a box into L2 only: a hint, allowed before what the box holds is known to be written.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap *map, int32_t x, int32_t y)
+{
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)),
+                 "r"(x), "r"(y)
+                 : "memory");
+}
+
 __device__ __forceinline__ void bulk_commit_group() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 
 // Until at most N of this thread's bulk groups are still READING their shared-memory source.

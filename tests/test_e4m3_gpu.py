@@ -360,6 +360,37 @@ def test_product_past_32_bits(ctx, parts):
         del big, big_s, out
 
 
+@EVERY_KERNEL
+@pytest.mark.parametrize("m", [1, 16, 48, 100])
+def test_operands_written_by_the_call_before(ctx, m, parts):
+    """Quantiser and product one behind the other, the same buffers again and again: no product sees the values before."""
+    import torch
+    g = gen(81)
+    n, k, rounds = 1000, 4096, 12
+    xs = [torch.randn((m, k), generator=g, device="cuda").to(torch.bfloat16) for _ in range(rounds)]
+    ws = [(torch.randn((n, k), generator=g, device="cuda") * 2.0 ** (i % 5)).to(torch.bfloat16) for i in range(rounds)]
+    want = []
+    for x, w in zip(xs, ws):
+        given = *ctx.quantize_e4m3(x), *ctx.quantize_e4m3(w, 128)
+        torch.cuda.synchronize()
+        want.append(ctx.gemm_e4m3(*given))
+        torch.cuda.synchronize()
+    qx, sx = ctx.quantize_e4m3(xs[0])
+    qw, sw = ctx.quantize_e4m3(ws[0], 128)
+    torch.cuda.synchronize()
+    for order in (0, 1):  # the weights, then the rows of A, quantised last
+        got = []
+        for x, w in zip(xs, ws):
+            for last in (order, 1 - order):
+                if last:
+                    ctx.quantize_e4m3(w, 128, out=qw, scales=sw)
+                else:
+                    ctx.quantize_e4m3(x, out=qx, scales=sx)
+            got.append(ctx.gemm_e4m3(qx, sx, qw, sw))
+        ctx.poll()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize("block_rows", [1, 128])
 @pytest.mark.parametrize("cols", [16_384, 16_391])
 def test_quantize_past_32_bits(ctx, cols, block_rows):
