@@ -432,12 +432,22 @@ gemm_bf16_sm100_grouped(const __grid_constant__ RowMaps tma_a, const __grid_cons
             const uint32_t taddr = tmem_base + acc * kGroupedTileRows + ((quarter * 32u) << 16);
             const uint32_t pair_col = tile.n_blk * kGroupedTileCols + cta_rank * kBlockM + (quarter >> 1) * 64u;
             const uint32_t warp_col = pair_col + (quarter & 1u) * 32u;
-            if (pair_col < p.n) {
+            // The accumulator goes back as soon as it is in registers, without a release: the loads are complete, and a release
+            // at cluster scope would wait for the warp's stores.
+            auto hand_back = [&] {
+                ptx::tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    ptx::mbar_arrive_cluster_addr_relaxed(ptx::mapa_shared(acc_empty_bar(acc), 0));
+            };
+            if (pair_col < p.n && turn * 32u < tile.rows) {
 #pragma unroll 1
                 for (uint32_t r = turn * 32u; r < tile.rows; r += 64) {
                     uint32_t v[32];
                     ptx::tmem_ld_32x32b_x32(taddr + r, v);
                     ptx::tmem_ld_wait();
+                    if (r + 64 >= tile.rows)
+                        hand_back();
                     const uint32_t valid = min(32u, tile.rows - r);
                     if (p.c_tma_ok)
                         store_transposed_chunk_tma(p, &tma_c, stage_u32, 1u + share, quarter & 1u, tile.row0 + r, valid, pair_col, lane, v);
@@ -445,11 +455,9 @@ gemm_bf16_sm100_grouped(const __grid_constant__ RowMaps tma_a, const __grid_cons
                         store_transposed_chunk(p, tile.row0 + r, valid, warp_col + lane, lane, v);
                     __syncwarp();
                 }
+            } else {
+                hand_back();
             }
-            ptx::tcgen05_fence_before();
-            __syncwarp();
-            if (lane == 0)
-                ptx::mbar_arrive_cluster_addr(ptx::mapa_shared(acc_empty_bar(acc), 0));
             if (++acc == 2) {
                 acc = 0;
                 acc_phase ^= 1u;

@@ -15,7 +15,7 @@
 //
 // Roles per CTA: TMA producer, MMA issuer (leader only), eight epilogue warps, the fix warp.
 // Bound: tensor pipe where groups have two thousand rows (8 x 2048, 4096 x 4096: 379 us, 1.45 PFLOP/s); below, what a tile costs
-// beside its sum (16 x 512, 4096 x 2048: 134 us, 113 without the stores of DW).
+// beside its sum (16 x 512, 4096 x 2048: 130 to 148 us by where the operands lie, 113 without the stores of DW).
 #pragma once
 #include "gemm_sm100_grouped.cuh"
 
@@ -142,18 +142,19 @@ __device__ __forceinline__ WgradTile wgrad_tile(uint32_t t, uint32_t m_blocks, u
 }
 
 // Drains this warp's 32 x 256 part of the accumulator (or writes zeros) through shared memory and TMA stores of 32 x 64
-// boxes into matrix `z` of the stack; the map clips at N and K.
+// boxes into matrix `z` of the stack; the map clips at N and K.  `loaded` is called once, when the last of it is in registers.
+template <typename Loaded>
 __device__ __forceinline__ void wgrad_drain_tma(const GroupedParams &p, const CUtensorMap *tma_c, uint32_t stage_u32,
                                                 uint32_t taddr, bool zeros, uint32_t lane, uint32_t row0, uint32_t col0,
-                                                uint32_t z, uint32_t turn)
+                                                uint32_t z, uint32_t turn, Loaded loaded)
 {
-    if (row0 >= p.n)
-        return;
+    // groups of 64 columns that K has in this tile, as far as this warp's rows exist
+    const uint32_t groups = row0 >= p.n ? 0u : min(kGroupedTileCols / 64u, (p.k - col0 + 63u) / 64u);
+    if (turn >= groups)
+        loaded();
 #pragma unroll 1
-    for (uint32_t g = turn; g < kGroupedTileCols / 64; g += 2) {
+    for (uint32_t g = turn; g < groups; g += 2) {
         const uint32_t col = col0 + g * 64u;
-        if (col >= p.k)
-            break;
         uint32_t v0[32], v1[32];
         if (zeros) {
 #pragma unroll
@@ -164,6 +165,8 @@ __device__ __forceinline__ void wgrad_drain_tma(const GroupedParams &p, const CU
             ptx::tmem_ld_32x32b_x32(taddr + g * 64u + 32u, v1);
             ptx::tmem_ld_wait();
         }
+        if (g + 2 >= groups)
+            loaded();
         if (lane == 0)
             ptx::bulk_wait_group_read<0>();  // the buffer's last store has read it
         __syncwarp();
@@ -194,9 +197,10 @@ __device__ __forceinline__ void wgrad_drain_tma(const GroupedParams &p, const CU
 
 // The same with plain stores, for a DW whose rows are not 16-byte aligned: lane = row, 2-byte stores that are
 // consecutive across the warp after a transposition through the warp's staging buffer.
+template <typename Loaded>
 __device__ __forceinline__ void wgrad_drain_plain(const GroupedParams &p, uint8_t *stage_warp, uint32_t taddr, bool zeros,
                                                   uint32_t lane, uint32_t row0, uint32_t col0, uint32_t z,
-                                                  uint32_t turn)
+                                                  uint32_t turn, Loaded loaded)
 {
     GemmParams q{};
     q.c = p.c + static_cast<uint64_t>(z) * p.c_stride;
@@ -215,6 +219,8 @@ __device__ __forceinline__ void wgrad_drain_plain(const GroupedParams &p, uint8_
             ptx::tmem_ld_32x32b_x32(taddr + c * 32u, v);
             ptx::tmem_ld_wait();
         }
+        if (c + 2 >= kGroupedTileCols / 32)
+            loaded();
         store_chunk(q, stage_warp, row0, col0 + c * 32u, lane, v);
         __syncwarp();
     }
@@ -445,15 +451,22 @@ gemm_bf16_sm100_grouped_wgrad(const __grid_constant__ CUtensorMap tma_dc, const 
             const uint32_t taddr = tmem_base + acc * kGroupedTileCols + ((quarter * 32u) << 16);
             const uint32_t row0 = tile.m_blk * 2 * kBlockM + cta_rank * kBlockM + quarter * 32u;
             const uint32_t col0 = tile.n_blk * kGroupedTileCols;
-            if (p.c_tma_ok)
-                wgrad_drain_tma(p, &tma_dw, stage_u32, taddr, zeros, lane, row0, col0, tile.group, turn);
-            else
-                wgrad_drain_plain(p, stage_warp, taddr, zeros, lane, row0, col0, tile.group, turn);
-            if (!zeros) {
+            // The accumulator goes back as soon as it is in registers, without a release: the loads are complete, and a release
+            // at cluster scope would wait for the warp's stores, 3300 cycles a
+            // tile (16 uneven groups of 2000 rows in all, 2048 x 2048: 42 -> 33 us; 64 of 8192, 2048 x 1024: 94 -> 75).
+            auto hand_back = [&] {
+                if (zeros)
+                    return;
                 ptx::tcgen05_fence_before();
                 __syncwarp();
                 if (lane == 0)
-                    ptx::mbar_arrive_cluster_addr(ptx::mapa_shared(acc_empty_bar(acc), 0));
+                    ptx::mbar_arrive_cluster_addr_relaxed(ptx::mapa_shared(acc_empty_bar(acc), 0));
+            };
+            if (p.c_tma_ok)
+                wgrad_drain_tma(p, &tma_dw, stage_u32, taddr, zeros, lane, row0, col0, tile.group, turn, hand_back);
+            else
+                wgrad_drain_plain(p, stage_warp, taddr, zeros, lane, row0, col0, tile.group, turn, hand_back);
+            if (!zeros) {
                 if (++acc == 2) {
                     acc = 0;
                     acc_phase ^= 1u;
