@@ -12,8 +12,9 @@
 // and add to 128 fp32 registers per thread; they hand the buffer back as soon as its last column is in registers.
 //
 // Bound: per k-block and SM the MMA needs 512 cycles, the TMEM read 256 (512 bytes a cycle), the fp32 multiply-adds 256
-// issue slots per scheduler: the tensor pipe leads if the hand-over of buffers stays hidden.  8192^3: 493 to 573 us as the part's
-// power allows (1.9 to 2.2 PFLOP/s), 418 with the promotion taken out.
+// issue slots per scheduler.  A block takes about 860: a buffer's round (MMA, commit to both CTAs, 330 cycles to read it out,
+// arrival at the leader) is longer than two blocks' MMAs, and more buffers do not fit.  Without scales, or with half the
+// multiply-adds, it is 3 % faster.  8192^3: 486 to 550 us as the part's power allows (2.0 to 2.3 PFLOP/s).
 #pragma once
 #include "gemm_common.cuh"
 
@@ -22,7 +23,7 @@ namespace maize {
 constexpr uint32_t kF8BlockK = 128;        // e4m3 elements per k-block = one 128-byte swizzle row = one scale
 constexpr uint32_t kF8UmmaK = 32;          // K per tcgen05.mma for 8-bit operands
 constexpr uint32_t kF8PromoteWarps = 8;    // two per quarter of the lanes: columns 0-127 and 128-255
-constexpr uint32_t kF8ControlWarps = 4;    // producer, MMA issuer, two idle: a whole warpgroup, so that it can give registers away
+constexpr uint32_t kF8ControlWarps = 4;    // producer, two MMA issuers, one idle: a whole warpgroup, so that it can give registers away
 constexpr uint32_t kF8Threads = 32 * (kF8ControlWarps + kF8PromoteWarps);
 // 384 threads are launched with 168 registers each (504 over the three warpgroups); the control warpgroup keeps 56, the two
 // promotion warpgroups take 224 each: 56 + 2 * 224 = 504.
@@ -43,7 +44,7 @@ struct F8SmemLayout {
     static constexpr uint32_t kStagingOffset = STAGES * kStageBytes;
     static constexpr uint32_t kStagingBytes = kF8PromoteWarps * kTmaStoreBufBytes;
     static constexpr uint32_t kBarOffset = kStagingOffset + kStagingBytes;
-    static constexpr uint32_t kNumBars = 2 * STAGES + 4;
+    static constexpr uint32_t kNumBars = 2 * STAGES + 6;
     static constexpr uint32_t kTmemSlotOffset = kBarOffset + kNumBars * 8;
     static constexpr uint32_t kAbortOffset = kTmemSlotOffset + 4;
     static constexpr uint32_t kUsedBytes = kAbortOffset + 4;
@@ -179,6 +180,7 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
     auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (STAGES + s); };
     auto acc_full_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + b); };
     auto acc_empty_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + 2 + b); };
+    auto turn_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + 4 + b); };  // the other issuer's MMAs are in the pipe
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem_gen + L::kTmemSlotOffset);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem_gen + L::kAbortOffset);
 
@@ -203,6 +205,7 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
         for (uint32_t b = 0; b < 2; ++b) {
             ptx::mbar_init(acc_full_bar(b), 1);
             ptx::mbar_init(acc_empty_bar(b), 2 * kF8PromoteWarps);  // one lane per promotion warp of both CTAs
+            ptx::mbar_init(turn_bar(b), 1);
         }
         *abort_flag = 0;
         ptx::fence_barrier_init();
@@ -254,37 +257,39 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
             role_ok = ok;
         }
         __syncwarp();
-    } else if (warp == 1) {
-        // ------------------------------------------- MMA issuer (leader only) --
+    } else if (warp == 1 || warp == 2) {
+        // ------------------------------- MMA issuers (leader only), a buffer each --
+        // Blocks of 128 k do not depend on each other: warp 1 issues the even ones, warp 2 the odd ones, and one does its waits and
+        // commits (some 300 cycles a block) while the other's MMAs run (4096^3: 69 -> 66 us, 8192^3: 509 -> 489).  They take
+        // turns: side by side in the pipe two blocks would both end late.
         if (lane == 0 && cta_rank == 0) {
-            uint32_t stage = 0, phase = 0;
-            uint32_t acc = 0, acc_phase = 0;
+            const uint32_t acc = warp - 1u;
+            const uint32_t blocks = pair < num_tiles ? ((num_tiles - pair - 1u) / num_pairs + 1u) * num_kb : 0u;
+            uint32_t stage = acc, phase = 0, acc_phase = 0;
             bool ok = true;
-            for (uint32_t t = pair; ok && t < num_tiles; t += num_pairs) {
-                for (uint32_t kb = 0; kb < num_kb; ++kb) {
-                    ok = wait_bounded<true>(full_bar(stage), phase, ctl, 2) &&
-                         wait_bounded<true>(acc_empty_bar(acc), acc_phase ^ 1u, ctl, 2);
-                    if (!ok)
-                        break;
-                    ptx::tcgen05_fence_after();
-                    const uint32_t sa = smem_base + stage * L::kStageBytes;
-                    const uint64_t da = ptx::make_smem_desc_sw128(sa);
-                    const uint64_t db = ptx::make_smem_desc_sw128(sa + L::kABytes);
-                    const uint32_t tmem_d = tmem_base + acc * 256u;
+            for (uint32_t it = acc; it < blocks; it += 2) {
+                ok = wait_bounded<true>(full_bar(stage), phase, ctl, 2) &&
+                     wait_bounded<true>(acc_empty_bar(acc), acc_phase ^ 1u, ctl, 2) &&
+                     wait_bounded(turn_bar(acc), acc == 0u ? acc_phase ^ 1u : acc_phase, ctl, 2);
+                if (!ok)
+                    break;
+                ptx::tcgen05_fence_after();
+                const uint32_t sa = smem_base + stage * L::kStageBytes;
+                const uint64_t da = ptx::make_smem_desc_sw128(sa);
+                const uint64_t db = ptx::make_smem_desc_sw128(sa + L::kABytes);
+                const uint32_t tmem_d = tmem_base + acc * 256u;
 #pragma unroll
-                    for (uint32_t k = 0; k < kF8BlockK / kF8UmmaK; ++k)
-                        ptx::mma_f8_2cta(tmem_d, da + 2u * k, db + 2u * k, kIdesc, k != 0u ? 1u : 0u);
-                    ptx::mma_commit_2cta_mask(acc_full_bar(acc), 3);
-                    ptx::mma_commit_2cta_mask(empty_bar(stage), 3);
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
-                    if (++acc == 2) {
-                        acc = 0;
-                        acc_phase ^= 1u;
-                    }
+                for (uint32_t k = 0; k < kF8BlockK / kF8UmmaK; ++k)
+                    ptx::mma_f8_2cta(tmem_d, da + 2u * k, db + 2u * k, kIdesc, k != 0u ? 1u : 0u);
+                ptx::mbar_arrive(turn_bar(acc ^ 1u));
+                ptx::mma_commit_2cta_mask(acc_full_bar(acc), 3);
+                ptx::mma_commit_2cta_mask(empty_bar(stage), 3);
+                stage += 2;
+                if (stage >= STAGES) {
+                    stage -= STAGES;
+                    phase ^= 1u;
                 }
+                acc_phase ^= 1u;
             }
             role_ok = ok;
         }

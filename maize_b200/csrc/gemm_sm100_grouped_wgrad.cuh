@@ -15,7 +15,7 @@
 //
 // Roles per CTA: TMA producer, MMA issuer (leader only), eight epilogue warps, the fix warp.
 // Bound: tensor pipe where groups have two thousand rows (8 x 2048, 4096 x 4096: 379 us, 1.45 PFLOP/s); below, what a tile costs
-// beside its sum (16 x 512, 4096 x 2048: 130 to 148 us by where the operands lie, 113 without the stores of DW).
+// beside its sum (16 x 512, 4096 x 2048: 148 us, 113 without the stores of DW).
 #pragma once
 #include "gemm_sm100_grouped.cuh"
 
