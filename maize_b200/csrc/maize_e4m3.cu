@@ -255,8 +255,8 @@ maize_status_t maize_gemm_e4m3(maize_ctx_t *ctx, const void *a, uint64_t lda, co
     if (tiles > 0x7fffffffull)
         return fail(ctx, MAIZE_ERR_UNSUPPORTED, "too many output tiles");
     const uint32_t grid = maize::persistent_grid(ctx, tiles, 2);
-    return maize::launch(ctx, maize::kAttrE4m3, maize::gemm_e4m3_sm100_2cta<6>, grid, maize::kF8Threads,
-                         maize::F8SmemLayout<6>::kDynamicBytes, stream, ta, tb, tc, f);
+    return maize::launch(ctx, maize::kAttrE4m3, maize::gemm_e4m3_sm100_2cta<5>, grid, maize::kF8Threads,
+                         maize::F8SmemLayout<5>::kDynamicBytes, stream, ta, tb, tc, f);
 }
 
 }  // extern "C"
