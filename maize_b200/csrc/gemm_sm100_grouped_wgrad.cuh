@@ -25,7 +25,8 @@ namespace maize {
 constexpr uint32_t kWgradEpilogueWarps = 8;
 constexpr uint32_t kWgradFixWarp = 2 + kWgradEpilogueWarps;
 constexpr uint32_t kWgradThreads = 32 * (kWgradFixWarp + 1);
-// One staging buffer of 32 rows x 64 columns per warp (a second one, at the cost of a ring stage, gained nothing).
+// One staging buffer of 32 rows x 64 columns per warp (a second one, at the cost of a ring stage, lost: 16 uneven groups of 8192
+// rows, 4096 x 2048, 146 us instead of 136).
 constexpr uint32_t kWgradStageWarpBytes = kTmaStoreBufBytes;
 
 template <uint32_t STAGES>
