@@ -56,17 +56,22 @@ def _stream_handle(stream) -> Optional[int]:
 
 _torch = None
 _raw_stream = None
+_empty = None
+_current_device = None
 _devices = ()
 
 
 def _types():
-    """The torch module, imported with the first call that has tensors to look at; with it, torch's name of every device and
-    the shortest way to a device's current stream that this torch has."""
-    global _torch, _raw_stream, _devices
+    """The torch module, imported with the first call that has tensors to look at; with it, torch's name of every device, and the
+    shortest ways that this torch has to a device's current stream and to a new tensor on the current device."""
+    global _torch, _raw_stream, _empty, _current_device, _devices
     if _torch is None:
         import torch
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda device: torch.cuda.current_stream(device).cuda_stream)
+        # sizes, strides, type -> tensor of the current device: 0.75 us, torch.empty takes 1.6
+        _empty = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+        _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
         _devices = tuple(torch.device("cuda", i) for i in range(torch.cuda.device_count()))
         _torch = torch
     return _torch
@@ -283,6 +288,9 @@ class Context:
                 raise MaizeError(_ffi.INVALID_ARG, f"out: expected {' x '.join(map(str, shape))}")
             return out
         if stream is None:
+            if _empty is not None and 0 not in shape and _current_device() == self.device:
+                last = shape[-1]
+                return _empty(shape, (last, 1) if len(shape) == 2 else (shape[1] * last, last, 1), dtype)
             return _torch.empty(*shape, dtype=dtype, device=_devices[self.device])
         if isinstance(stream, int):
             stream = _torch.cuda.ExternalStream(stream, device=self.device)
