@@ -335,6 +335,21 @@ def test_refusals(ctx):
 
 
 @EVERY_KERNEL
+@pytest.mark.parametrize("ctas", [1, 2, 5, 20])
+def test_few_ctas_many_rounds(ctx, ctas, parts):
+    """A limit on the CTAs makes every one of them go through many tiles, with odd and even numbers of k-blocks."""
+    ctx.set("max_ctas", ctas)
+    try:
+        for m, n, k in ((600, 1000, 400), (300, 777, 128), (20, 2000, 1040), (50, 1500, 640), (1030, 520, 256)):
+            a, sa, b, sb = operands(m + n + k, m, n, k)
+            ref, size = plain_product(a, sa, b, sb)
+            close(ctx.gemm_e4m3(a, sa, b, sb), ref, size, k, f"{m} {n} {k}")
+        ctx.poll()
+    finally:
+        ctx.set("max_ctas", 0)
+
+
+@EVERY_KERNEL
 def test_product_past_32_bits(ctx, parts):
     """The last rows of operands and of a result that lie more than 2^32 bytes behind the start."""
     import torch

@@ -140,6 +140,28 @@ def test_sizes_beyond_the_entry_points_range_are_refused(ctx):
     assert ctx._lib.calls == []
 
 
+def test_results_are_allocated_on_the_contexts_device(ctx, monkeypatch):
+    """The short way to a new tensor gives one of the current device: it is taken only where that is the context's."""
+    gemm = sys.modules["maize_b200.gemm"]
+    asked = []
+    monkeypatch.setattr(gemm, "_empty", lambda shape, strides, dtype: asked.append((shape, strides, dtype)))
+    monkeypatch.setattr(gemm, "_current_device", lambda: 1)
+    monkeypatch.setattr(gemm, "_devices", (torch.device("cpu"), torch.device("cpu")))
+    result = maize_b200.Context._result
+    ctx.device = 0
+    assert result(ctx, None, (3, 5), BF16, None).shape == (3, 5) and asked == []
+    ctx.device = 1
+    result(ctx, None, (3, 5), F8, None)
+    result(ctx, None, (2, 3, 5), BF16, None)
+    assert asked == [((3, 5), (5, 1), F8), ((2, 3, 5), (15, 5, 1), BF16)]
+    for shape in ((0, 5), (3, 0), (2, 0, 5)):
+        out = result(ctx, None, shape, BF16, None)
+        assert out.shape == shape and out.is_contiguous()
+    assert len(asked) == 2
+    monkeypatch.setattr(gemm, "_empty", None)
+    assert result(ctx, None, (3, 5), BF16, None).shape == (3, 5)
+
+
 def test_module_functions_refuse_cpu_tensors():
     a = t(4, 16)
     for call in (lambda: maize_b200.grouped_gemm(a, t(1, 8, 16), offs(0, 4)), lambda: maize_b200.quantize_e4m3(a),

@@ -502,6 +502,51 @@ def test_order_of_uneven_groups(ctx, parts, sizes):
 
 
 @EVERY_KERNEL
+@pytest.mark.parametrize("ctas", [1, 2, 5, 20])
+def test_few_ctas_many_rounds(ctx, ctas, parts):
+    """A limit on the CTAs makes every one of them go through many tiles, of rows that differ."""
+    ctx.set("max_ctas", ctas)
+    try:
+        sizes = [70, 0, 1, 300, 33, 64, 129, 5, 0, 31]
+        check_grouped(ctx, sizes, 520, 200, False, seed=55)
+        check_grouped(ctx, sizes, 520, 200, True, seed=56)
+        check_wgrad(ctx, sizes, 520, 200, seed=57)
+    finally:
+        ctx.set("max_ctas", 0)
+
+
+def test_first_calls_of_a_context_inside_a_capture():
+    """What a context finds out with its first call of a kind is found out while a graph is captured, too."""
+    import torch
+    import maize_b200
+    g = gen(58)
+    sizes = [30, 0, 7]
+    o = offsets_of(sizes)
+    x, w, dy = bf16(g, (37, 1024)), bf16(g, (3, 136, 1024), 0.1), bf16(g, (37, 136))
+    usual = maize_b200.Context(0)
+    for parts in (0, 1, 2, 4, 8):
+        usual.set("k_parts", parts)
+        qx, sx = usual.quantize_e4m3(x)
+        qw, sw = usual.quantize_e4m3(w[0], 128)
+        want = (usual.grouped_gemm(x, w, o), usual.grouped_gemm_kn(dy, w, o), usual.grouped_gemm_wgrad(x, dy, o), qx, sx, qw, sw,
+                usual.gemm_e4m3(qx, sx, qw, sw))
+        usual.poll()
+        fresh = maize_b200.Context(0)
+        fresh.set("k_parts", parts)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = (fresh.grouped_gemm(x, w, o), fresh.grouped_gemm_kn(dy, w, o), fresh.grouped_gemm_wgrad(x, dy, o),
+                   *fresh.quantize_e4m3(x), *fresh.quantize_e4m3(w[0], 128), fresh.gemm_e4m3(qx, sx, qw, sw))
+        graph.replay()
+        fresh.poll()
+        for a, b in zip(got, want):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        del graph, got
+        fresh.close()
+    usual.close()
+
+
+@EVERY_KERNEL
 def test_elements_past_32_bits(ctx, parts):
     """Rows of A and C, matrices of B and of DB that lie more than 2^32 bytes behind the start: a group at the very end."""
     import torch
