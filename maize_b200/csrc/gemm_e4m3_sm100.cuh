@@ -12,9 +12,10 @@
 // and add to 128 fp32 registers per thread; they hand the buffer back as soon as its last column is in registers.
 //
 // Bound: per k-block and SM the MMA needs 512 cycles, the TMEM read 256 (512 bytes a cycle), the fp32 multiply-adds 256
-// issue slots per scheduler.  A block takes about 860: a buffer's round (MMA, commit to both CTAs, 330 cycles to read it out,
-// arrival at the leader) is longer than two blocks' MMAs, and more buffers do not fit.  Without scales, or with half the
-// multiply-adds, it is 3 % faster.  8192^3: 486 to 550 us as the part's power allows (2.0 to 2.3 PFLOP/s).
+// issue slots per scheduler.  A block takes about 860 cycles: the two issuers (waits, four MMAs, two commits) and the promotion
+// warps (wait, vote, scales, 330 cycles until the buffer goes back, the rest of the sums) are each that long, latencies and
+// not pipes (FMA 40 % busy), and taking work out of one of them alone gains 3 % or less (three quarters of the scale loads: nothing; half
+// the multiply-adds: 3 %).  8192^3: 486 to 550 us as the part's power allows (2.0 to 2.3 PFLOP/s).
 #pragma once
 #include "gemm_common.cuh"
 
@@ -230,6 +231,8 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
         ptx::grid_dependency_wait();
     }
 
+    // Waits acquire at CTA scope: tensor memory and asynchronous copies come with the barrier's own phase, no thread's stores
+    // do (with cluster scope 4111 x 3967 x 4112 took 81.6 us instead of 77.3, 4096 x 4096 x 7168 110 instead of 108).
     bool role_ok = true;
     if (warp < kF8ControlWarps) {
         ptx::setmaxnreg_dec<kF8ControlRegs>();
@@ -243,7 +246,7 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
                 const int32_t m0 = static_cast<int32_t>(tc.m_blk * 2 * kBlockM + cta_rank * kBlockM);
                 const int32_t n0 = static_cast<int32_t>(tc.n_blk * 256u + cta_rank * 128u);
                 for (uint32_t kb = 0; kb < num_kb; ++kb) {
-                    ok = wait_bounded<true>(empty_bar(stage), phase ^ 1u, ctl, 1);
+                    ok = wait_bounded(empty_bar(stage), phase ^ 1u, ctl, 1);
                     if (!ok)
                         break;
                     const uint32_t sa = smem_base + stage * L::kStageBytes;
@@ -273,8 +276,8 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
             uint32_t stage = acc, phase = 0, acc_phase = 0;
             bool ok = true;
             for (uint32_t it = acc; it < blocks; it += 2) {
-                ok = wait_bounded<true>(full_bar(stage), phase, ctl, 2) &&
-                     wait_bounded<true>(acc_empty_bar(acc), acc_phase ^ 1u, ctl, 2) &&
+                ok = wait_bounded(full_bar(stage), phase, ctl, 2) &&
+                     wait_bounded(acc_empty_bar(acc), acc_phase ^ 1u, ctl, 2) &&
                      wait_bounded(turn_bar(acc), acc == 0u ? acc_phase ^ 1u : acc_phase, ctl, 2);
                 if (!ok)
                     break;
