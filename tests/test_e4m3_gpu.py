@@ -349,6 +349,30 @@ def test_few_ctas_many_rounds(ctx, ctas, parts):
         ctx.set("max_ctas", 0)
 
 
+@pytest.mark.parametrize("parts", [1], indirect=True)
+@pytest.mark.parametrize("k", [16, 128, 272])
+@pytest.mark.parametrize("m,n,ctas", [(1030, 520, 2), (2048, 1032, 4), (1000, 1080, 6), (600, 904, 2), (520, 1856, 2), (4096, 4104, 0),
+                                      (8192, 8200, 0), (8192, 8256, 0)])
+def test_edge_tiles_between_whole_ones(ctx, m, n, ctas, k, parts):
+    """Short sums, so that a tile's stores are still on their way when the next tile's begin; the last columns are half a tile's or
+    less (N % 128 of 8 to 64), so that a warp has one store there and two in the tiles before and after."""
+    import torch
+    a, sa, b, sb = operands(m + n + k, m, n, k)
+    ref, size = plain_product(a, sa, b, sb)
+    ctx.set("max_ctas", ctas)
+    try:
+        first = ctx.gemm_e4m3(a, sa, b, sb)
+        close(first, ref, size, k, f"{m} x {n} x {k}")
+        outs = [torch.empty_like(first) for _ in range(4)]
+        for _ in range(10):
+            for out in outs:
+                ctx.gemm_e4m3(a, sa, b, sb, out=out.fill_(7.0))
+            assert all(torch.equal(out, first) for out in outs)
+        ctx.poll()
+    finally:
+        ctx.set("max_ctas", 0)
+
+
 @EVERY_KERNEL
 def test_product_past_32_bits(ctx, parts):
     """The last rows of operands and of a result that lie more than 2^32 bytes behind the start."""
