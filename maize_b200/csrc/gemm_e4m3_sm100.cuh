@@ -329,14 +329,14 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
             for (int i = 0; i < 64; ++i)
                 acc[i] = 0ull;
             // the scales of the next two k-blocks are on their way behind this one's work
-            float a0 = ptx::ld_f32_nc(sa), b0 = ptx::ld_f32_nc(sb);
+            float a0 = ptx::ld_f32(sa), b0 = ptx::ld_f32(sb);
             const uint32_t last = num_kb - 1;
-            float a1 = ptx::ld_f32_nc(sa + min(1u, last)), b1 = ptx::ld_f32_nc(sb + min(1u, last));
+            float a1 = ptx::ld_f32(sa + min(1u, last)), b1 = ptx::ld_f32(sb + min(1u, last));
             for (uint32_t kb = 0; kb < num_kb; ++kb) {
                 const float s = a0 * b0;
                 a0 = a1, b0 = b1;
-                a1 = ptx::ld_f32_nc(sa + min(kb + 2, last));
-                b1 = ptx::ld_f32_nc(sb + min(kb + 2, last));
+                a1 = ptx::ld_f32(sa + min(kb + 2, last));
+                b1 = ptx::ld_f32(sb + min(kb + 2, last));
                 ok = wait_bounded(acc_full_bar(buf), buf_phase, ctl, 3);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok)

@@ -223,14 +223,14 @@ gemm_e4m3_sm100_skinny(const __grid_constant__ CUtensorMap tma_a, const __grid_c
             float a0 = 0.0f, a1 = 0.0f, x0 = 0.0f, x1 = 0.0f, y0 = 0.0f, y1 = 0.0f;
             if (num_kb > 0) {  // the scales of the next two k-blocks are on their way behind this one's work
                 const uint32_t one = min(1u, last_kb);
-                a0 = ptx::ld_f32_nc(sa), x0 = ptx::ld_f32_nc(sb0), y0 = ptx::ld_f32_nc(sb1);
-                a1 = ptx::ld_f32_nc(sa + one), x1 = ptx::ld_f32_nc(sb0 + one), y1 = ptx::ld_f32_nc(sb1 + one);
+                a0 = ptx::ld_f32(sa), x0 = ptx::ld_f32(sb0), y0 = ptx::ld_f32(sb1);
+                a1 = ptx::ld_f32(sa + one), x1 = ptx::ld_f32(sb0 + one), y1 = ptx::ld_f32(sb1 + one);
             }
             for (uint32_t kb = 0; kb < num_kb; ++kb) {
                 const float s0 = a0 * x0, s1 = a0 * y0;
                 const uint32_t ahead = min(kb + 2, last_kb);
                 a0 = a1, x0 = x1, y0 = y1;
-                a1 = ptx::ld_f32_nc(sa + ahead), x1 = ptx::ld_f32_nc(sb0 + ahead), y1 = ptx::ld_f32_nc(sb1 + ahead);
+                a1 = ptx::ld_f32(sa + ahead), x1 = ptx::ld_f32(sb0 + ahead), y1 = ptx::ld_f32(sb1 + ahead);
                 ok = wait_bounded(acc_full_bar(acc), acc_phase, ctl, 3);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok)

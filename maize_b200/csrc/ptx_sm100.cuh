@@ -569,11 +569,12 @@ __device__ __forceinline__ void fma_f32x2(uint64_t &acc, uint64_t a, uint64_t b)
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
 }
 
-// Read-only load that stays where it is written (the compiler may sink an ordinary one to its use).
-__device__ __forceinline__ float ld_f32_nc(const float *p)
+// Load that stays where it is written (the compiler may sink an ordinary one to its use).  Not by the read-only path: that is for
+// memory which nothing writes while the kernel runs, and a kernel started by launch_dependents runs beside the one before it.
+__device__ __forceinline__ float ld_f32(const float *p)
 {
     float v;
-    asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
     return v;
 }
 

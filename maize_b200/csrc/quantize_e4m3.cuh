@@ -113,13 +113,15 @@ __device__ __forceinline__ uint4 lane_convert(const Sixteen &v, float inverse, b
     return make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
 }
 
-// Elements c .. c+7 of a row of `cols` as four words; those outside [0, cols) are zeros and not read.
+// Elements c .. c+7 of a row of `cols` as four words; those outside [0, cols) are zeros and not read.  Ordinary loads, here and
+// below: the kernel before may still be writing X when this one starts, and the wait for it orders these, but not loads by
+// the read-only path.
 __device__ __forceinline__ uint4 load_elements(const __nv_bfloat16 *row, int32_t c, int32_t cols)
 {
     uint32_t h[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-        h[j] = (c + j >= 0 && c + j < cols) ? __ldg(reinterpret_cast<const uint16_t *>(row + c + j)) : 0u;
+        h[j] = (c + j >= 0 && c + j < cols) ? *reinterpret_cast<const uint16_t *>(row + c + j) : 0u;
     return make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
 }
 
@@ -127,7 +129,7 @@ __device__ __forceinline__ uint4 load_elements(const __nv_bfloat16 *row, int32_t
 __device__ __forceinline__ uint4 load_piece(const __nv_bfloat16 *row, int32_t c, int32_t cols)
 {
     if (c >= 0 && c + 8 <= cols)
-        return __ldg(reinterpret_cast<const uint4 *>(row + c));
+        return *reinterpret_cast<const uint4 *>(row + c);
     if (c + 8 > 0 && c < cols)
         return load_elements(row, c, cols);
     return make_uint4(0u, 0u, 0u, 0u);

@@ -430,6 +430,79 @@ def test_operands_written_by_the_call_before(ctx, m, parts):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("parts", [0, 1, 4], indirect=True)
+@pytest.mark.parametrize("first", ["gemm", "grouped_gemm", "gemm_e4m3"])
+@pytest.mark.parametrize("m,k", [(4, 2048), (64, 1040), (300, 2056)])
+def test_chain_of_products_and_quantisers(ctx, m, k, first, parts):
+    """Product -> quantiser -> product -> quantiser (by rows and by blocks) -> product over the same buffers again and again, eager
+    and from a captured graph: every call reads what the one right before it wrote, at the values that a chain with a
+    synchronisation behind each call gives.  The rounds' sizes differ by powers of two, so that a stale scale shows."""
+    import torch
+    g = gen(82)
+    n, inner, rounds = 1040, 512, 8
+    rand = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    k16 = k // 16 * 16  # of X's columns, what the products by e4m3 take
+    us = [(rand(m, inner) * 2.0 ** (3 * i % 7)).to(torch.bfloat16) for i in range(rounds)]
+    v = rand(k, inner).to(torch.bfloat16)
+    qw, sw = ctx.quantize_e4m3(rand(n, k16).to(torch.bfloat16), 128)
+    qv, sv = ctx.quantize_e4m3(v, 128)
+    qus = [ctx.quantize_e4m3(u) for u in us]
+    offsets = torch.tensor([0, m // 2, m], dtype=torch.int32, device="cuda")
+    stack = torch.stack([v, v.flip(0)])
+    torch.cuda.synchronize()
+    f8, f32 = torch.float8_e4m3fn, torch.float32
+    new = lambda *s, d=torch.bfloat16: torch.zeros(s, dtype=d, device="cuda")  # noqa: E731
+    x, y = new(m, k), new(m, n)
+    qx, sx = new(m, k16, d=f8), new(m, -(-k16 // 128), d=f32)
+    qy, sy, qb, sb = new(m, n, d=f8), new(m, -(-n // 128), d=f32), new(m, n, d=f8), new(-(-m // 128), -(-n // 128), d=f32)
+    held = [new(m, m) for _ in range(rounds)]
+
+    def one(i, wait=lambda: None):
+        if first == "gemm":
+            ctx.gemm(us[i], v, out=x)
+        elif first == "grouped_gemm":
+            ctx.grouped_gemm(us[i], stack, offsets, out=x)
+        else:
+            ctx.gemm_e4m3(*qus[i], qv, sv, out=x)
+        wait()
+        ctx.quantize_e4m3(x[:, :k16], out=qx, scales=sx)
+        wait()
+        ctx.gemm_e4m3(qx, sx, qw, sw, out=y)
+        wait()
+        ctx.quantize_e4m3(y, 128, out=qb, scales=sb)
+        wait()
+        ctx.quantize_e4m3(y, out=qy, scales=sy)
+        wait()
+        ctx.gemm_e4m3(qy, sy, qb, sb, out=held[i])
+        wait()
+        return held[i]
+
+    want = []
+    for i in range(rounds):
+        want.append(one(i, torch.cuda.synchronize).clone())
+        torch.cuda.synchronize()
+    assert len({float(w.float().abs().max()) for w in want}) == rounds
+    right = lambda: all(torch.equal(h, w) for h, w in zip(held, want))  # noqa: E731
+    for _ in range(6):
+        for h in held:
+            h.zero_()
+        for i in range(rounds):
+            one(i)
+        ctx.poll()
+        assert right()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for i in range(rounds):
+            one(i)
+    for _ in range(6):
+        for h in held:
+            h.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert right()
+    ctx.poll()
+
+
 @pytest.mark.parametrize("block_rows", [1, 128])
 @pytest.mark.parametrize("cols", [16_384, 16_391])
 def test_quantize_past_32_bits(ctx, cols, block_rows):

@@ -194,3 +194,13 @@ def test_compiled_calls_agree_with_ctypes():
             getattr(calls, name)(*[0] * (count - 1))
         with pytest.raises(TypeError):
             getattr(calls, name)(*["0"] * count)
+
+
+def test_no_read_only_loads_beside_the_kernel_before():
+    """A kernel launched with programmatic stream serialization runs while the one before it still writes: none of these may
+    read by the read-only path.  The two files that do hold kernels launched in plain stream order."""
+    import re
+    from maize_b200.build import CSRC
+    found = {f.name: len(re.findall(r"\b__ldg\(|ld\.global[.\w:]*\.nc\b", f.read_text())) for f in sorted(CSRC.glob("*.cu*"))}
+    # the pitch-aligning copy, and the pushes of the multi-GPU path
+    assert {name: n for name, n in found.items() if n} == {"gemm_common.cuh": 1, "mc_bcast.cuh": 1}
