@@ -116,11 +116,12 @@ __device__ __forceinline__ void f8_store_rows(const GemmParams &p, uint32_t stag
 }
 
 // Writes this warp's 32 rows x 128 columns of C, held as 128 fp32 per lane (lane = row): through the warp's staging buffers
-// and TMA stores, or f8_store_rows where C's rows are not for TMA.  `buf` alternates with every store there is, not with the
-// halves of a tile: at the right edge of C a tile may have the first half only, and the next tile's first store has to leave
-// the buffer alone that this one still reads.
+// and TMA stores, or f8_store_rows where C's rows are not for TMA.  A buffer for each half.  At the right edge of C a tile may
+// have the first half only, so how many stores lie between two of one buffer is not known: before the first half all of the
+// tile before have read theirs.  They had this tile's sum to do it in (buffers that alternate with every store and a wait for
+// all but the last one: 8192^3 553 us instead of 536).
 __device__ __forceinline__ void f8_store(const GemmParams &p, const CUtensorMap *tma_c, uint32_t stage_u32, uint32_t lane,
-                                         uint32_t row0, uint32_t col0, const uint64_t (&acc)[64], uint32_t &buf)
+                                         uint32_t row0, uint32_t col0, const uint64_t (&acc)[64])
 {
     if (row0 >= p.m)
         return;
@@ -128,11 +129,12 @@ __device__ __forceinline__ void f8_store(const GemmParams &p, const CUtensorMap 
     for (uint32_t g = 0; g < 2; ++g) {
         const uint32_t col = col0 + g * 64u;
         if (col < p.n) {
-            if (p.c_tma_ok && lane == 0)
-                ptx::bulk_wait_group_read<1>();  // the store before last has read this buffer
-            __syncwarp();
-            const uint32_t buffer = stage_u32 + buf * kTmaStoreBufBytes;
-            buf ^= 1u;
+            if (g == 0) {
+                if (p.c_tma_ok && lane == 0)
+                    ptx::bulk_wait_group_read<0>();
+                __syncwarp();
+            }
+            const uint32_t buffer = stage_u32 + g * kTmaStoreBufBytes;
             const uint32_t row = buffer + lane * 128u;
             const uint32_t sw = lane & 7u;
 #pragma unroll
@@ -315,7 +317,6 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
         const uint32_t lane_cols = tmem_base + ((quarter * 32u) << 16) + half * 128u;
         const uint32_t leader_empty0 = ptx::mapa_shared(acc_empty_bar(0), 0);
         uint32_t buf = 0, buf_phase = 0;
-        uint32_t store_buf = 0;  // staging buffer of the next store
         bool ok = true;
         for (uint32_t t = pair; ok && t < num_tiles; t += num_pairs) {
             const TileCoord tc = tile_coord(t, p);
@@ -369,7 +370,7 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
             }
             if (!ok)
                 break;
-            f8_store(p, &tma_c, stage_u32, lane, row0, col0, acc, store_buf);
+            f8_store(p, &tma_c, stage_u32, lane, row0, col0, acc);
             __syncwarp();
         }
         if (p.c_tma_ok)
