@@ -369,9 +369,9 @@ MAIZE_API maize_status_t maize_grouped_gemm_bf16_wgrad(maize_ctx_t *ctx, const v
  *
  * maize_gemm_e4m3: C (M x N bf16) = sum over k-blocks j of a_scales[m][j] * b_scales[n / 128][j] * (the product of the
  * block's elements of A (M x K, e4m3) and B (N x K, e4m3)).  a_scales is M x ceil(K/128), b_scales ceil(N/128) x
- * ceil(K/128), row pitches ld_a_scales and ld_b_scales; any fp32 scales (the product of two should be a normal fp32
- * number).  Sums are fp32, C is rounded once.  K, lda and ldb multiples of 16, A and B 16-byte aligned; C needs 2-byte
- * alignment.
+ * ceil(K/128), row pitches ld_a_scales and ld_b_scales; any fp32 scales, also where the product of two would overflow or
+ * underflow by itself.  Sums are fp32, C is rounded once.  K, lda and ldb multiples of 16, A and B 16-byte aligned; C needs
+ * 2-byte alignment.
  *
  * Neither call uses scratch memory.
  */

@@ -3,8 +3,8 @@
 //     C[m, n] = sum over k-blocks j of  sa[m, j] * sb[n / 128, j] * sum over k in block j of  qa[m, k] * qb[n, k]
 //
 // sa: one fp32 per row of A and k-block; sb: one fp32 per 128 x 128 block of B.  The inner sum is one tensor-core pass over
-// 128 k (four tcgen05.mma.kind::f8f6f4 of 32), the outer one runs in fp32 registers ("promotion"): any scales, no rounding
-// but fp32's until C is rounded to bf16 once.
+// 128 k (four tcgen05.mma.kind::f8f6f4 of 32), the outer one runs in fp32 registers ("promotion"): any scales, also where the
+// product of the two is out of fp32's range (f8_prescale below), no rounding but fp32's until C is rounded to bf16 once.
 //
 // A CTA pair computes a 256 x 256 tile (128 x 256 per CTA).  One k-block of both operands is one 128-byte swizzle row, so
 // the ring looks like the bf16 kernel's with twice the k per byte.  TMEM holds two accumulator buffers of 256 columns, one
@@ -172,6 +172,27 @@ __device__ __forceinline__ void f8_promote(uint64_t (&acc)[PAIRS], int first, co
         ptx::fma_f32x2(acc[first + i], ptx::pack_f32x2(v[2 * i], v[2 * i + 1]), ss);
 }
 
+// The sums of a block are multiplied by the product of its two scales where that is a normal number or one of them is zero.  A
+// product that overflows, or loses bits below 2^-126, says nothing about the sums times both.
+__device__ __forceinline__ bool f8_product_serves(float a, float b, float product)
+{
+    return (fabsf(product) >= 1.17549435e-38f && fabsf(product) <= 3.40282347e38f) || a == 0.0f || b == 0.0f;
+}
+
+// Where it does not serve: v *= the larger scale, and the answer is the smaller one, for f8_promote.  In this order nothing goes
+// out of range that the result does not.  Lanes whose product serves keep v and get the product, so that a row's result does
+// not depend on its neighbours' scales.
+__device__ __forceinline__ float f8_prescale(uint32_t (&v)[32], float a, float b)
+{
+    const float product = a * b;
+    const bool serves = f8_product_serves(a, b, product), a_first = fabsf(a) > fabsf(b);
+    const float larger = serves ? 1.0f : (a_first ? a : b);
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+        v[i] = __float_as_uint(__uint_as_float(v[i]) * larger);
+    return serves ? product : (a_first ? b : a);
+}
+
 template <uint32_t STAGES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kF8Threads, 1)
 gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
@@ -335,22 +356,41 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
             float a1 = ptx::ld_f32(sa + min(1u, last)), b1 = ptx::ld_f32(sb + min(1u, last));
             for (uint32_t kb = 0; kb < num_kb; ++kb) {
                 const float s = a0 * b0;
+                const bool serves = f8_product_serves(a0, b0, s);
                 a0 = a1, b0 = b1;
                 a1 = ptx::ld_f32(sa + min(kb + 2, last));
                 b1 = ptx::ld_f32(sb + min(kb + 2, last));
                 ok = wait_bounded(acc_full_bar(buf), buf_phase, ctl, 3);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok)
-                    break;
-                ptx::tcgen05_fence_after();
                 const uint32_t taddr = lane_cols + buf * 256u;
-                const uint64_t ss = ptx::pack_f32x2(__float_as_uint(s), __float_as_uint(s));
                 // Two loads of 32 columns in flight at a time: a load's latency, not its transfer, is what a warp waits for,
                 // and tcgen05.wait::ld waits for all of them.
                 uint32_t v0[32], v1[32];
-                ptx::tmem_ld_32x32b_x32(taddr, v0);
-                ptx::tmem_ld_32x32b_x32(taddr + 32u, v1);
-                ptx::tmem_ld_wait();
+                uint64_t ss = ptx::pack_f32x2(__float_as_uint(s), __float_as_uint(s));
+                // For scales whose product is out of range.  They are loaded again, so that the usual block holds nothing for them, and the
+                // usual block's first loads stand by themselves, so that it has one branch more than without (8192^3 541 us
+                // instead of 533; two more 545; a second way through the whole block spills and takes up to twice as long).
+                auto prescale = [&] {
+                    const float a = ptx::ld_f32(sa + kb), b = ptx::ld_f32(sb + kb);
+                    const uint32_t rest = __float_as_uint(f8_prescale(v0, a, b));
+                    f8_prescale(v1, a, b);
+                    ss = ptx::pack_f32x2(rest, rest);
+                };
+                const bool usual = __all_sync(0xffffffffu, ok && serves);  // one vote for both
+                if (usual) {
+                    ptx::tcgen05_fence_after();
+                    ptx::tmem_ld_32x32b_x32(taddr, v0);
+                    ptx::tmem_ld_32x32b_x32(taddr + 32u, v1);
+                    ptx::tmem_ld_wait();
+                } else {
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok)
+                        break;
+                    ptx::tcgen05_fence_after();
+                    ptx::tmem_ld_32x32b_x32(taddr, v0);
+                    ptx::tmem_ld_32x32b_x32(taddr + 32u, v1);
+                    ptx::tmem_ld_wait();
+                    prescale();
+                }
                 f8_promote(acc, 0, v0, ss);
                 ptx::tmem_ld_32x32b_x32(taddr + 64u, v0);
                 f8_promote(acc, 16, v1, ss);
@@ -361,6 +401,8 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
                 __syncwarp();
                 if (lane == 0)
                     ptx::mbar_arrive_cluster_addr_relaxed(leader_empty0 + 8u * buf);
+                if (!usual)
+                    prescale();
                 f8_promote(acc, 32, v0, ss);
                 f8_promote(acc, 48, v1, ss);
                 if (++buf == 2) {

@@ -228,18 +228,25 @@ gemm_e4m3_sm100_skinny(const __grid_constant__ CUtensorMap tma_a, const __grid_c
             }
             for (uint32_t kb = 0; kb < num_kb; ++kb) {
                 const float s0 = a0 * x0, s1 = a0 * y0;
+                const bool serve = f8_product_serves(a0, x0, s0) && f8_product_serves(a0, y0, s1);
                 const uint32_t ahead = min(kb + 2, last_kb);
                 a0 = a1, x0 = x1, y0 = y1;
                 a1 = ptx::ld_f32(sa + ahead), x1 = ptx::ld_f32(sb0 + ahead), y1 = ptx::ld_f32(sb1 + ahead);
                 ok = wait_bounded(acc_full_bar(acc), acc_phase, ctl, 3);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok)
-                    break;
+                const bool usual = __all_sync(0xffffffffu, ok && serve);  // one vote for both
+                if (!usual) {
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok)
+                        break;
+                }
                 ptx::tcgen05_fence_after();
                 const uint32_t taddr = lane_addr + acc * L::kTileCols;
-                auto scale = [&](uint32_t c) {
-                    const uint32_t bits = __float_as_uint((second >> c) & 1u ? s1 : s0);
-                    return ptx::pack_f32x2(bits, bits);
+                auto promote = [&](uint32_t c, uint32_t(&v)[32]) {
+                    const bool next = ((second >> c) & 1u) != 0u;
+                    float s = next ? s1 : s0;
+                    if (!usual)
+                        s = f8_prescale(v, ptx::ld_f32(sa + kb), ptx::ld_f32((next ? sb1 : sb0) + kb));
+                    f8_promote<L::kWarpCols / 2>(sum, 16 * c, v, ptx::pack_f32x2(__float_as_uint(s), __float_as_uint(s)));
                 };
                 uint32_t v0[32], v1[32];
                 if (cols > 0) {
@@ -254,10 +261,10 @@ gemm_e4m3_sm100_skinny(const __grid_constant__ CUtensorMap tma_a, const __grid_c
                 if (lane == 0)
                     ptx::mbar_arrive(acc_empty_bar(acc));
                 if (cols > 0) {
-                    f8_promote<L::kWarpCols / 2>(sum, 0, v0, scale(0));
+                    promote(0, v0);
                     if constexpr (kChunks == 2)
                         if (cols > 32)
-                            f8_promote<L::kWarpCols / 2>(sum, 16, v1, scale(1));
+                            promote(1, v1);
                 }
                 if (++acc == L::kBuffers) {
                     acc = 0;

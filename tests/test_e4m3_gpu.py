@@ -232,6 +232,81 @@ def test_extreme_scales(ctx, m, parts):
     close(out, ref, size, k)
 
 
+@EVERY_KERNEL
+@pytest.mark.parametrize("m", [3, 50, 100, 300])
+@pytest.mark.parametrize("kind", ["over", "under", "lost", "mixed"])
+def test_scales_whose_product_is_no_normal_number(ctx, m, kind, parts):
+    """Each pair of scales times a block's sum is in range, their product alone is not: above 2^128, below 2^-149, or between that and
+    2^-126, where it would lose bits.  Beside the tolerance above: half of the smallest bf16 step, 2^-134, and for every block half
+    of the smallest fp32 step."""
+    import torch
+    n, k = 300, 512
+    g = gen(91)
+    f8 = torch.float8_e4m3fn
+    kb = k // 128
+    rand = lambda *s: torch.rand(s, generator=g, device="cuda")  # noqa: E731
+    a, b = (256 + 192 * rand(m, k)).to(f8), (256 + 192 * rand(n, k)).to(f8)
+    sa, sb = 1 + rand(m, kb), 1 + rand(3, kb)
+    if kind == "over":
+        # block 0: sums of 0; block 1: sums of 2^-9 at least, times 2^130
+        a[:, :128] = 0
+        sa[:, 0] *= 2.0 ** 100
+        sb[:, 0] *= 2.0 ** 60
+        a[:, 128:256] = 0
+        b[:, 128:256] = 0
+        a[:, 130:134] = (2.0 ** -9)
+        b[:, 130:134] = (1.0 + rand(n, 4)).to(f8)
+        sa[::2, 1] *= 2.0 ** 125
+        sa[1::2, 1] *= 2.0 ** 5
+        sb[:, 1] *= 2.0 ** 5
+        sb[1, 1] *= 2.0 ** -9
+    elif kind == "under":   # 2^-152 times sums of 2^24
+        sa *= 2.0 ** -100
+        sb *= 2.0 ** -52
+    elif kind == "lost":    # 2^-145: a product of four bits
+        sa *= 2.0 ** -45
+        sb *= 2.0 ** -100
+    else:                   # every other row, and one block of columns; zeros beside them
+        sa[::2] *= 2.0 ** -60
+        sa[1::4] = 0
+        sa[3::4] *= 2.0 ** -40
+        sb[1] *= 2.0 ** -85
+        sb[2, 1] = 0
+        sb[2, 0] = 2.0 ** 127
+    out = ctx.gemm_e4m3(a, sa, b, sb)
+    ctx.poll()
+    ref, size = plain_product(a, sa, b, sb)
+    assert torch.isfinite(out.double()).all()
+    tol = 2.0 ** -8 * ref.abs() + (1 + 2.0 ** -8) * (128 + kb + 2) * 2.0 ** -23 * size + 2.0 ** -134 + 2 * kb * 2.0 ** -150
+    assert ((out.double() - ref).abs() <= tol).all()
+    if parts == 1:  # a row's result does not depend on what stands in the rows beside it
+        assert torch.equal(ctx.gemm_e4m3(a[1:2], sa[1:2], b, sb), out[1:2])
+
+
+@EVERY_KERNEL
+@pytest.mark.parametrize("m", [2, 40, 300])
+def test_infinite_and_nan_scales(ctx, m, parts):
+    """As the formula has it: infinite where a block's sum is not zero, NaN where it is; no other row or column is touched."""
+    import torch
+    n, k = 300, 512
+    f8 = torch.float8_e4m3fn
+    a, b = torch.ones((m, k), device="cuda").to(f8), torch.ones((n, k), device="cuda").to(f8)
+    sa, sb = torch.ones((m, 4), device="cuda"), torch.ones((3, 4), device="cuda")
+    sa[1, 2] = float("inf")
+    sb[1, 3] = float("nan")
+    out = ctx.gemm_e4m3(a, sa, b, sb).float()
+    b.view(torch.uint8)[5, 256:384] = 0
+    zero = ctx.gemm_e4m3(a, sa, b, sb).float()
+    ctx.poll()
+    want = torch.full((m, n), 512.0, device="cuda")
+    want[1] = float("inf")
+    want[:, 128:256] = float("nan")
+    assert same(out, want)
+    want[:, 5] = 384.0
+    want[1, 5] = float("nan")
+    assert same(zero, want)
+
+
 @pytest.mark.parametrize("m", [1, 16, 300])
 def test_quantized_linear_layer(ctx, m):
     """As they are used together: weights quantised once in 128 x 128 blocks, activations row by row, one product; against
