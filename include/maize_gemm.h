@@ -365,7 +365,7 @@ MAIZE_API maize_status_t maize_grouped_gemm_bf16_wgrad(maize_ctx_t *ctx, const v
  * ceil(rows/128) x ceil(cols/128)); the last block of a row or column may be cut short.  The scale is the smallest power
  * of two s >= 2^-126 with max|x| <= 448 s (1 for a block of zeros), so x / s is exact and the one rounding is to e4m3,
  * nearest even.  An element that is not finite becomes NaN and has no part in the maximum.  Any alignment that the element
- * types allow; rows of X that start 16-byte and rows of Q that start 8-byte aligned go faster.
+ * types allow; rows of X that start 16-byte aligned go faster, and with them rows of Q that start 16-byte aligned.
  *
  * maize_gemm_e4m3: C (M x N bf16) = sum over k-blocks j of a_scales[m][j] * b_scales[n / 128][j] * (the product of the
  * block's elements of A (M x K, e4m3) and B (N x K, e4m3)).  a_scales is M x ceil(K/128), b_scales ceil(N/128) x
