@@ -101,17 +101,20 @@ _calls = None
 
 
 def load_calls():
-    """The entry points of ``csrc/calls.c`` as plain callables where that module has been built, else the ctypes ones."""
+    """The entry points of ``csrc/calls.c`` as plain callables where that module has been built and loads, else the ctypes ones."""
     global _calls
     if _calls is None:
         lib = load()
         import importlib.util
         import sysconfig
         path = LIB_PATH.with_name("maize_calls" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+        _calls = lib
         if path.exists():
             spec = importlib.util.spec_from_file_location("maize_calls", path)
-            _calls = importlib.util.module_from_spec(spec)
-            spec.loader.exec_module(_calls)
-        else:
-            _calls = lib
+            try:
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                _calls = module
+            except ImportError:  # not for this Python or this library
+                pass
     return _calls

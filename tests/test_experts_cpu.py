@@ -1,13 +1,14 @@
 """CPU tests of the host side of the grouped and 8-bit calls: what the binding hands to the C entry points, what it refuses
 before it hands anything over, and what the C entry points refuse without a context.  No GPU: the library is replaced by a
 recorder, and the context's "device" is the one torch reports for CPU tensors."""
+import os
 import sys
 
 import pytest
 import torch
 
 import maize_b200
-from maize_b200 import _ffi
+from maize_b200 import _ffi, build
 
 BF16, F8 = torch.bfloat16, torch.float8_e4m3fn
 
@@ -200,7 +201,50 @@ def test_no_read_only_loads_beside_the_kernel_before():
     """A kernel launched with programmatic stream serialization runs while the one before it still writes: none of these may
     read by the read-only path.  The two files that do hold kernels launched in plain stream order."""
     import re
-    from maize_b200.build import CSRC
-    found = {f.name: len(re.findall(r"\b__ldg\(|ld\.global[.\w:]*\.nc\b", f.read_text())) for f in sorted(CSRC.glob("*.cu*"))}
+    found = {f.name: len(re.findall(r"\b__ldg\(|ld\.global[.\w:]*\.nc\b", f.read_text())) for f in sorted(build.CSRC.glob("*.cu*"))}
     # the pitch-aligning copy, and the pushes of the multi-GPU path
     assert {name: n for name, n in found.items() if n} == {"gemm_common.cuh": 1, "mc_bcast.cuh": 1}
+
+
+def compiler(tmp_path, monkeypatch, script):
+    """Puts a C compiler of its own in front, and the callables where it may write them."""
+    cc = tmp_path / "cc"
+    cc.write_text("#!/bin/sh\n" + script)
+    cc.chmod(0o755)
+    monkeypatch.setattr(build, "CALLS_OUT", tmp_path / "calls.so")
+    monkeypatch.setattr(build, "_calls_compiler", lambda: str(cc))
+    monkeypatch.setattr(build, "is_stale", lambda: False)
+    monkeypatch.setattr(build, "find_nvcc", lambda: pytest.fail("the library is not stale"))
+    return build.CALLS_OUT
+
+
+WRITES_ITS_OUTPUT = 'while [ "$1" != -o ]; do shift; done; echo x > "$2"\n'
+
+
+def test_a_failing_c_compiler_does_not_stop_the_build(tmp_path, monkeypatch, capsys):
+    out = compiler(tmp_path, monkeypatch, "echo no such symbol >&2; exit 1\n")
+    out.write_text("of an earlier build")
+    os.utime(out, (1, 1))
+    assert build.build() == build.OUT
+    assert not out.exists()  # what the old callables were built for is gone
+    err = capsys.readouterr().err
+    assert "no such symbol" in err and "ctypes" in err
+
+
+def test_missing_and_old_callables_are_built(tmp_path, monkeypatch):
+    out = compiler(tmp_path, monkeypatch, WRITES_ITS_OUTPUT)
+    assert build.calls_are_stale()
+    build.build()
+    assert out.exists() and not build.calls_are_stale()
+    os.utime(out, (1, 1))
+    assert build.calls_are_stale()
+    monkeypatch.setattr(build, "_calls_compiler", lambda: None)
+    assert not build.calls_are_stale()  # nothing can be built here: the library alone is up to date
+
+
+def test_callables_that_do_not_load_leave_ctypes(tmp_path, monkeypatch):
+    lib = _ffi.load()
+    monkeypatch.setattr(_ffi, "LIB_PATH", tmp_path / "libmaize_gemm.so")
+    monkeypatch.setattr(_ffi, "_calls", None)
+    (tmp_path / build.CALLS_OUT.name).write_text("not a module")
+    assert _ffi.load_calls() is lib
