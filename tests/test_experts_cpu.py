@@ -163,6 +163,28 @@ def test_results_are_allocated_on_the_contexts_device(ctx, monkeypatch):
     assert result(ctx, None, (3, 5), BF16, None).shape == (3, 5)
 
 
+@pytest.mark.parametrize("fault", ["signature", "shape", "strides", "dtype", "none"])
+def test_an_undocumented_allocation_is_tried_before_it_is_used(ctx, monkeypatch, fault):
+    """A torch that keeps the name of the short way to a new tensor but not what it does: results come by torch.empty."""
+    gemm = sys.modules["maize_b200.gemm"]
+    asked = []
+
+    def other(shape, strides, dtype):
+        asked.append(shape)
+        if fault == "signature":
+            raise TypeError("takes 2 positional arguments but 3 were given")
+        shape, strides = ((5, 3), (3, 1)) if fault == "shape" else (shape, (1, shape[0]) if fault == "strides" else strides)
+        return torch.empty_strided(shape, strides, dtype=torch.float32 if fault == "dtype" else dtype)
+
+    monkeypatch.setattr(gemm, "_empty", gemm._on_trial(other))
+    monkeypatch.setattr(gemm, "_current_device", lambda: -1)  # as CPU tensors have it
+    monkeypatch.setattr(gemm, "_devices", (torch.device("cpu"),))
+    for _ in range(3):
+        out = maize_b200.Context._result(ctx, None, (3, 5), BF16, None)
+        assert out.shape == (3, 5) and out.is_contiguous() and out.dtype is BF16
+    assert len(asked) == (3 if fault == "none" else 1) and gemm._empty is (other if fault == "none" else None)
+
+
 def test_module_functions_refuse_cpu_tensors():
     a = t(4, 16)
     for call in (lambda: maize_b200.grouped_gemm(a, t(1, 8, 16), offs(0, 4)), lambda: maize_b200.quantize_e4m3(a),
