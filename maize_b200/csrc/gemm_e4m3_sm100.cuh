@@ -262,73 +262,73 @@ gemm_e4m3_sm100_2cta(const __grid_constant__ CUtensorMap tma_a, const __grid_con
     bool role_ok = true;
     if (warp < kF8ControlWarps) {
         ptx::setmaxnreg_dec<kF8ControlRegs>();
-    if (warp == 0) {
-        // ------------------------------------------------------- TMA producer --
-        if (lane == 0) {
-            uint32_t stage = 0, phase = 0;
-            bool ok = true;
-            for (uint32_t t = pair; ok && t < num_tiles; t += num_pairs) {
-                const TileCoord tc = tile_coord(t, p);
-                const int32_t m0 = static_cast<int32_t>(tc.m_blk * 2 * kBlockM + cta_rank * kBlockM);
-                const int32_t n0 = static_cast<int32_t>(tc.n_blk * 256u + cta_rank * 128u);
-                for (uint32_t kb = 0; kb < num_kb; ++kb) {
-                    ok = wait_bounded(empty_bar(stage), phase ^ 1u, ctl, 1);
-                    if (!ok)
-                        break;
-                    const uint32_t sa = smem_base + stage * L::kStageBytes;
-                    const uint32_t leader_full = ptx::mapa_shared(full_bar(stage), 0);
-                    if (cta_rank == 0)
-                        ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * L::kStageBytes);
-                    const int32_t kx = static_cast<int32_t>(kb * kF8BlockK);
-                    ptx::tma_load_2d_pair(sa, &tma_a, leader_full, kx, m0);
-                    ptx::tma_load_2d_pair(sa + L::kABytes, &tma_b, leader_full, kx, n0);
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
+        if (warp == 0) {
+            // ------------------------------------------------------- TMA producer --
+            if (lane == 0) {
+                uint32_t stage = 0, phase = 0;
+                bool ok = true;
+                for (uint32_t t = pair; ok && t < num_tiles; t += num_pairs) {
+                    const TileCoord tc = tile_coord(t, p);
+                    const int32_t m0 = static_cast<int32_t>(tc.m_blk * 2 * kBlockM + cta_rank * kBlockM);
+                    const int32_t n0 = static_cast<int32_t>(tc.n_blk * 256u + cta_rank * 128u);
+                    for (uint32_t kb = 0; kb < num_kb; ++kb) {
+                        ok = wait_bounded(empty_bar(stage), phase ^ 1u, ctl, 1);
+                        if (!ok)
+                            break;
+                        const uint32_t sa = smem_base + stage * L::kStageBytes;
+                        const uint32_t leader_full = ptx::mapa_shared(full_bar(stage), 0);
+                        if (cta_rank == 0)
+                            ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * L::kStageBytes);
+                        const int32_t kx = static_cast<int32_t>(kb * kF8BlockK);
+                        ptx::tma_load_2d_pair(sa, &tma_a, leader_full, kx, m0);
+                        ptx::tma_load_2d_pair(sa + L::kABytes, &tma_b, leader_full, kx, n0);
+                        if (++stage == STAGES) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
                     }
                 }
+                role_ok = ok;
             }
-            role_ok = ok;
-        }
-        __syncwarp();
-    } else if (warp == 1 || warp == 2) {
-        // ------------------------------- MMA issuers (leader only), a buffer each --
-        // Blocks of 128 k do not depend on each other: warp 1 issues the even ones, warp 2 the odd ones, and one does its waits and
-        // commits (some 300 cycles a block) while the other's MMAs run (4096^3: 69 -> 66 us, 8192^3: 509 -> 489).  They take
-        // turns: side by side in the pipe two blocks would both end late.
-        if (lane == 0 && cta_rank == 0) {
-            const uint32_t acc = warp - 1u;
-            const uint32_t blocks = pair < num_tiles ? ((num_tiles - pair - 1u) / num_pairs + 1u) * num_kb : 0u;
-            uint32_t stage = acc, phase = 0, acc_phase = 0;
-            bool ok = true;
-            for (uint32_t it = acc; it < blocks; it += 2) {
-                ok = wait_bounded(full_bar(stage), phase, ctl, 2) &&
-                     wait_bounded(acc_empty_bar(acc), acc_phase ^ 1u, ctl, 2) &&
-                     wait_bounded(turn_bar(acc), acc == 0u ? acc_phase ^ 1u : acc_phase, ctl, 2);
-                if (!ok)
-                    break;
-                ptx::tcgen05_fence_after();
-                const uint32_t sa = smem_base + stage * L::kStageBytes;
-                const uint64_t da = ptx::make_smem_desc_sw128(sa);
-                const uint64_t db = ptx::make_smem_desc_sw128(sa + L::kABytes);
-                const uint32_t tmem_d = tmem_base + acc * 256u;
-#pragma unroll
-                for (uint32_t k = 0; k < kF8BlockK / kF8UmmaK; ++k)
-                    ptx::mma_f8_2cta(tmem_d, da + 2u * k, db + 2u * k, kIdesc, k != 0u ? 1u : 0u);
-                ptx::mbar_arrive(turn_bar(acc ^ 1u));
-                ptx::mma_commit_2cta_mask(acc_full_bar(acc), 3);
-                ptx::mma_commit_2cta_mask(empty_bar(stage), 3);
-                stage += 2;
-                if (stage >= STAGES) {
-                    stage -= STAGES;
-                    phase ^= 1u;
+            __syncwarp();
+        } else if (warp == 1 || warp == 2) {
+            // ------------------------------- MMA issuers (leader only), a buffer each --
+            // Blocks of 128 k do not depend on each other: warp 1 issues the even ones, warp 2 the odd ones, and one does its waits and
+            // commits (some 300 cycles a block) while the other's MMAs run (4096^3: 69 -> 66 us, 8192^3: 509 -> 489).  They take
+            // turns: side by side in the pipe two blocks would both end late.
+            if (lane == 0 && cta_rank == 0) {
+                const uint32_t acc = warp - 1u;
+                const uint32_t blocks = pair < num_tiles ? ((num_tiles - pair - 1u) / num_pairs + 1u) * num_kb : 0u;
+                uint32_t stage = acc, phase = 0, acc_phase = 0;
+                bool ok = true;
+                for (uint32_t it = acc; it < blocks; it += 2) {
+                    ok = wait_bounded(full_bar(stage), phase, ctl, 2) &&
+                         wait_bounded(acc_empty_bar(acc), acc_phase ^ 1u, ctl, 2) &&
+                         wait_bounded(turn_bar(acc), acc == 0u ? acc_phase ^ 1u : acc_phase, ctl, 2);
+                    if (!ok)
+                        break;
+                    ptx::tcgen05_fence_after();
+                    const uint32_t sa = smem_base + stage * L::kStageBytes;
+                    const uint64_t da = ptx::make_smem_desc_sw128(sa);
+                    const uint64_t db = ptx::make_smem_desc_sw128(sa + L::kABytes);
+                    const uint32_t tmem_d = tmem_base + acc * 256u;
+    #pragma unroll
+                    for (uint32_t k = 0; k < kF8BlockK / kF8UmmaK; ++k)
+                        ptx::mma_f8_2cta(tmem_d, da + 2u * k, db + 2u * k, kIdesc, k != 0u ? 1u : 0u);
+                    ptx::mbar_arrive(turn_bar(acc ^ 1u));
+                    ptx::mma_commit_2cta_mask(acc_full_bar(acc), 3);
+                    ptx::mma_commit_2cta_mask(empty_bar(stage), 3);
+                    stage += 2;
+                    if (stage >= STAGES) {
+                        stage -= STAGES;
+                        phase ^= 1u;
+                    }
+                    acc_phase ^= 1u;
                 }
-                acc_phase ^= 1u;
+                role_ok = ok;
             }
-            role_ok = ok;
+            __syncwarp();
         }
-        __syncwarp();
-    }
     } else {
         ptx::setmaxnreg_inc<kF8PromoteRegs>();
         // ---------------------------------------------- promotion and epilogue --
