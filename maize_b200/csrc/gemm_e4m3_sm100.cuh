@@ -15,7 +15,7 @@
 // issue slots per scheduler.  A block takes about 860 cycles: the two issuers (waits, four MMAs, two commits) and the promotion
 // warps (wait, vote, scales, 330 cycles until the buffer goes back, the rest of the sums) are each that long, latencies and
 // not pipes (FMA 40 % busy), and taking work out of one of them alone gains 3 % or less (three quarters of the scale loads: nothing; half
-// the multiply-adds: 3 %).  8192^3: 486 to 550 us as the part's power allows (2.0 to 2.3 PFLOP/s).
+// the multiply-adds: 3 %).  8192^3: 478 to 558 us as the part's power allows (2.0 to 2.3 PFLOP/s).
 #pragma once
 #include "gemm_common.cuh"
 

@@ -14,6 +14,9 @@
 // shared memory; each adds its share in the order of the parts, rounds once and stores.  No global scratch, a fixed order.
 // (Eight parts lost more in the exchange and in clusters that do not fit beside each other than they gained.)
 //
+// The kernels with one or two copies need more than the 168 registers that ten warps leave them and spill 236 to 244 bytes; those with
+// four take 148.
+//
 // The host picks the tile's width so that the tiles fill whole rounds of clusters (16384 rows over 74 pairs: one round of
 // 224).  The columns of a warp lie in at most two scale blocks of B, each chunk of 32 in one.
 #pragma once

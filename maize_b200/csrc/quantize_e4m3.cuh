@@ -7,7 +7,7 @@
 // three mantissa bits at any magnitude down to 2^-6, 14 binades below the largest.
 //
 // Bound: HBM; 2 bytes read and 1 written per element.  A block's elements stay in registers between the maximum and the
-// conversion, so the input is read once.  8192 x 8192: 32.4 us either way, 6.2 TB/s.
+// conversion, so the input is read once.  8192 x 8192: 32.4 us by rows, 32.6 by blocks, 6.2 TB/s.
 #pragma once
 #include "gemm_common.cuh"
 

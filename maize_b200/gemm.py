@@ -451,6 +451,7 @@ _default_ctx = {}
 
 
 def default_context(device: Optional[int] = None) -> Context:
+    """The cached Context of a device, which the module's functions use: for one host thread at a time, like any Context."""
     import torch
     if device is None:
         device = torch.cuda.current_device()
